@@ -24,6 +24,7 @@ LAYOUT_DTYPE_CODES = {
     torch.float16: 5, torch.bfloat16: 6, torch.float32: 7, torch.float64: 8,
 }
 DATA_DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+EIGHT_BIT_DTYPE_CODES = {torch.float8_e4m3fn: 3, torch.float8_e5m2: 4}
 
 # name -> (restype, argtypes); must list every symbol the header declares
 SIGNATURES = {
@@ -76,6 +77,17 @@ SIGNATURES = {
     "bsp_bias_add": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p]),
     "bsp_bias_grad": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p]),
     "bsp_sum_chunks": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "bsp_grouped_max_groups": (c_int, []),
+    "bsp_grouped_matmul": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_int64,
+                                   c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p]),
+    "bsp_grouped_weight_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64,
+                                        c_int64, c_void_p, c_int, c_void_p, c_void_p]),
+    "bsp_grouped_matmul_scaled": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                          c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64,
+                                          c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p]),
+    "bsp_quantize_rows": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p]),
+    "bsp_quantize_blocks": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_int,
+                                    c_void_p, c_void_p]),
     "bsp_selftest_wait_limit": (c_int, [ctypes.c_uint32, c_void_p, c_void_p]),
     "bsp_transpose_blocks": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p]),
 }

@@ -1,0 +1,269 @@
+"""Matrix products grouped by expert, in 16 bits with gradients and in 8 bits with block scales.
+
+The rows of ``x`` are sorted by group; ``group_offsets`` (on the device) says where each group's rows begin and end.
+A layer of experts is a block-sparse product whose row blocks have any height: where ``matmul`` takes a layout of
+equal blocks, the functions here take the group bounds, so no row is padded to a block and no layout is rebuilt when
+the router sends the next batch elsewhere.  The group bounds are never read back to the host; all calls can be
+recorded into a CUDA graph and replayed with other bounds in the same tensor.
+
+No counterpart in the blksprs library.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from .. import _cabi
+from ..plan import status_word
+from ..utils.tools import cast_for_autocast, plain_dispatch
+from ..utils.validation import contiguous_enabled, validate_device, validate_dimensions, validation_enabled
+
+_16_BIT = (torch.float16, torch.bfloat16)
+_OUT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+SCALE_BLOCK = 128
+MAX_GROUPS = 1024
+
+
+def _copied(t: Tensor) -> Tensor:
+    if not contiguous_enabled():
+        raise ValueError("Tensor must be contiguous")
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _row_operand(t: Tensor) -> tuple[Tensor, int]:
+    """``t`` (rows, width) and its row stride as the kernels read it: contiguous rows that start on 16-byte
+    boundaries, any stride between them; a copy where ``t`` is not like that."""
+    rows, width = t.shape
+    vector = 16 // t.element_size()
+    if t.stride(1) == 1 and t.data_ptr() % 16 == 0:
+        if rows == 1:
+            return t, width
+        ld = t.stride(0)
+        if ld >= width and ld % vector == 0:
+            return t, ld
+    return _copied(t), width
+
+
+def _weight_operand(w: Tensor, columns_inner: bool = True) -> tuple[Tensor, int, int, bool]:
+    """``w`` (groups, depth, columns), group stride, stride of the outer of the two matrix dimensions and whether
+    the columns are the inner one.  Both storage orders are read in place; anything else is copied.
+    ``columns_inner`` = False: only the depth may be the inner dimension (8-bit operands)."""
+    groups, depth, cols = w.shape
+    vector = 16 // w.element_size()
+    sg, sk, sn = w.stride()
+    if w.data_ptr() % 16 == 0 and (groups == 1 or (sg >= vector and sg % vector == 0)):
+        if groups == 1:
+            sg = depth * cols
+        if columns_inner and sn == 1 and sk >= cols and sk % vector == 0:
+            return w, sg, sk, True
+        if sk == 1 and sn >= depth and sn % vector == 0:
+            return w, sg, sn, False
+    if columns_inner:
+        return _copied(w), depth * cols, cols, True
+    return _copied(w.transpose(1, 2)).transpose(1, 2), depth * cols, depth, False
+
+
+def _validate_groups(x: Tensor, w: Tensor, group_offsets: Tensor, vector: int) -> None:
+    if group_offsets.dtype not in (torch.int32, torch.int64):
+        raise ValueError("Group offsets must have either int32 or int64 dtype")
+    if group_offsets.dim() != 1 or group_offsets.size(0) != w.size(0) + 1:
+        raise ValueError("Group offsets must have one entry more than there are groups")
+    if not group_offsets.is_contiguous():
+        raise ValueError("Tensor must be contiguous")
+    if x.size(1) != w.size(1):
+        raise ValueError("Inner dimensions of tensors must match")
+    if w.size(0) > MAX_GROUPS:
+        raise ValueError(f"Number of groups must be at most {MAX_GROUPS}")
+    if x.size(1) % vector or w.size(2) % 8:
+        raise ValueError(f"Inner dimension must be divisible by {vector} and columns by 8")
+
+
+def _validate(x: Tensor, w: Tensor, group_offsets: Tensor) -> None:
+    if not validation_enabled():
+        return
+    validate_dimensions(x, dims=2)
+    validate_dimensions(w)
+    if x.dtype not in _16_BIT:
+        raise ValueError("Tensor must have either float16 or bfloat16 dtype")
+    if w.dtype != x.dtype:
+        raise ValueError("Tensors must have same dtype")
+    _validate_groups(x, w, group_offsets, 8)
+    validate_device(x, w, group_offsets)
+
+
+def _rows_product(x: Tensor, w: Tensor, group_offsets: Tensor) -> Tensor:
+    """``out[t] = x[t] @ w[group of t]``, zero for rows of no group."""
+    rows, depth = x.shape
+    groups, _, cols = w.shape
+    if rows == 0 or cols == 0 or depth == 0 or groups == 0:
+        return torch.zeros((rows, cols), dtype=x.dtype, device=x.device)
+    x, ld_x = _row_operand(x)
+    w, group_stride, ld_w, columns_inner = _weight_operand(w)
+    device = x.device
+    with _cabi.device_guard(device):
+        out = torch.empty((rows, cols), dtype=x.dtype, device=device)
+        _cabi.check(_cabi.lib().bsp_grouped_matmul(
+            x.data_ptr(), ld_x, w.data_ptr(), group_stride, ld_w, columns_inner, group_offsets.data_ptr(),
+            group_offsets.dtype == torch.int64, rows, groups, depth, cols, out.data_ptr(),
+            _cabi.DATA_DTYPE_CODES[x.dtype], status_word(device).data_ptr(), _cabi.stream_handle(device)),
+            "bsp_grouped_matmul")
+    return out
+
+
+def _weight_gradient(x: Tensor, grad: Tensor, group_offsets: Tensor, groups: int) -> Tensor:
+    """``out[e] = x[rows of e]^T @ grad[rows of e]``, zero for groups without rows."""
+    rows, depth = x.shape
+    cols = grad.size(1)
+    if rows == 0 or cols == 0 or depth == 0 or groups == 0:
+        return torch.zeros((groups, depth, cols), dtype=x.dtype, device=x.device)
+    x, ld_x = _row_operand(x)
+    grad, ld_grad = _row_operand(grad)
+    device = x.device
+    with _cabi.device_guard(device):
+        out = torch.empty((groups, depth, cols), dtype=x.dtype, device=device)
+        _cabi.check(_cabi.lib().bsp_grouped_weight_grad(
+            x.data_ptr(), ld_x, grad.data_ptr(), ld_grad, group_offsets.data_ptr(),
+            group_offsets.dtype == torch.int64, rows, groups, depth, cols, out.data_ptr(),
+            _cabi.DATA_DTYPE_CODES[x.dtype], status_word(device).data_ptr(), _cabi.stream_handle(device)),
+            "bsp_grouped_weight_grad")
+    return out
+
+
+class _GroupedMatmul(torch.autograd.Function):
+    """Differentiable in ``x`` and ``w``: dX = dO W^T (the same rows product), dW = X^T dO by group."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, w: Tensor, group_offsets: Tensor):
+        ctx.save_for_backward(x, w, group_offsets)
+        return _rows_product(x, w, group_offsets)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    @plain_dispatch
+    def backward(ctx, grad_output: Tensor):
+        x, w, group_offsets = ctx.saved_tensors
+        if grad_output.dtype != x.dtype:
+            grad_output = grad_output.to(x.dtype)
+        grad_x = grad_w = None
+        if ctx.needs_input_grad[0]:
+            grad_x = _rows_product(grad_output, w.transpose(1, 2), group_offsets)
+        if ctx.needs_input_grad[1]:
+            if w.stride(1) == 1 and w.stride(2) != 1:
+                # weights stored with the depth innermost get their gradient in the same order
+                grad_w = _weight_gradient(grad_output, x, group_offsets, w.size(0)).transpose(1, 2)
+            else:
+                grad_w = _weight_gradient(x, grad_output, group_offsets, w.size(0))
+        return grad_x, grad_w, None
+
+
+@plain_dispatch
+def _grouped_matmul_eager(x, w, group_offsets):
+    x, w = cast_for_autocast(x, w)
+    _validate(x, w, group_offsets)
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        return _GroupedMatmul.apply(x, w, group_offsets)
+    return _rows_product(x, w, group_offsets)
+
+
+_grouped_matmul_no_compile = torch.compiler.disable(_grouped_matmul_eager)
+
+
+@torch.amp.custom_fwd(device_type="cuda")
+def grouped_matmul(x: Tensor, w: Tensor, group_offsets: Tensor) -> Tensor:
+    """Multiplies the rows of every group with that group's matrix.
+
+    ``out[t] = x[t] @ w[e]`` for ``group_offsets[e] <= t < group_offsets[e + 1]``; rows of no group (before the
+    first offset, behind the last) are zero, and so are their gradients and the gradient of a group without rows.
+    Sums run in float32 and are rounded once.
+
+    Args:
+        x (Tensor): The rows ``(T, K)``, sorted by group, float16 or bfloat16. ``K`` is a multiple of 8.
+        w (Tensor): One matrix per group ``(E, K, N)``, same dtype, ``E <= 1024``, ``N`` a multiple of 8. Either of
+            the last two dimensions may be the contiguous one (``linear_weights.transpose(1, 2)`` is not copied).
+        group_offsets (Tensor): int32 or int64 ``(E + 1,)`` on the device, non-decreasing, within ``0 .. T``. The
+            values are not read by the host: ones that break this are clamped on the device and reported by
+            ``plan.check_device_status``.
+
+    Returns:
+        Tensor: The products ``(T, N)``.
+    """
+    impl = _grouped_matmul_no_compile if torch.compiler.is_compiling() else _grouped_matmul_eager
+    return impl(x, w, group_offsets)
+
+
+def _blocks_of(size: int) -> int:
+    return -(-size // SCALE_BLOCK)
+
+
+def _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype) -> None:
+    if out_dtype not in _OUT_DTYPES:
+        raise ValueError("Output dtype must be float16, bfloat16, or float32")
+    if not validation_enabled():
+        return
+    validate_dimensions(x, scale_x, dims=2)
+    validate_dimensions(w, scale_w)
+    for t in (x, w):
+        if t.dtype not in _cabi.EIGHT_BIT_DTYPE_CODES:
+            raise ValueError("Tensor must have either float8_e4m3fn or float8_e5m2 dtype")
+    for t in (scale_x, scale_w):
+        if t.dtype != torch.float32:
+            raise ValueError("Tensor must have float32 dtype")
+    _validate_groups(x, w, group_offsets, 16)
+    if tuple(scale_x.shape) != (x.size(0), _blocks_of(x.size(1))):
+        raise ValueError(f"Scale shape {tuple(scale_x.shape)} doesn't match expected "
+                         f"{(x.size(0), _blocks_of(x.size(1)))}")
+    expected = (w.size(0), _blocks_of(w.size(1)), _blocks_of(w.size(2)))
+    if tuple(scale_w.shape) != expected:
+        raise ValueError(f"Scale shape {tuple(scale_w.shape)} doesn't match expected {expected}")
+    if torch.is_grad_enabled() and (scale_x.requires_grad or scale_w.requires_grad or x.requires_grad
+                                    or w.requires_grad):
+        raise ValueError("The scaled product has no gradient")
+    validate_device(x, scale_x, w, scale_w, group_offsets)
+
+
+@plain_dispatch
+def _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtype):
+    _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype)
+    rows, depth = x.shape
+    groups, _, cols = w.shape
+    if rows == 0 or cols == 0 or depth == 0 or groups == 0:
+        return torch.zeros((rows, cols), dtype=out_dtype, device=x.device)
+    x, ld_x = _row_operand(x)
+    w, group_stride, ld_w, _ = _weight_operand(w, columns_inner=False)
+    device = x.device
+    with _cabi.device_guard(device):
+        out = torch.empty((rows, cols), dtype=out_dtype, device=device)
+        _cabi.check(_cabi.lib().bsp_grouped_matmul_scaled(
+            x.data_ptr(), ld_x, _cabi.EIGHT_BIT_DTYPE_CODES[x.dtype], scale_x.data_ptr(), *scale_x.stride(),
+            w.data_ptr(), group_stride, ld_w, _cabi.EIGHT_BIT_DTYPE_CODES[w.dtype], scale_w.data_ptr(),
+            *scale_w.stride(), group_offsets.data_ptr(), group_offsets.dtype == torch.int64, rows, groups, depth,
+            cols, out.data_ptr(), _cabi.DATA_DTYPE_CODES[out_dtype], status_word(device).data_ptr(),
+            _cabi.stream_handle(device)), "bsp_grouped_matmul_scaled")
+    return out
+
+
+_grouped_matmul_scaled_no_compile = torch.compiler.disable(_grouped_matmul_scaled_eager)
+
+
+def grouped_matmul_scaled(x: Tensor, scale_x: Tensor, w: Tensor, scale_w: Tensor, group_offsets: Tensor,
+                          out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """:func:`grouped_matmul` of 8-bit operands that carry a scale for each block of 128.
+
+    ``out[t, n] = sum over b of scale_x[t, b] * scale_w[e, b, n // 128] * (x[t, block b] . w[e, block b, n])``, the
+    operands :func:`quantize_rows` and :func:`quantize_blocks` make. One group (``group_offsets = [0, T]``) is a
+    linear layer. Every sum is float32, the result is rounded once. No gradient.
+
+    Args:
+        x (Tensor): The rows ``(T, K)``, sorted by group, float8_e4m3fn or float8_e5m2. ``K`` is a multiple of 16.
+        scale_x (Tensor): float32 ``(T, ceil(K / 128))``, any strides.
+        w (Tensor): One matrix per group ``(E, K, N)`` of either 8-bit type, ``N`` a multiple of 8, with ``K``
+            contiguous (the order ``quantize_blocks`` returns); any other order is copied on every call.
+        scale_w (Tensor): float32 ``(E, ceil(K / 128), ceil(N / 128))``, any strides.
+        group_offsets (Tensor): As in :func:`grouped_matmul`.
+        out_dtype (torch.dtype): float16, bfloat16 (default) or float32.
+
+    Returns:
+        Tensor: The products ``(T, N)``; rows of no group are zero.
+    """
+    impl = _grouped_matmul_scaled_no_compile if torch.compiler.is_compiling() else _grouped_matmul_scaled_eager
+    return impl(x, scale_x, w, scale_w, group_offsets, out_dtype)

@@ -1,0 +1,94 @@
+"""8-bit values with a scale for each block of 128: the operands of ``grouped_matmul_scaled``.
+
+``scale = max(largest magnitude of the block / largest value of the type, 2**-126)``, ``q = value / scale`` rounded
+to nearest even.  A block that holds an infinity or a NaN has a scale that is not finite and multiplies out to NaN;
+other blocks are not touched by it.  No counterpart in the blksprs library.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from .. import _cabi
+from ..utils.tools import plain_dispatch
+from ..utils.validation import contiguous_enabled, validate_device, validate_dimensions, validation_enabled
+
+SCALE_BLOCK = 128
+
+
+def _validate(t: Tensor, dtype: torch.dtype, dims: int) -> None:
+    if dtype not in _cabi.EIGHT_BIT_DTYPE_CODES:
+        raise ValueError("Output dtype must be float8_e4m3fn or float8_e5m2")
+    if not validation_enabled():
+        return
+    validate_dimensions(t, dims=dims)
+    if t.dtype not in _cabi.DATA_DTYPE_CODES:
+        raise ValueError("Tensor must have either float16, bfloat16, or float32 dtype")
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise ValueError("Rounding to 8 bits has no gradient")
+    validate_device(t)
+
+
+@plain_dispatch
+def _quantize_rows_eager(x: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    _validate(x, dtype, 2)
+    rows, width = x.shape
+    if x.stride(1) != 1 and width > 1:
+        if not contiguous_enabled():
+            raise ValueError("Tensor must be contiguous")
+        x = x.contiguous()
+    device = x.device
+    with _cabi.device_guard(device):
+        q = torch.empty((rows, width), dtype=dtype, device=device)
+        scale = torch.empty((rows, -(-width // SCALE_BLOCK)), dtype=torch.float32, device=device)
+        _cabi.check(_cabi.lib().bsp_quantize_rows(
+            x.data_ptr(), x.stride(0), rows, width, _cabi.DATA_DTYPE_CODES[x.dtype], q.data_ptr(),
+            _cabi.EIGHT_BIT_DTYPE_CODES[dtype], scale.data_ptr(), _cabi.stream_handle(device)), "bsp_quantize_rows")
+    return q, scale
+
+
+@plain_dispatch
+def _quantize_blocks_eager(w: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    _validate(w, dtype, 3)
+    groups, depth, cols = w.shape
+    device = w.device
+    with _cabi.device_guard(device):
+        q = torch.empty((groups, cols, depth), dtype=dtype, device=device).transpose(1, 2)
+        scale = torch.empty((groups, -(-depth // SCALE_BLOCK), -(-cols // SCALE_BLOCK)), dtype=torch.float32,
+                            device=device)
+        _cabi.check(_cabi.lib().bsp_quantize_blocks(
+            w.data_ptr(), *w.stride(), groups, depth, cols, _cabi.DATA_DTYPE_CODES[w.dtype], q.data_ptr(),
+            _cabi.EIGHT_BIT_DTYPE_CODES[dtype], scale.data_ptr(), _cabi.stream_handle(device)), "bsp_quantize_blocks")
+    return q, scale
+
+
+_quantize_rows_no_compile = torch.compiler.disable(_quantize_rows_eager)
+_quantize_blocks_no_compile = torch.compiler.disable(_quantize_blocks_eager)
+
+
+def quantize_rows(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[Tensor, Tensor]:
+    """Rounds rows to 8 bits with a scale for each 128 neighbouring values of a row.
+
+    Args:
+        x (Tensor): The rows ``(T, K)``, float16, bfloat16 or float32; the last block of a row may be short.
+        dtype (torch.dtype): float8_e4m3fn (default) or float8_e5m2.
+
+    Returns:
+        tuple[Tensor, Tensor]: The rounded rows ``(T, K)`` and the scales, float32 ``(T, ceil(K / 128))``.
+    """
+    return (_quantize_rows_no_compile if torch.compiler.is_compiling() else _quantize_rows_eager)(x, dtype)
+
+
+def quantize_blocks(w: Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[Tensor, Tensor]:
+    """Rounds matrices to 8 bits with a scale for each block of 128 x 128.
+
+    Args:
+        w (Tensor): One matrix per group ``(E, K, N)``, float16, bfloat16 or float32, any strides; the blocks at the
+            edges may be smaller.
+        dtype (torch.dtype): float8_e4m3fn (default) or float8_e5m2.
+
+    Returns:
+        tuple[Tensor, Tensor]: The rounded matrices ``(E, K, N)``, stored with ``K`` contiguous as
+        ``grouped_matmul_scaled`` reads them, and the scales, float32 ``(E, ceil(K / 128), ceil(N / 128))``.
+    """
+    return (_quantize_blocks_no_compile if torch.compiler.is_compiling() else _quantize_blocks_eager)(w, dtype)

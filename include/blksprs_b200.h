@@ -56,6 +56,8 @@ enum {
 
 /* element type of a compressed tensor */
 enum { BSP_F16 = 0, BSP_BF16 = 1, BSP_F32 = 2 };
+/* element type of an 8-bit operand of the scaled products (never of a compressed tensor) */
+enum { BSP_E4M3 = 3, BSP_E5M2 = 4 };
 
 /* which block product a launch computes; A, B, O are compressed tensors */
 enum {
@@ -411,6 +413,65 @@ int bsp_bias_grad(const void* grad_out, const int64_t* lut, int64_t n_blocks, in
  * backward of `w.repeat(batch, 1, 1)` (blksprs/utils/processing.py:52). */
 int bsp_sum_chunks(const void* parts, int64_t n_chunks, int64_t numel, int dtype,
                    void* out, void* stream);
+
+/* ---- products grouped by expert ------------------------------------------
+ * No counterpart in the blksprs library.  The rows of x are sorted by group:
+ * group e owns the rows offsets[e] <= t < offsets[e + 1] (device memory,
+ * groups + 1 values, int32 or with offsets_i64 != 0 int64; non-decreasing,
+ * within 0 .. rows).  Values that break this are clamped (no access leaves a
+ * buffer) and record BSP_ERR_DEVICE_RANGE in *status_word (may be NULL).
+ * Pointers start on 16-byte boundaries and every stride (in elements) is a
+ * multiple of 16 bytes; groups <= bsp_grouped_max_groups(). */
+int bsp_grouped_max_groups(void);
+
+/* out[t, :] = x[t, :] * w[e] for the rows t of group e, zero for rows of no
+ * group.  x: (rows, depth), row stride ld_x; w: (groups, depth, cols) with
+ * strides (group_stride_w, ld_w, 1) if w_cols_inner != 0, else
+ * (group_stride_w, 1, ld_w); out: contiguous (rows, cols).  fp16 / bf16,
+ * accumulated in fp32 and rounded once; depth and cols are multiples of 8. */
+int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, int64_t group_stride_w, int64_t ld_w,
+                       int w_cols_inner, const void* offsets, int offsets_i64, int64_t rows, int64_t groups,
+                       int64_t depth, int64_t cols, void* out, int dtype, int32_t* status_word, void* stream);
+
+/* out[e] = sum over the rows t of group e of x[t, :]^T * grad[t, :]; zero for
+ * a group without rows.  x: (rows, depth), grad: (rows, cols), out: contiguous
+ * (groups, depth, cols); types and sizes as above, rows >= 1. */
+int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* grad, int64_t ld_grad, const void* offsets,
+                            int offsets_i64, int64_t rows, int64_t groups, int64_t depth, int64_t cols, void* out,
+                            int dtype, int32_t* status_word, void* stream);
+
+/* out[t, n] = sum over the blocks b of 128 contraction values of
+ * scale_x[t, b] * scale_w[e, b, n / 128] * (x[t, b] . w[e, b, n]) for the rows
+ * t of group e, zero for rows of no group.  x: (rows, depth) of BSP_E4M3 or
+ * BSP_E5M2; w: (groups, depth, cols) of either type with strides
+ * (group_stride_w, 1, ld_w); scales fp32 with the given element strides; out:
+ * contiguous (rows, cols) of BSP_F16 / BSP_BF16 / BSP_F32.  depth is a multiple
+ * of 16 (the last block of a row may be short), cols of 8.  The products of a
+ * block are added up in fp32, then scaled, then added up in fp32. */
+int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x, const float* scale_x, int64_t sx_row,
+                              int64_t sx_block, const void* w, int64_t group_stride_w, int64_t ld_w, int type_w,
+                              const float* scale_w, int64_t sw_group, int64_t sw_k, int64_t sw_n,
+                              const void* offsets, int offsets_i64, int64_t rows, int64_t groups, int64_t depth,
+                              int64_t cols, void* out, int out_dtype, int32_t* status_word, void* stream);
+
+/* ---- 8-bit values with a scale for each block of 128 ----------------------
+ * scale = max(largest magnitude of the block / largest value of the type,
+ * 2^-126), q = value / scale rounded to nearest even.  A block that holds an
+ * infinity has an infinite scale, one that holds a NaN a NaN scale (both are
+ * NaN when multiplied out).  Input fp16 / bf16 / fp32. */
+
+/* Blocks of 1 x 128 along a row.  x: (rows, width), row stride ld_x; q:
+ * contiguous (rows, width); scale: contiguous (rows, ceil(width / 128)). */
+int bsp_quantize_rows(const void* x, int64_t ld_x, int64_t rows, int64_t width, int dtype, void* q, int type_q,
+                      float* scale, void* stream);
+
+/* Blocks of 128 x 128.  w: (groups, depth, cols) with element strides
+ * (group_stride_w, stride_depth, stride_cols); q: (groups, depth, cols) with
+ * strides (depth * cols, 1, depth), the order bsp_grouped_matmul_scaled reads;
+ * scale: contiguous (groups, ceil(depth / 128), ceil(cols / 128)). */
+int bsp_quantize_blocks(const void* w, int64_t group_stride_w, int64_t stride_depth, int64_t stride_cols,
+                        int64_t groups, int64_t depth, int64_t cols, int dtype, void* q, int type_q, float* scale,
+                        void* stream);
 
 #ifdef __cplusplus
 }
