@@ -7,25 +7,30 @@
 //                     and every 128 x 128 block of w with a scale of its own
 // Group lengths are known on the device only; nothing is read back to the host.
 //
-// Roles of the operands.  The tensor core multiplies A (M = 128 rows) by B (N columns, any multiple
-// of 16 up to 256).  M is the contiguous dimension of the output (the output features of a weight)
-// and N runs over the rows, so that a group's last tile costs what its rows cost (N = its length
-// rounded up to 32) and one row costs an MMA of N = 32, not a tile of 128.  Accumulator lanes are
-// output columns: a warp's 32 lanes hold 32 neighbouring elements of one output row.
+// Two SMs share a tile (cta_group::2): M = 256, 128 accumulator lanes in each SM, N up to 256.  Each
+// SM stages half of either operand, 32 KiB per 128 bytes of contraction; one SM alone with a tile of
+// 128 x 256 would stage 48 KiB for the same 512 cycles of tensor-core work, and shared memory would
+// be the bound (written once by TMA, read once by the MMA at 128 bytes per cycle: 768 cycles).
 //
-// One persistent CTA per SM, 12 warps: warp 0 copies tiles with TMA into a ring in shared memory
-// (128 bytes of contraction per row: 64 values of 16 bits or 128 of 8), warp 1 issues the MMAs,
-// warp 2 owns tensor memory, warps 4-11 are the epilogue.  Two accumulators of 256 columns: the
-// epilogue of one tile runs under the MMAs of the next.
+// Roles of the operands.
+//   16 bits: M runs over the output's contiguous dimension (output features), N over its rows.  N is any
+//   multiple of 32, so a group's last tile costs what its rows cost.  Lanes are output columns.
+//   8 bits: M runs over the rows, N over the output features.  A lane is a row of x, so a step's scale
+//   (one for each row and each 128 features) is one register per thread.
 //
-// Rows of a tile behind the end of its group belong to other groups: they only reach accumulator
-// columns that are not stored.  In the weight gradient the rows are the contraction, so there the
-// last (partial) step of a group is cut to a multiple of 16 rows and what is left of those 16 is
-// zeroed in shared memory before the MMA reads it.
+// Persistent CTA pairs, 12 warps per CTA: warp 0 copies tiles with TMA into a ring in shared memory,
+// warp 1 of the first CTA issues the MMAs, warp 2 owns tensor memory, warps 4-11 are the epilogue.
+// Two accumulators of 256 columns: the epilogue of one tile (8 bits: of one step) runs under the MMAs
+// of the next.
+//
+// Rows of a tile behind the end of its group belong to other groups: they only reach accumulator rows
+// that are not stored.  In the weight gradient the rows are the contraction, so there the last
+// (partial) step of a group is cut to a multiple of 16 rows and what is left of those 16 is zeroed in
+// shared memory before the MMA reads it.
 //
 // Every mbarrier wait is bounded (about one second): one that runs out records
-// BSP_ERR_DEVICE_TIMEOUT in the status word, all roles leave, copies in flight are waited for,
-// tensor memory is freed.  Offsets that decrease or leave 0 .. T record BSP_ERR_DEVICE_RANGE and
+// BSP_ERR_DEVICE_TIMEOUT in the status word, all roles leave, copies and MMAs in flight are waited
+// for, tensor memory is freed.  Offsets that decrease or leave 0 .. T record BSP_ERR_DEVICE_RANGE and
 // are clamped, so every access stays in bounds whatever they hold.
 #include <stdio.h>
 
@@ -42,23 +47,22 @@ namespace {
 
 constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
-constexpr int kTileM = 128;           // output columns of a tile
-constexpr int kTileN = 256;           // rows of a tile (at most)
-constexpr int kStages = 4;
-constexpr int kABytes = kTileM * 128;
-constexpr int kBBytes = kTileN * 128;
-constexpr int kStageBytes = kABytes + kBBytes;
+constexpr int kTile = 256;            // M and (at most) N of a pair's tile
+constexpr int kHalf = 128;            // what one CTA of the pair stages of either
+constexpr int kStages = 6;
+constexpr int kOperandBytes = kHalf * 128;
+constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kMaxGroups = 1024;      // bounded by the group table in shared memory
 constexpr int kBand = 8;              // row tiles that are walked together for every column tile
 
-constexpr int kModeRows = 0, kModeContract = 1;
+enum Mode { kRows16, kGrad16, kRows8 };
 
 struct Smem {
     static constexpr int kData = kStages * kStageBytes;
-    static constexpr int kScale = 2 * kTileN * 4;
-    static constexpr int kTable = 2 * (kMaxGroups + 1) * 4;
-    static constexpr int kBars = (2 * kStages + 5) * 8;
-    static constexpr int kTotal = kData + kScale + kTable + kBars + 64 + 1024;
+    static constexpr int kStaging = kEpiWarps * 2048;
+    static constexpr int kTable = (2 * (kMaxGroups + 1) * 4 + 7) & ~7;
+    static constexpr int kBars = (3 * kStages + 5) * 8;
+    static constexpr int kTotal = kData + kStaging + kTable + kBars + 1024;
 };
 
 struct Params {
@@ -82,84 +86,197 @@ struct Params {
 struct Tile {
     int group;
     int r0, rows;    // first output row (of the whole output, or of the group's output), rows to store
-    int c0;
+    int c0, cols;    // first output column, columns to store
+    int n;           // N of the MMA
     int t0;          // weight gradient: first contraction row
     int depth;       // contraction length
 };
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+// ---- PTX of CTA pairs --------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Copies into this CTA's shared memory that report to a barrier of either CTA of the pair.
+__device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
         ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                          uint32_t accumulate) {
+template <bool F8>
+__device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t accumulate) {
+    if (F8)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs when the MMAs issued so far are done.
+__device__ __forceinline__ void pair_commit(uint32_t bar) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
+// mbar_wait without a call: a call would have the epilogue's sums saved around it, and its registers are not
+// counted in a warpgroup's share.
+__device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
+                                             bool honor_abort = true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long t0 = global_timer();
+    for (uint32_t it = 1;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 0xff) == 0) {
+            if (honor_abort && *abort_flag) return false;
+            if (global_timer() - t0 > kWaitLimitNs) {
+                *abort_flag = 1;
+                if (status) *status = BSP_ERR_DEVICE_TIMEOUT;
+                return false;
+            }
+        }
+    }
+}
 // A bounded wait of a whole warp: true only if it succeeded for every lane, so that the lanes go on or leave together.
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status));
+    return __all_sync(0xffffffffu, bounded_wait(bar, parity, abort_flag, status));
 }
+// Orders what the other CTA wrote before its arrival (the barrier's wait acquires for this CTA only).
+__device__ __forceinline__ void acquire_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 
 __device__ __forceinline__ int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
-// Rows of a group are cut into the fewest tiles of at most kTileN rows, all of about the same height.
+// 16 bits: the rows of a group are cut into the fewest tiles of at most kTile rows, all of about the same height.
 __device__ __forceinline__ int tile_height(int m) {
-    const int n = (m + kTileN - 1) / kTileN;
+    const int n = (m + kTile - 1) / kTile;
     return n == 0 ? 0 : round_up((m + n - 1) / n, 32);
 }
 
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+// ---- epilogue pieces ----------------------------------------------------------------
+// A warp's staging area holds 32 output rows x 64 bytes; the 16-byte pieces of row r are permuted by
+// (r / 2) mod 4, which keeps both the writes below and the reads free of bank conflicts.
+__device__ __forceinline__ uint32_t staged_at(int row, int piece) { return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); }
 
-// 32 accumulator columns of one warp = 32 rows of the output, lane = output column.
-template <typename T>
-__device__ __forceinline__ void store_columns(T* out, int64_t ld, const float* v, int rows, bool col_ok) {
-    if (!col_ok) return;
+// Stores the staged rows: four lanes write the 64 bytes of a row, eight rows per instruction.
+__device__ __forceinline__ void store_staged(uint32_t staging, char* out, int64_t row_bytes, int rows, int bytes) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-        if (j < rows) out[j * ld] = from_float<T>(v[j]);
+    for (int i = 0; i < 4; ++i) {
+        const int row = 8 * i + (lane >> 2), piece = lane & 3;
+        uint32_t v[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(staging + staged_at(row, piece)));
+        if (row < rows && piece * 16 < bytes) st_global_16B(out + row * row_bytes + piece * 16, v);
+    }
+    __syncwarp();
 }
 
-template <int MODE, bool F8, bool A_MN>
-__global__ void __launch_bounds__(kThreads, 1)
+// v = 32 accumulator columns of one warp, lane = output column, column = output row: packs neighbouring
+// output columns (neighbouring lanes) into words; even lanes keep even rows, odd lanes odd rows.
+template <typename T>
+__device__ __forceinline__ void stage_transposed(uint32_t staging, const float* v) {
+    const int lane = threadIdx.x & 31, odd = lane & 1;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const uint32_t mine = pack2<T>(v[2 * j], v[2 * j + 1]);      // rows 2j, 2j + 1 of this column
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+        const uint32_t word = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+        const int row = 2 * j + odd;
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(staging + staged_at(row, lane >> 3) + ((lane >> 1) & 3) * 4), "r"(word) : "memory");
+    }
+}
+
+// 64 bytes of one output row per lane.
+__device__ __forceinline__ void stage_row(uint32_t staging, const uint32_t* words) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                     ::"r"(staging + staged_at(lane, i)), "r"(words[4 * i]), "r"(words[4 * i + 1]), "r"(words[4 * i + 2]), "r"(words[4 * i + 3]) : "memory");
+}
+
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
+
+// sum += v * s on 16 neighbouring columns; sums are kept as pairs, two fp32 multiply-adds per instruction.
+__device__ __forceinline__ void add_scaled(unsigned long long* sum, const uint32_t* v, unsigned long long s2) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        unsigned long long b;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "r"(v[2 * j]), "r"(v[2 * j + 1]));
+        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum[j]) : "l"(b), "l"(s2));
+    }
+}
+__device__ __forceinline__ float low_half(unsigned long long v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float high_half(unsigned long long v) { return __uint_as_float((uint32_t)(v >> 32)); }
+
+template <int MODE, bool A_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CUtensorMap map_b_small, const Params p) {
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
     const uint32_t data = (raw + 1023u) & ~1023u;
     unsigned char* data_ptr = smem_raw + (data - raw);
-    float* scale_s = reinterpret_cast<float*>(data_ptr + Smem::kData);
-    int* row_start = reinterpret_cast<int*>(data_ptr + Smem::kData + Smem::kScale);   // groups + 1
-    int* tile_start = row_start + kMaxGroups + 1;                                     // groups + 1
-    const uint32_t bars = data + Smem::kData + Smem::kScale + ((Smem::kTable + 7) & ~7);
+    int* row_start = reinterpret_cast<int*>(data_ptr + Smem::kData + Smem::kStaging);   // groups + 1
+    int* tile_start = row_start + kMaxGroups + 1;                                       // groups + 1
+    const uint32_t bars = data + Smem::kData + Smem::kStaging + Smem::kTable;
     const uint32_t full_bar = bars, empty_bar = bars + 8 * kStages, tfull_bar = bars + 16 * kStages,
-                   tempty_bar = tfull_bar + 16, drain_bar = tempty_bar + 16;
+                   tempty_bar = tfull_bar + 16, drain_bar = tempty_bar + 16, zeroed_bar = drain_bar + 8;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     __shared__ int issued_stages;
+    __shared__ int issued_tails[kStages];
     volatile int* abort_flag = &abort_word;
 
-    constexpr int KE = F8 ? 128 : 64;        // contraction values of a ring entry
+    constexpr bool F8 = MODE == kRows8;
+    constexpr int KE = F8 ? 128 : 64;        // contraction values of a ring entry (128 bytes)
     constexpr int KSTEP = F8 ? 32 : 16;      // contraction values of one MMA
-    constexpr bool B_MN = MODE == kModeContract;
+    constexpr bool B_MN = MODE == kGrad16;
 
+    const uint32_t rank = cluster_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full_bar + 8 * s, 1);
             mbar_init(empty_bar + 8 * s, 1);
+            mbar_init(zeroed_bar + 8 * s, 1);
+            issued_tails[s] = 0;
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(tfull_bar + 8 * i, 1);
-            mbar_init(tempty_bar + 8 * i, kEpiWarps);
+            mbar_init(tempty_bar + 8 * i, 2 * kEpiWarps);
         }
         mbar_init(drain_bar, 1);
         abort_word = 0;
@@ -176,15 +293,15 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         row_start[i] = (int)c;
     }
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;"
                      ::"r"(smem_addr(&tmem_slot)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    const int c_tiles = (p.cols + kTileM - 1) / kTileM;
+    const int c_tiles = (p.cols + kTile - 1) / kTile;
     if (warp == 0) {
         int high = 0, before = 0;
         for (int base = 0; base <= p.groups; base += 32) {
@@ -201,11 +318,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             if (i <= p.groups) row_start[i] = v;
         }
         __syncwarp();
-        if (MODE == kModeRows) {
+        if (MODE != kGrad16) {
             for (int base = 0; base < p.groups; base += 32) {
                 const int i = base + lane;
                 int n = 0;
-                if (i < p.groups) n = (row_start[i + 1] - row_start[i] + kTileN - 1) / kTileN * c_tiles;
+                if (i < p.groups) n = (row_start[i + 1] - row_start[i] + kTile - 1) / kTile * c_tiles;
                 const int own = n;
                 for (int d = 1; d < 32; d <<= 1) {
                     const int o = __shfl_up_sync(0xffffffffu, n, d);
@@ -218,14 +335,16 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
     }
     __syncthreads();
+    cluster_sync();      // the other CTA's barriers and tensor memory are ready
 
-    const int r_tiles_all = (p.out_rows + kTileN - 1) / kTileN;
-    const int n_tiles = MODE == kModeRows ? tile_start[p.groups] : p.groups * c_tiles * r_tiles_all;
+    const int r_tiles_all = (p.out_rows + kTile - 1) / kTile;
+    const int n_tiles = MODE != kGrad16 ? tile_start[p.groups] : p.groups * c_tiles * r_tiles_all;
+    const int first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
 
     auto tile_at = [&](int t) -> Tile {
         Tile o;
         int local, r_tiles;
-        if (MODE == kModeRows) {
+        if (MODE != kGrad16) {
             int lo = 0, hi = p.groups - 1;          // the last group whose first tile is at or before t
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
@@ -233,7 +352,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             }
             o.group = lo;
             local = t - tile_start[lo];
-            r_tiles = (row_start[lo + 1] - row_start[lo] + kTileN - 1) / kTileN;
+            r_tiles = (row_start[lo + 1] - row_start[lo] + kTile - 1) / kTile;
         } else {
             r_tiles = r_tiles_all;
             o.group = t / (c_tiles * r_tiles);
@@ -243,205 +362,274 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const int in_band = min(kBand, r_tiles - band * kBand);
         const int rest = local - band * kBand * c_tiles;
         const int c = rest / in_band, r = band * kBand + rest - c * in_band;
-        o.c0 = c * kTileM;
+        o.c0 = c * kTile;
+        o.cols = min(kTile, p.cols - o.c0);
         const int first = row_start[o.group], m = row_start[o.group + 1] - first;
-        if (MODE == kModeRows) {
-            const int h = tile_height(m);
+        if (MODE == kGrad16) {
+            o.r0 = r * kTile;
+            o.rows = min(kTile, p.out_rows - o.r0);
+            o.t0 = first;
+            o.depth = m;
+        } else {
+            const int h = MODE == kRows16 ? tile_height(m) : kTile;
             o.r0 = first + r * h;
             o.rows = min(h, m - r * h);
             o.t0 = 0;
             o.depth = p.depth;
-        } else {
-            o.r0 = r * kTileN;
-            o.rows = min(kTileN, p.out_rows - o.r0);
-            o.t0 = first;
-            o.depth = m;
         }
+        o.n = round_up(MODE == kRows8 ? o.cols : o.rows, 32);
         return o;
     };
 
-    if (warp == 0) {
-        // ---------------- copies ----------------
-        if (lane == 0) {
-            uint32_t it = 0;
+    // 8 bits: an epilogue thread holds 128 sums and 32 values on their way from tensor memory.  The warps of
+    // the first warpgroup give 96 registers each, those of the other two take 48: nothing is left over.
+    if (warp < 4) {
+        if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0) {
+            // ---------------- copies: each CTA its half of either operand ----------------
+            if (lane == 0) {
+                uint32_t it = 0;
+                bool alive = true;
+                for (int t = first_tile; t < n_tiles && alive; t += tile_step) {
+                    const Tile o = tile_at(t);
+                    const int half = o.n / 2;
+                    const int steps = (o.depth + KE - 1) / KE;
+                    // bytes of B one CTA copies
+                    const int b_bytes = B_MN ? (half + 63) / 64 * 8192 : half == kHalf ? kOperandBytes : (half + 31) / 32 * 4096;
+                    for (int k = 0; k < steps; ++k, ++it) {
+                        const uint32_t s = it % kStages;
+                        if (it >= kStages &&
+                            !bounded_wait(empty_bar + 8 * s, (it / kStages - 1) & 1, abort_flag, p.status)) {
+                            alive = false;
+                            break;
+                        }
+                        const uint32_t a = data + s * kStageBytes, b = a + kOperandBytes;
+                        // both halves report to the first CTA's barrier; in a step whose last rows have to be
+                        // zeroed the second CTA's half reports to the stage's barrier there, which has no other use
+                        const bool split = MODE == kGrad16 && ((o.depth - k * KE) & (KSTEP - 1)) && k == steps - 1;
+                        uint32_t bar = map_to_rank(full_bar + 8 * s, 0);
+                        if (rank == 0) {
+                            mbar_arrive_expect_tx(full_bar + 8 * s, (kOperandBytes + b_bytes) * (split ? 1 : 2));
+                            issued_stages = (int)it + 1;
+                        } else if (split) {
+                            bar = map_to_rank(full_bar + 8 * s, 1);
+                            mbar_arrive_expect_tx(full_bar + 8 * s, kOperandBytes + b_bytes);
+                            ++issued_tails[s];
+                        }
+                        if (MODE == kRows16) {
+                            const int m0 = o.c0 + rank * kHalf, n0 = o.r0 + rank * half;
+                            if (A_MN) {
+                                pair_load_3d(a, &map_a, m0, k * KE, o.group, bar);
+                                pair_load_3d(a + 8192, &map_a, m0 + 64, k * KE, o.group, bar);
+                            } else {
+                                pair_load_3d(a, &map_a, k * KE, m0, o.group, bar);
+                            }
+                            if (half == kHalf) {
+                                pair_load_2d(b, &map_b, k * KE, n0, bar);
+                            } else {
+                                for (int r = 0; r < half; r += 32) pair_load_2d(b + r * 128, &map_b_small, k * KE, n0 + r, bar);
+                            }
+                        } else if (MODE == kRows8) {
+                            const int m0 = o.r0 + rank * kHalf, n0 = o.c0 + rank * half;
+                            pair_load_2d(a, &map_a, k * KE, m0, bar);
+                            if (half == kHalf) {
+                                pair_load_3d(b, &map_b, k * KE, n0, o.group, bar);
+                            } else {
+                                for (int r = 0; r < half; r += 32) pair_load_3d(b + r * 128, &map_b_small, k * KE, n0 + r, o.group, bar);
+                            }
+                        } else {
+                            const int m0 = o.c0 + rank * kHalf, n0 = o.r0 + rank * half, t0 = o.t0 + k * KE;
+                            pair_load_2d(a, &map_a, m0, t0, bar);
+                            pair_load_2d(a + 8192, &map_a, m0 + 64, t0, bar);
+                            for (int r = 0; r < half; r += 64) pair_load_2d(b + r * 128, &map_b, n0 + r, t0, bar);
+                        }
+                    }
+                }
+                // the last arrivals from the first CTA's MMAs land before this CTA may leave
+                for (uint32_t i = it > kStages ? it - kStages : 0; i < it && alive; ++i)
+                    alive = bounded_wait(empty_bar + 8 * (i % kStages), (i / kStages) & 1, abort_flag, p.status);
+            }
+            __syncwarp();
+        } else if (warp == 1 && (rank == 0 || MODE == kGrad16)) {
+            // ---------------- MMAs (first CTA); zeroing of last rows (both) ----------------
+            uint32_t it = 0, acc = 0;
+            uint32_t tail_parity = 0;       // one bit per stage: uses of its barriers for zeroed rows
             bool alive = true;
-            for (int t = blockIdx.x; t < n_tiles && alive; t += gridDim.x) {
+            for (int t = first_tile; t < n_tiles && alive; t += tile_step) {
                 const Tile o = tile_at(t);
-                const int n = round_up(o.rows, 32);
                 const int steps = (o.depth + KE - 1) / KE;
+                const uint32_t idesc = p.idesc | ((uint32_t)(o.n >> 3) << 17);
                 for (int k = 0; k < steps; ++k, ++it) {
                     const uint32_t s = it % kStages;
-                    if (it >= kStages &&
-                        !mbar_wait(empty_bar + 8 * s, (it / kStages - 1) & 1, abort_flag, p.status)) {
-                        alive = false;
-                        break;
-                    }
-                    const uint32_t a = data + s * kStageBytes, b = a + kABytes, bar = full_bar + 8 * s;
-                    const int b_bytes = B_MN ? (n + 63) / 64 * 8192 : n * 128;
-                    mbar_arrive_expect_tx(bar, kABytes + b_bytes);
-                    issued_stages = (int)it + 1;
-                    if (MODE == kModeRows) {
-                        if (A_MN) {
-                            tma_load_3d(a, &map_a, o.c0, k * KE, o.group, bar);
-                            tma_load_3d(a + 8192, &map_a, o.c0 + 64, k * KE, o.group, bar);
-                        } else {
-                            tma_load_3d(a, &map_a, k * KE, o.c0, o.group, bar);
+                    const uint32_t a = data + s * kStageBytes, b = a + kOperandBytes;
+                    const int valid = min(KE, o.depth - k * KE);
+                    const int mmas = (valid + KSTEP - 1) / KSTEP;
+                    const bool zero_rows = MODE == kGrad16 && (valid & (KSTEP - 1));
+                    if (rank == 0) {
+                        // a new accumulator: per tile, and for 8-bit operands per step (every step has its own scales)
+                        if (F8 || k == 0) {
+                            alive = acc < 2 || wait_all(tempty_bar + 8 * (acc & 1), (acc / 2 - 1) & 1, abort_flag, p.status);
+                            if (!alive) break;
                         }
-                        int r = 0;
-                        for (; r + 128 <= n; r += 128) tma_load_2d(b + r * 128, &map_b, k * KE, o.r0 + r, bar);
-                        for (; r < n; r += 32) tma_load_2d(b + r * 128, &map_b_small, k * KE, o.r0 + r, bar);
-                    } else {
-                        tma_load_2d(a, &map_a, o.c0, o.t0 + k * KE, bar);
-                        tma_load_2d(a + 8192, &map_a, o.c0 + 64, o.t0 + k * KE, bar);
-                        for (int r = 0; r < n; r += 64)
-                            tma_load_2d(b + r * 128, &map_b, o.r0 + r, o.t0 + k * KE, bar);
+                        alive = wait_all(full_bar + 8 * s, (it / kStages) & 1, abort_flag, p.status);
+                    } else if (zero_rows) {
+                        alive = wait_all(full_bar + 8 * s, (tail_parity >> s) & 1, abort_flag, p.status);
                     }
-                }
-            }
-        }
-    } else if (warp == 1) {
-        // ---------------- MMAs (the whole warp walks, lane 0 issues) ----------------
-        uint32_t it = 0, acc = 0;
-        bool alive = true;
-        for (int t = blockIdx.x; t < n_tiles && alive; t += gridDim.x) {
-            const Tile o = tile_at(t);
-            const int n = round_up(o.rows, 32);
-            const int steps = (o.depth + KE - 1) / KE;
-            const uint32_t idesc = p.idesc | ((uint32_t)(n >> 3) << 17);
-            for (int k = 0; k < steps; ++k, ++it) {
-                const uint32_t s = it % kStages;
-                // a new accumulator: per tile, and for 8-bit operands per step (every step has its own scales)
-                if (F8 || k == 0) {
-                    alive = acc < 2 || wait_all(tempty_bar + 8 * (acc & 1), (acc / 2 - 1) & 1, abort_flag, p.status);
                     if (!alive) break;
-                    tc_fence_after();
-                }
-                alive = wait_all(full_bar + 8 * s, (it / kStages) & 1, abort_flag, p.status);
-                if (!alive) break;
-                const uint32_t a = data + s * kStageBytes, b = a + kABytes;
-                const int valid = min(KE, o.depth - k * KE);
-                const int mmas = (valid + KSTEP - 1) / KSTEP;
-                if (MODE == kModeContract && (valid & (KSTEP - 1))) {
-                    // rows of the next group inside the last 16: zero them in every 64-wide atom
-                    const int pieces = (mmas * KSTEP - valid) * 8;     // 16-byte pieces per atom
-                    const int atoms = 2 + (n + 63) / 64;
-                    for (int i = lane; i < atoms * pieces; i += 32) {
-                        const int atom = i / pieces, at = i - atom * pieces;
-                        const uint32_t dst = (atom < 2 ? a + atom * 8192 : b + (atom - 2) * 8192) + valid * 128 + at * 16;
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+                    if (zero_rows) {
+                        // rows of the next group inside the last 16: zero them in every 64-wide atom
+                        const int pieces = (mmas * KSTEP - valid) * 8;     // 16-byte pieces per atom
+                        const int atoms = 2 + (o.n / 2 + 63) / 64;
+                        for (int i = lane; i < atoms * pieces; i += 32) {
+                            const int atom = i / pieces, at = i - atom * pieces;
+                            const uint32_t dst = (atom < 2 ? a + atom * 8192 : b + (atom - 2) * 8192) + valid * 128 + at * 16;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (rank == 1) {
+                            if (lane == 0) mbar_arrive_cluster(map_to_rank(zeroed_bar + 8 * s, 0));
+                        } else {
+                            alive = wait_all(zeroed_bar + 8 * s, (tail_parity >> s) & 1, abort_flag, p.status);
+                            if (!alive) break;
+                            acquire_cluster();
+                        }
+                        tail_parity ^= 1u << s;
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                }
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t d = tmem + (acc & 1) * kTileN;
-                    for (int kk = 0; kk < mmas; ++kk) {
-                        const uint64_t ad = A_MN ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
-                        const uint64_t bd = B_MN ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
-                        const uint32_t accumulate = kk > 0 || (!F8 && k > 0);
-                        if (F8) tc_mma_f8(d, ad, bd, idesc, accumulate);
-                        else tc_mma_f16(d, ad, bd, idesc, accumulate);
+                    if (rank == 0) {
+                        tc_fence_after();
+                        if (lane == 0) {
+                            const uint32_t d = tmem + (acc & 1) * kTile;
+                            for (int kk = 0; kk < mmas; ++kk) {
+                                const uint64_t ad = A_MN ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
+                                const uint64_t bd = B_MN ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
+                                pair_mma<F8>(d, ad, bd, idesc, kk > 0 || (!F8 && k > 0));
+                            }
+                            pair_commit(empty_bar + 8 * s);
+                            if (F8 || k == steps - 1) pair_commit(tfull_bar + 8 * (acc & 1));
+                        }
+                        __syncwarp();
+                        if (F8 || k == steps - 1) ++acc;
                     }
-                    tc_commit(empty_bar + 8 * s);
-                    if (F8 || k == steps - 1) tc_commit(tfull_bar + 8 * (acc & 1));
                 }
-                __syncwarp();
-                if (F8 || k == steps - 1) ++acc;
             }
+            if (!alive && rank == 0 && lane == 0) {
+                // the MMAs issued so far finish before tensor memory is given back
+                pair_commit(drain_bar);
+                bounded_wait(drain_bar, 0, abort_flag, nullptr, false);
+            }
+            __syncwarp();
         }
-        if (!alive && lane == 0) {
-            // the MMAs issued so far finish before tensor memory is given back
-            tc_commit(drain_bar);
-            mbar_wait_slow(drain_bar, 0, abort_flag, nullptr, kWaitLimitNs, false);
-        }
-        __syncwarp();
-    } else if (warp >= 4) {
+    } else {
+        if (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---------------- epilogue ----------------
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
-        const int epi_thread = threadIdx.x - 128;
+        const int quarter = warp & 3, part = (warp - 4) >> 2;
+        const uint32_t staging = data + Smem::kData + (warp - 4) * 2048;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t tempty_first = map_to_rank(tempty_bar, 0);
+        const int esize = p.out_dtype == BSP_F32 ? 4 : 2;
+        const int64_t row_bytes = (int64_t)p.cols * esize;
         // rows outside every group are zero
-        if (MODE == kModeRows) {
-            const int64_t head = row_start[0], tail0 = row_start[p.groups];
-            const int64_t outside = head + (p.rows - tail0);
-            const int esize = p.out_dtype == BSP_F32 ? 4 : 2;
-            const int64_t row_bytes = (int64_t)p.cols * esize, pieces = row_bytes / 16;
-            for (int64_t i = (int64_t)blockIdx.x * 256 + epi_thread; i < outside * pieces; i += (int64_t)gridDim.x * 256) {
+        if (MODE != kGrad16) {
+            const int64_t before = row_start[0], behind = row_start[p.groups], pieces = row_bytes / 16;
+            const int64_t outside = before + (p.rows - behind);
+            for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x - 128; i < outside * pieces; i += (int64_t)gridDim.x * 256) {
                 const int64_t r = i / pieces, at = i - r * pieces;
-                const int64_t row = r < head ? r : tail0 + (r - head);
+                const int64_t row = r < before ? r : behind + (r - before);
                 *reinterpret_cast<int4*>((char*)p.out + row * row_bytes + at * 16) = make_int4(0, 0, 0, 0);
             }
         }
         uint32_t acc = 0;
         bool alive = true;
-        // 8-bit operands: a wait that ran out ends no loop early, the eight warps keep meeting at their
-        // barrier and only skip what the wait was for
-        for (int t = blockIdx.x; t < n_tiles && (F8 || alive); t += gridDim.x) {
+        for (int t = first_tile; t < n_tiles && alive; t += tile_step) {
             const Tile o = tile_at(t);
-            const int n = round_up(o.rows, 32);
             const int steps = (o.depth + KE - 1) / KE;
-            const int c = o.c0 + quarter * 32 + lane;
-            const bool col_ok = c < p.cols;
-            const int64_t first = MODE == kModeRows ? o.r0 : (int64_t)o.group * p.out_rows + o.r0;
-            const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-            auto store = [&](int c32, const float* v) {
-                const int rows = o.rows - c32;
-                const int64_t at = (first + c32) * p.cols + c;
-                if (p.out_dtype == BSP_F32) store_columns((float*)p.out + at, p.cols, v, rows, col_ok);
-                else if (p.out_dtype == BSP_F16) store_columns((__half*)p.out + at, p.cols, v, rows, col_ok);
-                else store_columns((__nv_bfloat16*)p.out + at, p.cols, v, rows, col_ok);
-            };
             if (F8) {
-                // every step's 128 products per element come back from tensor memory, are multiplied by
-                // the step's scales and added up in fp32 registers
-                float sum[4][32];
+                // lane = row of x.  Every step's 128 products per element come back from tensor memory, are
+                // multiplied by the step's scale and added up in fp32 registers: 128 columns per thread, one
+                // 128-wide block of w's scales.
+                const int row = (int)rank * kHalf + quarter * 32 + lane;
+                const bool active = row < o.rows && part * 128 < o.cols;
+                const float* sx = p.scale_x + (int64_t)(o.r0 + row) * p.sx_row;
+                const float* sw = p.scale_w + (int64_t)o.group * p.sw_group + (int64_t)(o.c0 / 128 + part) * p.sw_n;
+                auto scale_at = [&](int k) {
+                    return active && k < steps ? sx[(int64_t)k * p.sx_block] * sw[(int64_t)k * p.sw_k] : 0.0f;
+                };
+                unsigned long long sum[64];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int j = 0; j < 64; ++j) sum[j] = 0;
+                float next[4];                // the scales of the next four steps
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) sum[i][j] = 0.0f;
-                const bool row_ok = epi_thread < o.rows;
-                const float* sx = p.scale_x + (int64_t)(o.r0 + epi_thread) * p.sx_row;
-                const float* sw = p.scale_w + (int64_t)o.group * p.sw_group + (int64_t)(o.c0 / 128) * p.sw_n;
-                float next = row_ok ? sx[0] * sw[0] : 0.0f;
-                for (int k = 0; k < steps; ++k, ++acc) {
-                    float* scale_now = scale_s + (acc & 1) * kTileN;
-                    scale_now[epi_thread] = next;
-                    if (k + 1 < steps)
-                        next = row_ok ? sx[(int64_t)(k + 1) * p.sx_block] * sw[(int64_t)(k + 1) * p.sw_k] : 0.0f;
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    if (alive) alive = wait_all(tfull_bar + 8 * (acc & 1), (acc / 2) & 1, abort_flag, p.status);
-                    if (alive) {
-                        tc_fence_after();
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int c32 = (2 * i + half) * 32;
-                            if (c32 < n) {
-                                uint32_t v[32];
-                                tc_ld32(lanes + (acc & 1) * kTileN + c32, v);
-                                tc_wait_ld();
-#pragma unroll
-                                for (int j = 0; j < 32; j += 4) {
-                                    const float4 f = *reinterpret_cast<const float4*>(scale_now + c32 + j);
-                                    sum[i][j] += __uint_as_float(v[j]) * f.x;
-                                    sum[i][j + 1] += __uint_as_float(v[j + 1]) * f.y;
-                                    sum[i][j + 2] += __uint_as_float(v[j + 2]) * f.z;
-                                    sum[i][j + 3] += __uint_as_float(v[j + 3]) * f.w;
-                                }
-                            }
-                        }
-                    }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(tempty_bar + 8 * (acc & 1));
-                }
-                if (alive) {
+                for (int i = 0; i < 4; ++i) next[i] = scale_at(i);
+                for (int k0 = 0; k0 < steps && alive; k0 += 4) {
+                    float now[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int c32 = (2 * i + half) * 32;
-                        if (c32 < n) store(c32, sum[i]);
+                        now[i] = next[i];
+                        next[i] = scale_at(k0 + 4 + i);
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        if (k0 + kk >= steps || !alive) break;
+                        alive = wait_all(tfull_bar + 8 * (acc & 1), (acc / 2) & 1, abort_flag, p.status);
+                        if (!alive) break;
+                        tc_fence_after();
+                        const uint32_t from = lanes + (acc & 1) * kTile + part * 128;
+                        if (part * 128 < o.n) {
+                            // columns behind n hold what an earlier tile left: they are not stored
+                            uint32_t v[2][16];
+                            unsigned long long s2;
+                            asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(now[kk]));
+                            tc_ld16(from, v[0]);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                tc_wait_ld();
+                                if (i < 7) tc_ld16(from + i * 16 + 16, v[(i + 1) & 1]);
+                                add_scaled(sum + 8 * i, v[i & 1], s2);
+                            }
+                        }
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(tempty_first + 8 * (acc & 1));
+                        ++acc;
+                    }
+                }
+                if (!alive) break;
+                const int first_row = (int)rank * kHalf + quarter * 32, rows = o.rows - first_row;
+                char* out = (char*)p.out + (o.r0 + first_row) * row_bytes + (int64_t)(o.c0 + part * 128) * esize;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int left = (o.cols - part * 128 - i * 32) * esize;
+                    if (left > 0) {
+                        uint32_t words[16];
+                        if (p.out_dtype == BSP_F32) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    words[2 * j] = (uint32_t)sum[16 * i + 8 * h + j];
+                                    words[2 * j + 1] = (uint32_t)(sum[16 * i + 8 * h + j] >> 32);
+                                }
+                                stage_row(staging, words);
+                                store_staged(staging, out + i * 128 + h * 64, row_bytes, rows, left - h * 64);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                words[j] = p.out_dtype == BSP_F16
+                                               ? pack2<__half>(low_half(sum[16 * i + j]), high_half(sum[16 * i + j]))
+                                               : pack2<__nv_bfloat16>(low_half(sum[16 * i + j]), high_half(sum[16 * i + j]));
+                            stage_row(staging, words);
+                            store_staged(staging, out + i * 64, row_bytes, rows, left);
+                        }
                     }
                 }
             } else {
+                // lane = output column
+                const int c = o.c0 + (int)rank * kHalf + quarter * 32;
+                const int64_t first = MODE == kRows16 ? o.r0 : (int64_t)o.group * p.out_rows + o.r0;
+                char* out = (char*)p.out + first * row_bytes + (int64_t)c * 2;
+                const int bytes = (p.cols - c) * 2;
                 const bool computed = steps > 0;    // a group without rows has a gradient of zero
                 if (computed) {
                     alive = wait_all(tfull_bar + 8 * (acc & 1), (acc / 2) & 1, abort_flag, p.status);
@@ -449,24 +637,24 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     tc_fence_after();
                 }
 #pragma unroll 1
-                for (int i = 0; i < 4; ++i) {
-                    const int c32 = (2 * i + half) * 32;
-                    if (c32 < n) {
-                        uint32_t v[32];
-                        if (computed) {
-                            tc_ld32(lanes + (acc & 1) * kTileN + c32, v);
-                            tc_wait_ld();
-                        } else {
+                for (int c32 = part * 32; c32 < o.n; c32 += 64) {
+                    uint32_t v[32];
+                    if (computed) {
+                        tc_ld32(lanes + (acc & 1) * kTile + c32, v);
+                        tc_wait_ld();
+                    } else {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = 0;
-                        }
-                        store(c32, reinterpret_cast<const float*>(v));
+                        for (int j = 0; j < 32; ++j) v[j] = 0;
                     }
+                    const float* f = reinterpret_cast<const float*>(v);
+                    if (p.out_dtype == BSP_F16) stage_transposed<__half>(staging, f);
+                    else stage_transposed<__nv_bfloat16>(staging, f);
+                    store_staged(staging, out + c32 * row_bytes, row_bytes, o.rows - c32, bytes);
                 }
                 if (computed) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(tempty_bar + 8 * (acc & 1));
+                    if (lane == 0) mbar_arrive_cluster(tempty_first + 8 * (acc & 1));
                     ++acc;
                 }
             }
@@ -476,18 +664,23 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     // ---------------- teardown ----------------
     tc_fence_before();
     __syncthreads();
-    if (abort_word) {
-        // copies in flight land before the block may leave
-        if (threadIdx.x == 0) {
+    if (abort_word && threadIdx.x == 0) {
+        // copies in flight land before the block may leave (the first CTA's barriers cover both halves)
+        if (rank == 0) {
             const int last = issued_stages;
             for (int i = last > kStages ? last - kStages : 0; i < last; ++i)
-                mbar_wait_slow(full_bar + 8 * (i % kStages), (i / kStages) & 1, abort_flag, nullptr, kWaitLimitNs, false);
+                bounded_wait(full_bar + 8 * (i % kStages), (i / kStages) & 1, abort_flag, nullptr, false);
+        } else {
+            for (int s = 0; s < kStages; ++s)
+                if (issued_tails[s] > 0)
+                    bounded_wait(full_bar + 8 * s, (issued_tails[s] - 1) & 1, abort_flag, nullptr, false);
         }
-        __syncthreads();
     }
+    __syncthreads();
+    cluster_sync();      // neither CTA leaves, nor frees tensor memory, while the other may still reach it
     if (warp == 2) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
 }
 
@@ -542,10 +735,10 @@ int rows_map(CUtensorMap* map, const void* base, int elem, int64_t rows, int64_t
     return make_map(map, base, elem, 2, dims, strides, box);
 }
 
-template <int MODE, bool F8, bool A_MN>
+template <int MODE, bool A_MN>
 int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mbs, const Params& p, int64_t most_tiles,
            cudaStream_t stream) {
-    auto kern = grouped_kernel<MODE, F8, A_MN>;
+    auto kern = grouped_kernel<MODE, A_MN>;
     static std::atomic<uint64_t> opted_in{0};
     int dev = 0;
     BSP_CUDA_TRY(cudaGetDevice(&dev));
@@ -554,25 +747,25 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mbs,
         BSP_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem::kTotal));
         opted_in.fetch_or(dev_bit, std::memory_order_release);
     }
-    const int sms = num_sms();
-    if (sms <= 0) return BSP_ERR_CUDA;
-    const int ctas = (int)(most_tiles < sms ? (most_tiles < 1 ? 1 : most_tiles) : sms);
+    const int pairs = num_sms() / 2;
+    if (pairs <= 0) return BSP_ERR_CUDA;
+    const int ctas = 2 * (int)(most_tiles < pairs ? (most_tiles < 1 ? 1 : most_tiles) : pairs);
     kern<<<ctas, kThreads, Smem::kTotal, stream>>>(ma, mb, mbs, p);
     BSP_LAUNCH_CHECK();
     return BSP_OK;
 }
 
-// Tiles of a rows product: a group of m rows has ceil(m / kTileN) <= m / kTileN + 1 row tiles, and no more
+// Tiles of a rows product: a group of m rows has ceil(m / kTile) <= m / kTile + 1 row tiles, and no more
 // groups than rows have any.
 int64_t most_row_tiles(int64_t rows, int64_t groups) {
-    return rows / kTileN + (groups < rows ? groups : rows);
+    return rows / kTile + (groups < rows ? groups : rows);
 }
 
 int check_sizes(int64_t rows, int64_t groups, int64_t depth, int64_t cols, const void* offsets) {
     if (rows < 0 || groups < 1 || depth < 1 || cols < 1 || !offsets) return BSP_ERR_INVALID_ARG;
     if (groups > kMaxGroups || rows > 0x7fffffffLL - 512 || depth > 0x7fffffffLL - 512 || cols > 0x7fffffffLL - 512)
         return BSP_ERR_UNSUPPORTED;
-    if ((rows / kTileN + groups) * ceil_div(cols, kTileM) > 0x7fffffffLL - 65536) return BSP_ERR_UNSUPPORTED;
+    if ((rows / kTile + groups) * ceil_div(cols, kTile) > 0x7fffffffLL - 65536) return BSP_ERR_UNSUPPORTED;
     return BSP_OK;
 }
 
@@ -600,9 +793,9 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
     CUtensorMap ma, mb, mbs;
     const int64_t dims[3] = {inner, outer, groups};
     const int64_t strides[2] = {ld_w * 2, (groups > 1 ? group_stride_w : outer * ld_w) * 2};
-    const int box[3] = {64, w_cols_inner ? 64 : kTileM, 1};
+    const int box[3] = {64, w_cols_inner ? 64 : kHalf, 1};
     if ((st = make_map(&ma, w, dtype, 3, dims, strides, box)) != BSP_OK) return st;
-    if ((st = rows_map(&mb, x, dtype, rows, depth, ld_x, 128)) != BSP_OK) return st;
+    if ((st = rows_map(&mb, x, dtype, rows, depth, ld_x, kHalf)) != BSP_OK) return st;
     if ((st = rows_map(&mbs, x, dtype, rows, depth, ld_x, 32)) != BSP_OK) return st;
     Params p = {};
     p.offsets = offsets;
@@ -614,12 +807,12 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
     p.out = out;
     p.out_dtype = dtype;
     const uint32_t fmt = dtype == BSP_BF16 ? 1u : 0u;
-    p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((w_cols_inner ? 1u : 0u) << 15) | ((uint32_t)(kTileM >> 4) << 24);
+    p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((w_cols_inner ? 1u : 0u) << 15) | ((uint32_t)(kTile >> 4) << 24);
     p.status = status_word;
-    const int64_t tiles = most_row_tiles(rows, groups) * ceil_div(cols, kTileM);
+    const int64_t tiles = most_row_tiles(rows, groups) * ceil_div(cols, kTile);
     cudaStream_t stream = (cudaStream_t)stream_;
-    return w_cols_inner ? launch<kModeRows, false, true>(ma, mb, mbs, p, tiles, stream)
-                        : launch<kModeRows, false, false>(ma, mb, mbs, p, tiles, stream);
+    return w_cols_inner ? launch<kRows16, true>(ma, mb, mbs, p, tiles, stream)
+                        : launch<kRows16, false>(ma, mb, mbs, p, tiles, stream);
 }
 
 extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* grad, int64_t ld_grad,
@@ -633,7 +826,7 @@ extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* 
     if (!x || !grad || !out || !aligned16(x) || !aligned16(grad) || !aligned16(out)) return BSP_ERR_INVALID_ARG;
     if ((depth & 7) || (cols & 7) || (ld_x & 7) || (ld_grad & 7) || ld_x < depth || ld_grad < cols)
         return BSP_ERR_INVALID_ARG;
-    const int64_t tiles = groups * ceil_div(depth, kTileN) * ceil_div(cols, kTileM);
+    const int64_t tiles = groups * ceil_div(depth, kTile) * ceil_div(cols, kTile);
     if (tiles > 0x7fffffffLL - 65536) return BSP_ERR_UNSUPPORTED;
     if ((st = bind_context()) != BSP_OK) return st;
     CUtensorMap ma, mb;
@@ -649,9 +842,9 @@ extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* 
     p.out = out;
     p.out_dtype = dtype;
     const uint32_t fmt = dtype == BSP_BF16 ? 1u : 0u;
-    p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(kTileM >> 4) << 24);
+    p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(kTile >> 4) << 24);
     p.status = status_word;
-    return launch<kModeContract, false, true>(ma, mb, mb, p, tiles, (cudaStream_t)stream_);
+    return launch<kGrad16, true>(ma, mb, mb, p, tiles, (cudaStream_t)stream_);
 }
 
 extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x, const float* scale_x,
@@ -674,10 +867,10 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
     CUtensorMap ma, mb, mbs;
     const int64_t dims[3] = {depth, cols, groups};
     const int64_t strides[2] = {ld_w, groups > 1 ? group_stride_w : cols * ld_w};
-    const int box[3] = {128, kTileM, 1};
-    if ((st = make_map(&ma, w, type_w, 3, dims, strides, box)) != BSP_OK) return st;
-    if ((st = rows_map(&mb, x, type_x, rows, depth, ld_x, 128)) != BSP_OK) return st;
-    if ((st = rows_map(&mbs, x, type_x, rows, depth, ld_x, 32)) != BSP_OK) return st;
+    const int box[3] = {128, kHalf, 1}, box_small[3] = {128, 32, 1};
+    if ((st = make_map(&mb, w, type_w, 3, dims, strides, box)) != BSP_OK) return st;
+    if ((st = make_map(&mbs, w, type_w, 3, dims, strides, box_small)) != BSP_OK) return st;
+    if ((st = rows_map(&ma, x, type_x, rows, depth, ld_x, kHalf)) != BSP_OK) return st;
     Params p = {};
     p.offsets = offsets;
     p.offsets_i64 = offsets_i64;
@@ -687,8 +880,8 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
     p.depth = (int)depth;
     p.out = out;
     p.out_dtype = out_dtype;
-    p.idesc = (1u << 4) | ((type_w == BSP_E5M2 ? 1u : 0u) << 7) | ((type_x == BSP_E5M2 ? 1u : 0u) << 10) |
-              ((uint32_t)(kTileM >> 4) << 24);
+    p.idesc = (1u << 4) | ((type_x == BSP_E5M2 ? 1u : 0u) << 7) | ((type_w == BSP_E5M2 ? 1u : 0u) << 10) |
+              ((uint32_t)(kTile >> 4) << 24);
     p.scale_x = scale_x;
     p.sx_row = sx_row;
     p.sx_block = sx_block;
@@ -697,6 +890,6 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
     p.sw_k = sw_k;
     p.sw_n = sw_n;
     p.status = status_word;
-    const int64_t tiles = most_row_tiles(rows, groups) * ceil_div(cols, kTileM);
-    return launch<kModeRows, true, false>(ma, mb, mbs, p, tiles, (cudaStream_t)stream_);
+    const int64_t tiles = most_row_tiles(rows, groups) * ceil_div(cols, kTile);
+    return launch<kRows8, false>(ma, mb, mbs, p, tiles, (cudaStream_t)stream_);
 }
