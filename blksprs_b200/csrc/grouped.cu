@@ -53,6 +53,8 @@ constexpr int kStages = 6;
 constexpr int kOperandBytes = kHalf * 128;
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kMaxGroups = 1024;      // bounded by the group table in shared memory
+constexpr int kScaleSlots = 8;        // steps whose scales are staged ahead
+constexpr int kScaleSlot = kHalf + 4; // floats of a slot: one per row of the CTA's half, one per 128 columns
 constexpr int kBand = 8;              // row tiles that are walked together for every column tile
 
 enum Mode { kRows16, kGrad16, kRows8 };
@@ -61,8 +63,9 @@ struct Smem {
     static constexpr int kData = kStages * kStageBytes;
     static constexpr int kStaging = kEpiWarps * 2048;
     static constexpr int kTable = (2 * (kMaxGroups + 1) * 4 + 7) & ~7;
-    static constexpr int kBars = (3 * kStages + 5) * 8;
-    static constexpr int kTotal = kData + kStaging + kTable + kBars + 1024;
+    static constexpr int kScales = kScaleSlots * kScaleSlot * 4;
+    static constexpr int kBars = (3 * kStages + 5 + 2 * kScaleSlots) * 8;
+    static constexpr int kTotal = kData + kStaging + kTable + kScales + kBars + 1024;
 };
 
 struct Params {
@@ -106,7 +109,13 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+// Arrival on a barrier of either CTA.  The plain form publishes no writes to the other CTA (tensor-memory reads
+// are ordered by the tcgen05 fence before it): with release at cluster scope every arrival waited for all of the
+// warp's memory traffic, 2000 cycles per 8-bit step.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // Copies into this CTA's shared memory that report to a barrier of either CTA of the pair.
@@ -120,26 +129,32 @@ __device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* ma
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
         ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
+// Called by a converged warp, issued by one elected lane: the operands are warp-uniform then.  (Issued from
+// inside `if (lane == 0)` the same MMAs came 855 cycles per four apart instead of 512.)
 template <bool F8>
 __device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t accumulate) {
     if (F8)
         asm volatile(
-            "{\n\t.reg .pred p;\n\t"
+            "{\n\t.reg .pred p, e;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
             "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+            "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
             ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
     else
         asm volatile(
-            "{\n\t.reg .pred p;\n\t"
+            "{\n\t.reg .pred p, e;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
             "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
             ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
-// Arrives on the barrier at this offset in both CTAs when the MMAs issued so far are done.
+// Arrives on the barrier at this offset in both CTAs when the MMAs issued so far are done (converged warp).
 __device__ __forceinline__ void pair_commit(uint32_t bar) {
     asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
         ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
@@ -147,19 +162,28 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
 // counted in a warpgroup's share.
 __device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
                                              bool honor_abort = true) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const unsigned long long t0 = global_timer();
+    unsigned long long t0 = 0;
     for (uint32_t it = 1;; ++it) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((it & 0xff) == 0) {
             if (honor_abort && *abort_flag) return false;
-            if (global_timer() - t0 > kWaitLimitNs) {
+            if (t0 == 0) {
+                t0 = global_timer();
+            } else if (global_timer() - t0 > kWaitLimitNs) {
                 *abort_flag = 1;
                 if (status) *status = BSP_ERR_DEVICE_TIMEOUT;
                 return false;
             }
         }
     }
+}
+__device__ __forceinline__ void copy_async_4(uint32_t to, const float* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ float shared_float(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
 }
 // A bounded wait of a whole warp: true only if it succeeded for every lane, so that the lanes go on or leave together.
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
@@ -220,27 +244,6 @@ __device__ __forceinline__ void stage_row(uint32_t staging, const uint32_t* word
                      ::"r"(staging + staged_at(lane, i)), "r"(words[4 * i]), "r"(words[4 * i + 1]), "r"(words[4 * i + 2]), "r"(words[4 * i + 3]) : "memory");
 }
 
-__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr) : "memory");
-}
-
-// sum += v * s on 16 neighbouring columns; sums are kept as pairs, two fp32 multiply-adds per instruction.
-__device__ __forceinline__ void add_scaled(unsigned long long* sum, const uint32_t* v, unsigned long long s2) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        unsigned long long b;
-        asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "r"(v[2 * j]), "r"(v[2 * j + 1]));
-        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum[j]) : "l"(b), "l"(s2));
-    }
-}
-__device__ __forceinline__ float low_half(unsigned long long v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float high_half(unsigned long long v) { return __uint_as_float((uint32_t)(v >> 32)); }
-
 template <int MODE, bool A_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -251,9 +254,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     unsigned char* data_ptr = smem_raw + (data - raw);
     int* row_start = reinterpret_cast<int*>(data_ptr + Smem::kData + Smem::kStaging);   // groups + 1
     int* tile_start = row_start + kMaxGroups + 1;                                       // groups + 1
-    const uint32_t bars = data + Smem::kData + Smem::kStaging + Smem::kTable;
+    const uint32_t scales = data + Smem::kData + Smem::kStaging + Smem::kTable;
+    const uint32_t bars = scales + Smem::kScales;
     const uint32_t full_bar = bars, empty_bar = bars + 8 * kStages, tfull_bar = bars + 16 * kStages,
-                   tempty_bar = tfull_bar + 16, drain_bar = tempty_bar + 16, zeroed_bar = drain_bar + 8;
+                   tempty_bar = tfull_bar + 16, drain_bar = tempty_bar + 16, zeroed_bar = drain_bar + 8,
+                   sfull_bar = zeroed_bar + 8 * kStages, sempty_bar = sfull_bar + 8 * kScaleSlots;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     __shared__ int issued_stages;
@@ -279,6 +284,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             mbar_init(tempty_bar + 8 * i, 2 * kEpiWarps);
         }
         mbar_init(drain_bar, 1);
+        for (int i = 0; i < kScaleSlots; ++i) {
+            mbar_init(sfull_bar + 8 * i, 32);
+            mbar_init(sempty_bar + 8 * i, kEpiWarps);
+        }
         abort_word = 0;
         issued_stages = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -488,7 +497,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                         if (rank == 1) {
-                            if (lane == 0) mbar_arrive_cluster(map_to_rank(zeroed_bar + 8 * s, 0));
+                            if (lane == 0) mbar_arrive_release_cluster(map_to_rank(zeroed_bar + 8 * s, 0));
                         } else {
                             alive = wait_all(zeroed_bar + 8 * s, (tail_parity >> s) & 1, abort_flag, p.status);
                             if (!alive) break;
@@ -498,26 +507,48 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     }
                     if (rank == 0) {
                         tc_fence_after();
-                        if (lane == 0) {
-                            const uint32_t d = tmem + (acc & 1) * kTile;
-                            for (int kk = 0; kk < mmas; ++kk) {
-                                const uint64_t ad = A_MN ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
-                                const uint64_t bd = B_MN ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
-                                pair_mma<F8>(d, ad, bd, idesc, kk > 0 || (!F8 && k > 0));
-                            }
-                            pair_commit(empty_bar + 8 * s);
-                            if (F8 || k == steps - 1) pair_commit(tfull_bar + 8 * (acc & 1));
+                        const uint32_t d = tmem + (acc & 1) * kTile;
+                        for (int kk = 0; kk < mmas; ++kk) {
+                            const uint64_t ad = A_MN ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
+                            const uint64_t bd = B_MN ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
+                            pair_mma<F8>(d, ad, bd, idesc, kk > 0 || (!F8 && k > 0));
                         }
-                        __syncwarp();
+                        pair_commit(empty_bar + 8 * s);
+                        if (F8 || k == steps - 1) pair_commit(tfull_bar + 8 * (acc & 1));
                         if (F8 || k == steps - 1) ++acc;
                     }
                 }
             }
-            if (!alive && rank == 0 && lane == 0) {
+            if (!alive && rank == 0) {
                 // the MMAs issued so far finish before tensor memory is given back
                 pair_commit(drain_bar);
                 bounded_wait(drain_bar, 0, abort_flag, nullptr, false);
             }
+            __syncwarp();
+        } else if (F8 && warp == 3) {
+            // ---------------- scales: this CTA's rows' and the tile's two column blocks', steps ahead ----------------
+            uint32_t at = 0;
+            bool alive = true;
+            for (int t = first_tile; t < n_tiles && alive; t += tile_step) {
+                const Tile o = tile_at(t);
+                const int steps = (o.depth + KE - 1) / KE;
+                const int first = (int)rank * kHalf;
+                const float* sx = p.scale_x + (int64_t)(o.r0 + first + lane) * p.sx_row;
+                const float* sw = p.scale_w + (int64_t)o.group * p.sw_group + (int64_t)(o.c0 / 128 + (lane & 1)) * p.sw_n;
+                for (int k = 0; k < steps; ++k, ++at) {
+                    const uint32_t slot = at % kScaleSlots;
+                    if (at >= kScaleSlots) alive = wait_all(sempty_bar + 8 * slot, (at / kScaleSlots - 1) & 1, abort_flag, p.status);
+                    if (!alive) break;
+                    const uint32_t to = scales + slot * kScaleSlot * 4;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (first + i * 32 + lane < o.rows)
+                            copy_async_4(to + (i * 32 + lane) * 4, sx + i * 32 * p.sx_row + k * p.sx_block);
+                    if (lane < 2 && lane * 128 < o.cols) copy_async_4(to + (kHalf + lane) * 4, sw + k * p.sw_k);
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sfull_bar + 8 * slot) : "memory");
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
         }
     } else {
@@ -548,50 +579,33 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 // lane = row of x.  Every step's 128 products per element come back from tensor memory, are
                 // multiplied by the step's scale and added up in fp32 registers: 128 columns per thread, one
                 // 128-wide block of w's scales.
-                const int row = (int)rank * kHalf + quarter * 32 + lane;
-                const bool active = row < o.rows && part * 128 < o.cols;
-                const float* sx = p.scale_x + (int64_t)(o.r0 + row) * p.sx_row;
-                const float* sw = p.scale_w + (int64_t)o.group * p.sw_group + (int64_t)(o.c0 / 128 + part) * p.sw_n;
-                auto scale_at = [&](int k) {
-                    return active && k < steps ? sx[(int64_t)k * p.sx_block] * sw[(int64_t)k * p.sw_k] : 0.0f;
-                };
-                unsigned long long sum[64];
+                float sum[128];
 #pragma unroll
-                for (int j = 0; j < 64; ++j) sum[j] = 0;
-                float next[4];                // the scales of the next four steps
-#pragma unroll
-                for (int i = 0; i < 4; ++i) next[i] = scale_at(i);
-                for (int k0 = 0; k0 < steps && alive; k0 += 4) {
-                    float now[4];
+                for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
+                for (int k = 0; k < steps; ++k, ++acc) {
+                    const uint32_t slot = acc % kScaleSlots, at = scales + slot * kScaleSlot * 4;
+                    alive = wait_all(sfull_bar + 8 * slot, (acc / kScaleSlots) & 1, abort_flag, p.status);
+                    if (!alive) break;
+                    const float scale = shared_float(at + (quarter * 32 + lane) * 4) * shared_float(at + (kHalf + part) * 4);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sempty_bar + 8 * slot);
+                    alive = wait_all(tfull_bar + 8 * (acc & 1), (acc / 2) & 1, abort_flag, p.status);
+                    if (!alive) break;
+                    tc_fence_after();
+                    // columns behind n, and rows behind the tile's, hold what came before: they are not stored
+                    const uint32_t from = lanes + (acc & 1) * kTile + part * 128;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        now[i] = next[i];
-                        next[i] = scale_at(k0 + 4 + i);
-                    }
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        if (k0 + kk >= steps || !alive) break;
-                        alive = wait_all(tfull_bar + 8 * (acc & 1), (acc / 2) & 1, abort_flag, p.status);
-                        if (!alive) break;
-                        tc_fence_after();
-                        const uint32_t from = lanes + (acc & 1) * kTile + part * 128;
-                        if (part * 128 < o.n) {
-                            // columns behind n hold what an earlier tile left: they are not stored
-                            uint32_t v[2][16];
-                            unsigned long long s2;
-                            asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(now[kk]));
-                            tc_ld16(from, v[0]);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                tc_wait_ld();
-                                if (i < 7) tc_ld16(from + i * 16 + 16, v[(i + 1) & 1]);
-                                add_scaled(sum + 8 * i, v[i & 1], s2);
-                            }
+                        uint32_t v[32];
+                        tc_ld32(from + i * 32, v);
+                        tc_wait_ld();
+                        if (i == 3) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive_pair(tempty_first + 8 * (acc & 1));
                         }
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(tempty_first + 8 * (acc & 1));
-                        ++acc;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[32 * i + j] = fmaf(__uint_as_float(v[j]), scale, sum[32 * i + j]);
                     }
                 }
                 if (!alive) break;
@@ -606,19 +620,15 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    words[2 * j] = (uint32_t)sum[16 * i + 8 * h + j];
-                                    words[2 * j + 1] = (uint32_t)(sum[16 * i + 8 * h + j] >> 32);
-                                }
+                                for (int j = 0; j < 16; ++j) words[j] = __float_as_uint(sum[32 * i + 16 * h + j]);
                                 stage_row(staging, words);
                                 store_staged(staging, out + i * 128 + h * 64, row_bytes, rows, left - h * 64);
                             }
                         } else {
 #pragma unroll
                             for (int j = 0; j < 16; ++j)
-                                words[j] = p.out_dtype == BSP_F16
-                                               ? pack2<__half>(low_half(sum[16 * i + j]), high_half(sum[16 * i + j]))
-                                               : pack2<__nv_bfloat16>(low_half(sum[16 * i + j]), high_half(sum[16 * i + j]));
+                                words[j] = p.out_dtype == BSP_F16 ? pack2<__half>(sum[32 * i + 2 * j], sum[32 * i + 2 * j + 1])
+                                                                  : pack2<__nv_bfloat16>(sum[32 * i + 2 * j], sum[32 * i + 2 * j + 1]);
                             stage_row(staging, words);
                             store_staged(staging, out + i * 64, row_bytes, rows, left);
                         }
@@ -654,7 +664,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 if (computed) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(tempty_first + 8 * (acc & 1));
+                    if (lane == 0) mbar_arrive_pair(tempty_first + 8 * (acc & 1));
                     ++acc;
                 }
             }
