@@ -129,8 +129,37 @@ __device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* ma
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
         ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
-// Called by a converged warp, issued by one elected lane: the operands are warp-uniform then.  (Issued from
-// inside `if (lane == 0)` the same MMAs came 855 cycles per four apart instead of 512.)
+// The MMAs of a whole ring entry (four; fewer only at the end of the contraction), then the stage's release, and
+// for a finished accumulator its hand-over.  Called by a converged warp, issued by one elected lane, in one piece:
+// the issue of an entry has to stay below the 512 cycles its MMAs take.  One by one, each with its own election,
+// descriptors and loop test, they took 740; from inside `if (lane == 0)` 850.
+// STEP_A / STEP_B: descriptor distance (16-byte units) of neighbouring MMAs.
+#define BSP_PAIR_MMA(KIND)                                                                                     \
+    asm volatile(                                                                                              \
+        "{\n\t.reg .pred p, t, e, f;\n\t.reg .b64 a, b;\n\t"                                                 \
+        "elect.sync _|e, 0xffffffff;\n\t"                                                                     \
+        "setp.ne.b32 p, %4, 0;\n\t"                                                                           \
+        "setp.ne.and.b32 f, %7, 0, e;\n\t"                                                                    \
+        "setp.eq.b32 t, 0, 0;\n\t"                                                                            \
+        "@e tcgen05.mma.cta_group::2.kind::" KIND " [%0], %1, %2, %3, p;\n\t"                                 \
+        "add.s64 a, %1, %8;\n\tadd.s64 b, %2, %9;\n\t"                                                       \
+        "@e tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %3, t;\n\t"                                   \
+        "add.s64 a, a, %8;\n\tadd.s64 b, b, %9;\n\t"                                                         \
+        "@e tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %3, t;\n\t"                                   \
+        "add.s64 a, a, %8;\n\tadd.s64 b, b, %9;\n\t"                                                         \
+        "@e tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %3, t;\n\t"                                   \
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], %10;\n\t" \
+        "@f tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%6], %10;\n\t}" \
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(release_bar), "r"(done_bar),   \
+          "r"(done), "n"(STEP_A), "n"(STEP_B), "h"((uint16_t)3) : "memory")
+template <bool F8, int STEP_A, int STEP_B>
+__device__ __forceinline__ void pair_mma_entry(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accumulate, uint32_t release_bar, uint32_t done_bar,
+                                               uint32_t done) {
+    if (F8) BSP_PAIR_MMA("f8f6f4");
+    else BSP_PAIR_MMA("f16");
+}
+#undef BSP_PAIR_MMA
 template <bool F8>
 __device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t accumulate) {
@@ -508,13 +537,19 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     if (rank == 0) {
                         tc_fence_after();
                         const uint32_t d = tmem + (acc & 1) * kTile;
-                        for (int kk = 0; kk < mmas; ++kk) {
-                            const uint64_t ad = A_MN ? make_smem_desc(a + kk * 2048, 8192, 1024) : make_smem_desc(a + kk * 32, 16, 1024);
-                            const uint64_t bd = B_MN ? make_smem_desc(b + kk * 2048, 8192, 1024) : make_smem_desc(b + kk * 32, 16, 1024);
-                            pair_mma<F8>(d, ad, bd, idesc, kk > 0 || (!F8 && k > 0));
+                        const uint64_t ad = A_MN ? make_smem_desc(a, 8192, 1024) : make_smem_desc(a, 16, 1024);
+                        const uint64_t bd = B_MN ? make_smem_desc(b, 8192, 1024) : make_smem_desc(b, 16, 1024);
+                        constexpr int STEP_A = A_MN ? 128 : 2, STEP_B = B_MN ? 128 : 2;
+                        const bool done = F8 || k == steps - 1;
+                        if (mmas == 4) {
+                            pair_mma_entry<F8, STEP_A, STEP_B>(d, ad, bd, idesc, !F8 && k > 0, empty_bar + 8 * s,
+                                                               tfull_bar + 8 * (acc & 1), done);
+                        } else {
+                            for (int kk = 0; kk < mmas; ++kk)
+                                pair_mma<F8>(d, ad + kk * STEP_A, bd + kk * STEP_B, idesc, kk > 0 || (!F8 && k > 0));
+                            pair_commit(empty_bar + 8 * s);
+                            if (done) pair_commit(tfull_bar + 8 * (acc & 1));
                         }
-                        pair_commit(empty_bar + 8 * s);
-                        if (F8 || k == steps - 1) pair_commit(tfull_bar + 8 * (acc & 1));
                         if (F8 || k == steps - 1) ++acc;
                     }
                 }
