@@ -47,24 +47,30 @@ namespace {
 
 constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
-constexpr int kTile = 256;            // M and (at most) N of a pair's tile
-constexpr int kHalf = 128;            // what one CTA of the pair stages of either
-constexpr int kStages = 6;
-constexpr int kOperandBytes = kHalf * 128;
-constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kTile = 256;            // M of a pair's tile (and N, 16 bits)
+constexpr int kHalf = 128;            // M in either CTA
 constexpr int kMaxGroups = 1024;      // bounded by the group table in shared memory
-constexpr int kScaleSlots = 8;        // steps whose scales are staged ahead
-constexpr int kScaleSlot = kHalf + 4; // floats of a slot: one per row of the CTA's half, one per 128 columns
+constexpr int kScaleSlots = 4;        // groups of four steps whose scales are staged ahead
+constexpr int kScaleSlot = 4 * kHalf + 8;   // floats of a slot: four per row of the CTA's half, four of either block of w
 constexpr int kBand = 8;              // row tiles that are walked together for every column tile
 
 enum Mode { kRows16, kGrad16, kRows8 };
 
+// N of a tile, accumulators in tensor memory (512 columns in all), ring stages.  (8 bits with four accumulators of
+// N = 128 instead: 389 against 310 us on 16 groups of 1024 rows, 4096 x 4096; the hand-over of an accumulator
+// costs about the same whatever its width.)
+template <int MODE> struct Cfg { static constexpr int kN = 256, kAccs = 2, kStages = 6; };
+
+template <int MODE>
 struct Smem {
+    static constexpr int kStages = Cfg<MODE>::kStages;
+    static constexpr int kABytes = kHalf * 128, kBBytes = Cfg<MODE>::kN / 2 * 128;
+    static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kData = kStages * kStageBytes;
     static constexpr int kStaging = kEpiWarps * 2048;
     static constexpr int kTable = (2 * (kMaxGroups + 1) * 4 + 7) & ~7;
-    static constexpr int kScales = kScaleSlots * kScaleSlot * 4;
-    static constexpr int kBars = (3 * kStages + 5 + 2 * kScaleSlots) * 8;
+    static constexpr int kScales = MODE == kRows8 ? kScaleSlots * kScaleSlot * 4 : 0;
+    static constexpr int kBars = (3 * kStages + 2 * Cfg<MODE>::kAccs + 1 + 2 * kScaleSlots) * 8;
     static constexpr int kTotal = kData + kStaging + kTable + kScales + kBars + 1024;
 };
 
@@ -187,10 +193,10 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
         ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
-// mbar_wait without a call: a call would have the epilogue's sums saved around it, and its registers are not
-// counted in a warpgroup's share.
+// mbar_wait without a call: a call would have the epilogue's sums saved around it.
 __device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
                                              bool honor_abort = true) {
+    if (mbar_try_wait(bar, parity)) return true;
     unsigned long long t0 = 0;
     for (uint32_t it = 1;; ++it) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -209,17 +215,35 @@ __device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, vola
 __device__ __forceinline__ void copy_async_4(uint32_t to, const float* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
-__device__ __forceinline__ float shared_float(uint32_t at) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+__device__ __forceinline__ float4 shared_float4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
 }
-// A bounded wait of a whole warp: true only if it succeeded for every lane, so that the lanes go on or leave together.
+// A bounded wait of a whole warp: true only if it succeeded for every lane, so that the lanes go on or leave
+// together.  The first try is a straight line: 27 cycles on a barrier that is through, against 76 for the loop.
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
-    return __all_sync(0xffffffffu, bounded_wait(bar, parity, abort_flag, status));
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    unsigned long long t0 = 0;
+    for (uint32_t it = 1;; ++it) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if ((it & 0xff) == 0) {
+            const unsigned long long now = global_timer();
+            if (t0 == 0) t0 = now;
+            const bool late = now - t0 > kWaitLimitNs && now > t0;
+            if (late) {
+                *abort_flag = 1;
+                if (status) *status = BSP_ERR_DEVICE_TIMEOUT;
+            }
+            if (__any_sync(0xffffffffu, late || *abort_flag)) return false;
+        }
+    }
 }
 // Orders what the other CTA wrote before its arrival (the barrier's wait acquires for this CTA only).
 __device__ __forceinline__ void acquire_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+
+// A value all lanes of a converged warp hold, told to the compiler: MMA operands then live in uniform registers.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 __device__ __forceinline__ int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
@@ -277,17 +301,20 @@ template <int MODE, bool A_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CUtensorMap map_b_small, const Params p) {
+    using L = Smem<MODE>;
+    constexpr int kStages = L::kStages, kStageBytes = L::kStageBytes, kABytes = L::kABytes, kBBytes = L::kBBytes;
+    constexpr int kN = Cfg<MODE>::kN, kAccs = Cfg<MODE>::kAccs;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
     const uint32_t data = (raw + 1023u) & ~1023u;
     unsigned char* data_ptr = smem_raw + (data - raw);
-    int* row_start = reinterpret_cast<int*>(data_ptr + Smem::kData + Smem::kStaging);   // groups + 1
-    int* tile_start = row_start + kMaxGroups + 1;                                       // groups + 1
-    const uint32_t scales = data + Smem::kData + Smem::kStaging + Smem::kTable;
-    const uint32_t bars = scales + Smem::kScales;
-    const uint32_t full_bar = bars, empty_bar = bars + 8 * kStages, tfull_bar = bars + 16 * kStages,
-                   tempty_bar = tfull_bar + 16, drain_bar = tempty_bar + 16, zeroed_bar = drain_bar + 8,
-                   sfull_bar = zeroed_bar + 8 * kStages, sempty_bar = sfull_bar + 8 * kScaleSlots;
+    const uint32_t scales = data + L::kData + L::kStaging;
+    int* row_start = reinterpret_cast<int*>(data_ptr + L::kData + L::kStaging + L::kScales);   // groups + 1
+    int* tile_start = row_start + kMaxGroups + 1;                                              // groups + 1
+    const uint32_t bars = scales + L::kScales + L::kTable;
+    const uint32_t full_bar = bars, empty_bar = full_bar + 8 * kStages, zeroed_bar = empty_bar + 8 * kStages,
+                   tfull_bar = zeroed_bar + 8 * kStages, tempty_bar = tfull_bar + 8 * kAccs,
+                   drain_bar = tempty_bar + 8 * kAccs, sfull_bar = drain_bar + 8, sempty_bar = sfull_bar + 8 * kScaleSlots;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     __shared__ int issued_stages;
@@ -300,7 +327,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     constexpr bool B_MN = MODE == kGrad16;
 
     const uint32_t rank = cluster_rank();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full_bar + 8 * s, 1);
@@ -308,7 +335,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             mbar_init(zeroed_bar + 8 * s, 1);
             issued_tails[s] = 0;
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kAccs; ++i) {
             mbar_init(tfull_bar + 8 * i, 1);
             mbar_init(tempty_bar + 8 * i, 2 * kEpiWarps);
         }
@@ -338,8 +365,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot;
-    const int c_tiles = (p.cols + kTile - 1) / kTile;
+    const uint32_t tmem = uniform(tmem_slot);
+    constexpr int kTileCols = MODE == kRows8 ? kN : kTile;       // of the output
+    const int c_tiles = (p.cols + kTileCols - 1) / kTileCols;
     if (warp == 0) {
         int high = 0, before = 0;
         for (int base = 0; base <= p.groups; base += 32) {
@@ -376,7 +404,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     cluster_sync();      // the other CTA's barriers and tensor memory are ready
 
     const int r_tiles_all = (p.out_rows + kTile - 1) / kTile;
-    const int n_tiles = MODE != kGrad16 ? tile_start[p.groups] : p.groups * c_tiles * r_tiles_all;
+    const int n_tiles = uniform(MODE != kGrad16 ? tile_start[p.groups] : p.groups * c_tiles * r_tiles_all);
     const int first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
 
     auto tile_at = [&](int t) -> Tile {
@@ -400,8 +428,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const int in_band = min(kBand, r_tiles - band * kBand);
         const int rest = local - band * kBand * c_tiles;
         const int c = rest / in_band, r = band * kBand + rest - c * in_band;
-        o.c0 = c * kTile;
-        o.cols = min(kTile, p.cols - o.c0);
+        o.c0 = c * kTileCols;
+        o.cols = min(kTileCols, p.cols - o.c0);
         const int first = row_start[o.group], m = row_start[o.group + 1] - first;
         if (MODE == kGrad16) {
             o.r0 = r * kTile;
@@ -420,9 +448,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     };
 
     // 8 bits: an epilogue thread holds 128 sums and 32 values on their way from tensor memory.  The warps of
-    // the first warpgroup give 96 registers each, those of the other two take 48: nothing is left over.
+    // the first warpgroup give 112 registers per thread, those of the other two take 56: nothing is left over.
     if (warp < 4) {
-        if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0) {
             // ---------------- copies: each CTA its half of either operand ----------------
             if (lane == 0) {
@@ -433,7 +461,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     const int half = o.n / 2;
                     const int steps = (o.depth + KE - 1) / KE;
                     // bytes of B one CTA copies
-                    const int b_bytes = B_MN ? (half + 63) / 64 * 8192 : half == kHalf ? kOperandBytes : (half + 31) / 32 * 4096;
+                    const int b_bytes = B_MN ? (half + 63) / 64 * 8192 : half == kN / 2 ? kBBytes : (half + 31) / 32 * 4096;
                     for (int k = 0; k < steps; ++k, ++it) {
                         const uint32_t s = it % kStages;
                         if (it >= kStages &&
@@ -441,17 +469,17 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                             alive = false;
                             break;
                         }
-                        const uint32_t a = data + s * kStageBytes, b = a + kOperandBytes;
+                        const uint32_t a = data + s * kStageBytes, b = a + kABytes;
                         // both halves report to the first CTA's barrier; in a step whose last rows have to be
                         // zeroed the second CTA's half reports to the stage's barrier there, which has no other use
                         const bool split = MODE == kGrad16 && ((o.depth - k * KE) & (KSTEP - 1)) && k == steps - 1;
                         uint32_t bar = map_to_rank(full_bar + 8 * s, 0);
                         if (rank == 0) {
-                            mbar_arrive_expect_tx(full_bar + 8 * s, (kOperandBytes + b_bytes) * (split ? 1 : 2));
+                            mbar_arrive_expect_tx(full_bar + 8 * s, (kABytes + b_bytes) * (split ? 1 : 2));
                             issued_stages = (int)it + 1;
                         } else if (split) {
                             bar = map_to_rank(full_bar + 8 * s, 1);
-                            mbar_arrive_expect_tx(full_bar + 8 * s, kOperandBytes + b_bytes);
+                            mbar_arrive_expect_tx(full_bar + 8 * s, kABytes + b_bytes);
                             ++issued_tails[s];
                         }
                         if (MODE == kRows16) {
@@ -462,7 +490,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                             } else {
                                 pair_load_3d(a, &map_a, k * KE, m0, o.group, bar);
                             }
-                            if (half == kHalf) {
+                            if (half == kN / 2) {
                                 pair_load_2d(b, &map_b, k * KE, n0, bar);
                             } else {
                                 for (int r = 0; r < half; r += 32) pair_load_2d(b + r * 128, &map_b_small, k * KE, n0 + r, bar);
@@ -470,7 +498,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         } else if (MODE == kRows8) {
                             const int m0 = o.r0 + rank * kHalf, n0 = o.c0 + rank * half;
                             pair_load_2d(a, &map_a, k * KE, m0, bar);
-                            if (half == kHalf) {
+                            if (half == kN / 2) {
                                 pair_load_3d(b, &map_b, k * KE, n0, o.group, bar);
                             } else {
                                 for (int r = 0; r < half; r += 32) pair_load_3d(b + r * 128, &map_b_small, k * KE, n0 + r, o.group, bar);
@@ -495,18 +523,19 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             bool alive = true;
             for (int t = first_tile; t < n_tiles && alive; t += tile_step) {
                 const Tile o = tile_at(t);
-                const int steps = (o.depth + KE - 1) / KE;
-                const uint32_t idesc = p.idesc | ((uint32_t)(o.n >> 3) << 17);
+                const int depth = uniform(o.depth), n = uniform(o.n);
+                const int steps = (depth + KE - 1) / KE;
+                const uint32_t idesc = p.idesc | ((uint32_t)(n >> 3) << 17);
                 for (int k = 0; k < steps; ++k, ++it) {
                     const uint32_t s = it % kStages;
-                    const uint32_t a = data + s * kStageBytes, b = a + kOperandBytes;
-                    const int valid = min(KE, o.depth - k * KE);
+                    const uint32_t a = data + s * kStageBytes, b = a + kABytes;
+                    const int valid = min(KE, depth - k * KE);
                     const int mmas = (valid + KSTEP - 1) / KSTEP;
                     const bool zero_rows = MODE == kGrad16 && (valid & (KSTEP - 1));
                     if (rank == 0) {
                         // a new accumulator: per tile, and for 8-bit operands per step (every step has its own scales)
                         if (F8 || k == 0) {
-                            alive = acc < 2 || wait_all(tempty_bar + 8 * (acc & 1), (acc / 2 - 1) & 1, abort_flag, p.status);
+                            alive = acc < kAccs || wait_all(tempty_bar + 8 * (acc % kAccs), (acc / kAccs - 1) & 1, abort_flag, p.status);
                             if (!alive) break;
                         }
                         alive = wait_all(full_bar + 8 * s, (it / kStages) & 1, abort_flag, p.status);
@@ -517,7 +546,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     if (zero_rows) {
                         // rows of the next group inside the last 16: zero them in every 64-wide atom
                         const int pieces = (mmas * KSTEP - valid) * 8;     // 16-byte pieces per atom
-                        const int atoms = 2 + (o.n / 2 + 63) / 64;
+                        const int atoms = 2 + (n / 2 + 63) / 64;
                         for (int i = lane; i < atoms * pieces; i += 32) {
                             const int atom = i / pieces, at = i - atom * pieces;
                             const uint32_t dst = (atom < 2 ? a + atom * 8192 : b + (atom - 2) * 8192) + valid * 128 + at * 16;
@@ -536,19 +565,19 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     }
                     if (rank == 0) {
                         tc_fence_after();
-                        const uint32_t d = tmem + (acc & 1) * kTile;
+                        const uint32_t d = tmem + acc % kAccs * kN;
                         const uint64_t ad = A_MN ? make_smem_desc(a, 8192, 1024) : make_smem_desc(a, 16, 1024);
                         const uint64_t bd = B_MN ? make_smem_desc(b, 8192, 1024) : make_smem_desc(b, 16, 1024);
                         constexpr int STEP_A = A_MN ? 128 : 2, STEP_B = B_MN ? 128 : 2;
                         const bool done = F8 || k == steps - 1;
                         if (mmas == 4) {
                             pair_mma_entry<F8, STEP_A, STEP_B>(d, ad, bd, idesc, !F8 && k > 0, empty_bar + 8 * s,
-                                                               tfull_bar + 8 * (acc & 1), done);
+                                                               tfull_bar + 8 * (acc % kAccs), done);
                         } else {
                             for (int kk = 0; kk < mmas; ++kk)
                                 pair_mma<F8>(d, ad + kk * STEP_A, bd + kk * STEP_B, idesc, kk > 0 || (!F8 && k > 0));
                             pair_commit(empty_bar + 8 * s);
-                            if (done) pair_commit(tfull_bar + 8 * (acc & 1));
+                            if (done) pair_commit(tfull_bar + 8 * (acc % kAccs));
                         }
                         if (F8 || k == steps - 1) ++acc;
                     }
@@ -561,7 +590,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             }
             __syncwarp();
         } else if (F8 && warp == 3) {
-            // ---------------- scales: this CTA's rows' and the tile's two column blocks', steps ahead ----------------
+            // ---------------- scales: this CTA's rows' and the tile's two blocks of w's, steps ahead ----------------
             uint32_t at = 0;
             bool alive = true;
             for (int t = first_tile; t < n_tiles && alive; t += tile_step) {
@@ -569,8 +598,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 const int steps = (o.depth + KE - 1) / KE;
                 const int first = (int)rank * kHalf;
                 const float* sx = p.scale_x + (int64_t)(o.r0 + first + lane) * p.sx_row;
-                const float* sw = p.scale_w + (int64_t)o.group * p.sw_group + (int64_t)(o.c0 / 128 + (lane & 1)) * p.sw_n;
-                for (int k = 0; k < steps; ++k, ++at) {
+                const float* sw = p.scale_w + (int64_t)o.group * p.sw_group + (int64_t)(o.c0 / 128 + ((lane >> 2) & 1)) * p.sw_n;
+                for (int k = 0; k < steps; k += 4, ++at) {
                     const uint32_t slot = at % kScaleSlots;
                     if (at >= kScaleSlots) alive = wait_all(sempty_bar + 8 * slot, (at / kScaleSlots - 1) & 1, abort_flag, p.status);
                     if (!alive) break;
@@ -578,8 +607,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (first + i * 32 + lane < o.rows)
-                            copy_async_4(to + (i * 32 + lane) * 4, sx + i * 32 * p.sx_row + k * p.sx_block);
-                    if (lane < 2 && lane * 128 < o.cols) copy_async_4(to + (kHalf + lane) * 4, sw + k * p.sw_k);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (k + j < steps)
+                                    copy_async_4(to + (i * 32 + lane) * 16 + j * 4, sx + i * 32 * p.sx_row + (k + j) * p.sx_block);
+                    if (lane < 8 && k + (lane & 3) < steps && (lane >> 2) * 128 < o.cols)
+                        copy_async_4(to + kHalf * 16 + lane * 4, sw + (k + (lane & 3)) * p.sw_k);
                     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sfull_bar + 8 * slot) : "memory");
                 }
             }
@@ -587,10 +620,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             __syncwarp();
         }
     } else {
-        if (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        if (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // ---------------- epilogue ----------------
         const int quarter = warp & 3, part = (warp - 4) >> 2;
-        const uint32_t staging = data + Smem::kData + (warp - 4) * 2048;
+        const uint32_t staging = data + L::kData + (warp - 4) * 2048;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t tempty_first = map_to_rank(tempty_bar, 0);
         const int esize = p.out_dtype == BSP_F32 ? 4 : 2;
@@ -605,42 +638,56 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 *reinterpret_cast<int4*>((char*)p.out + row * row_bytes + at * 16) = make_int4(0, 0, 0, 0);
             }
         }
-        uint32_t acc = 0;
+        uint32_t acc = 0, scale_group = 0;
         bool alive = true;
         for (int t = first_tile; t < n_tiles && alive; t += tile_step) {
             const Tile o = tile_at(t);
             const int steps = (o.depth + KE - 1) / KE;
             if (F8) {
                 // lane = row of x.  Every step's 128 products per element come back from tensor memory, are
-                // multiplied by the step's scale and added up in fp32 registers: 128 columns per thread, one
-                // 128-wide block of w's scales.
+                // multiplied by the step's scale and added up in fp32 registers, 128 columns per thread.
                 float sum[128];
 #pragma unroll
                 for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
-                for (int k = 0; k < steps; ++k, ++acc) {
-                    const uint32_t slot = acc % kScaleSlots, at = scales + slot * kScaleSlot * 4;
-                    alive = wait_all(sfull_bar + 8 * slot, (acc / kScaleSlots) & 1, abort_flag, p.status);
-                    if (!alive) break;
-                    const float scale = shared_float(at + (quarter * 32 + lane) * 4) * shared_float(at + (kHalf + part) * 4);
+                // the scales of four steps (this row's times the one of these 128 columns)
+                float scale[4];
+                auto fetch = [&]() {
+                    const uint32_t slot = scale_group % kScaleSlots, from = scales + slot * kScaleSlot * 4;
+                    if (!wait_all(sfull_bar + 8 * slot, (scale_group / kScaleSlots) & 1, abort_flag, p.status)) return false;
+                    const float4 x = shared_float4(from + (quarter * 32 + lane) * 16), w = shared_float4(from + kHalf * 16 + part * 16);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(sempty_bar + 8 * slot);
-                    alive = wait_all(tfull_bar + 8 * (acc & 1), (acc / 2) & 1, abort_flag, p.status);
+                    ++scale_group;
+                    scale[0] = x.x * w.x;
+                    scale[1] = x.y * w.y;
+                    scale[2] = x.z * w.z;
+                    scale[3] = x.w * w.w;
+                    return true;
+                };
+                for (int k0 = 0; k0 < steps && alive; k0 += 4) {
+                    alive = fetch();
                     if (!alive) break;
-                    tc_fence_after();
-                    // columns behind n, and rows behind the tile's, hold what came before: they are not stored
-                    const uint32_t from = lanes + (acc & 1) * kTile + part * 128;
+#pragma unroll 1
+                    for (int kk = 0; kk < 4 && k0 + kk < steps; ++kk, ++acc) {
+                        alive = wait_all(tfull_bar + 8 * (acc % kAccs), (acc / kAccs) & 1, abort_flag, p.status);
+                        if (!alive) break;
+                        tc_fence_after();
+                        const float f = kk == 0 ? scale[0] : kk == 1 ? scale[1] : kk == 2 ? scale[2] : scale[3];
+                        // columns behind n, and rows behind the tile's, hold what came before: they are not stored
+                        const uint32_t from = lanes + acc % kAccs * kN + part * 128;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t v[32];
-                        tc_ld32(from + i * 32, v);
-                        tc_wait_ld();
-                        if (i == 3) {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive_pair(tempty_first + 8 * (acc & 1));
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t v[32];
+                            tc_ld32(from + i * 32, v);
+                            tc_wait_ld();
+                            if (i == 3) {
+                                tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive_pair(tempty_first + 8 * (acc % kAccs));
+                            }
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) sum[32 * i + j] = fmaf(__uint_as_float(v[j]), f, sum[32 * i + j]);
                         }
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) sum[32 * i + j] = fmaf(__uint_as_float(v[j]), scale, sum[32 * i + j]);
                     }
                 }
                 if (!alive) break;
@@ -677,7 +724,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 const int bytes = (p.cols - c) * 2;
                 const bool computed = steps > 0;    // a group without rows has a gradient of zero
                 if (computed) {
-                    alive = wait_all(tfull_bar + 8 * (acc & 1), (acc / 2) & 1, abort_flag, p.status);
+                    alive = wait_all(tfull_bar + 8 * (acc % kAccs), (acc / kAccs) & 1, abort_flag, p.status);
                     if (!alive) break;
                     tc_fence_after();
                 }
@@ -685,7 +732,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 for (int c32 = part * 32; c32 < o.n; c32 += 64) {
                     uint32_t v[32];
                     if (computed) {
-                        tc_ld32(lanes + (acc & 1) * kTile + c32, v);
+                        tc_ld32(lanes + acc % kAccs * kN + c32, v);
                         tc_wait_ld();
                     } else {
 #pragma unroll
@@ -699,7 +746,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 if (computed) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_pair(tempty_first + 8 * (acc & 1));
+                    if (lane == 0) mbar_arrive_pair(tempty_first + 8 * (acc % kAccs));
                     ++acc;
                 }
             }
@@ -789,13 +836,13 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mbs,
     BSP_CUDA_TRY(cudaGetDevice(&dev));
     const uint64_t dev_bit = dev >= 0 && dev < 64 ? (1ull << dev) : 0;
     if (!(opted_in.load(std::memory_order_acquire) & dev_bit)) {
-        BSP_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem::kTotal));
+        BSP_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<MODE>::kTotal));
         opted_in.fetch_or(dev_bit, std::memory_order_release);
     }
     const int pairs = num_sms() / 2;
     if (pairs <= 0) return BSP_ERR_CUDA;
     const int ctas = 2 * (int)(most_tiles < pairs ? (most_tiles < 1 ? 1 : most_tiles) : pairs);
-    kern<<<ctas, kThreads, Smem::kTotal, stream>>>(ma, mb, mbs, p);
+    kern<<<ctas, kThreads, Smem<MODE>::kTotal, stream>>>(ma, mb, mbs, p);
     BSP_LAUNCH_CHECK();
     return BSP_OK;
 }
@@ -810,7 +857,7 @@ int check_sizes(int64_t rows, int64_t groups, int64_t depth, int64_t cols, const
     if (rows < 0 || groups < 1 || depth < 1 || cols < 1 || !offsets) return BSP_ERR_INVALID_ARG;
     if (groups > kMaxGroups || rows > 0x7fffffffLL - 512 || depth > 0x7fffffffLL - 512 || cols > 0x7fffffffLL - 512)
         return BSP_ERR_UNSUPPORTED;
-    if ((rows / kTile + groups) * ceil_div(cols, kTile) > 0x7fffffffLL - 65536) return BSP_ERR_UNSUPPORTED;
+    if ((rows / kTile + groups) * ceil_div(cols, 128) > 0x7fffffffLL - 65536) return BSP_ERR_UNSUPPORTED;
     return BSP_OK;
 }
 
@@ -912,7 +959,7 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
     CUtensorMap ma, mb, mbs;
     const int64_t dims[3] = {depth, cols, groups};
     const int64_t strides[2] = {ld_w, groups > 1 ? group_stride_w : cols * ld_w};
-    const int box[3] = {128, kHalf, 1}, box_small[3] = {128, 32, 1};
+    const int box[3] = {128, Cfg<kRows8>::kN / 2, 1}, box_small[3] = {128, 32, 1};
     if ((st = make_map(&mb, w, type_w, 3, dims, strides, box)) != BSP_OK) return st;
     if ((st = make_map(&mbs, w, type_w, 3, dims, strides, box_small)) != BSP_OK) return st;
     if ((st = rows_map(&ma, x, type_x, rows, depth, ld_x, kHalf)) != BSP_OK) return st;
@@ -935,6 +982,6 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
     p.sw_k = sw_k;
     p.sw_n = sw_n;
     p.status = status_word;
-    const int64_t tiles = most_row_tiles(rows, groups) * ceil_div(cols, kTile);
+    const int64_t tiles = most_row_tiles(rows, groups) * ceil_div(cols, Cfg<kRows8>::kN);
     return launch<kRows8, false>(ma, mb, mbs, p, tiles, (cudaStream_t)stream_);
 }
