@@ -20,10 +20,8 @@ __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-__device__ __forceinline__ float scale_of(uint32_t largest, float type_max) {
-    const float s = __uint_as_float(largest) / type_max;
+__device__ __forceinline__ float scale_of(float largest, float type_max) {
+    const float s = largest / type_max;
     return s < kSmallestScale ? kSmallestScale : s;      // a NaN stays
 }
 
@@ -33,25 +31,36 @@ __device__ __forceinline__ float scale_of(uint32_t largest, float type_max) {
 // round to zero in either type) has a residual above 2^-103.  Other scales divide.
 struct Divider {
     float scale, reciprocal;
-    bool fast;
-    __device__ __forceinline__ explicit Divider(float s)
-        : scale(s), reciprocal(1.0f / s), fast(s > 8.67e-19f && s < 1.0e30f) {}
-    __device__ __forceinline__ float operator()(float x) const {
-        if (!fast) return x / scale;
+    __device__ __forceinline__ bool fast() const { return scale > 8.67e-19f && scale < 1.0e30f; }
+    __device__ __forceinline__ float quick(float x) const {
         const float q = x * reciprocal;
         return fmaf(fmaf(-q, scale, x), reciprocal, q);
     }
 };
+__device__ __forceinline__ Divider divide_by(float scale) { return {scale, 1.0f / scale}; }
 
 template <bool E5M2>
 __device__ __forceinline__ uint32_t round2(float a, float b) {
     return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
 }
 template <bool E5M2>
-__device__ __forceinline__ uint2 round8(const float* v, const Divider& over) {
+__device__ __forceinline__ uint2 round8(float* v, const Divider& over) {
+    if (over.fast()) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = over.quick(v[j]);
+    } else {
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+            // one at a time: this is rare, and eight divisions in line would be most of the kernel's code
+            const float q = v[0] / over.scale;
+#pragma unroll
+            for (int i = 0; i < 7; ++i) v[i] = v[i + 1];
+            v[7] = q;
+        }
+    }
     uint32_t out[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = round2<E5M2>(over(v[2 * j]), over(v[2 * j + 1]));
+    for (int j = 0; j < 4; ++j) out[j] = round2<E5M2>(v[2 * j], v[2 * j + 1]);
     return make_uint2(out[0] | (out[1] << 16), out[2] | (out[3] << 16));
 }
 
@@ -74,11 +83,23 @@ struct Eight {
         }
     }
     __device__ __forceinline__ float at(int j) const { return as_float(reinterpret_cast<const T*>(raw)[j]); }
+    // Largest magnitude as a bit pattern; 16-bit types: of the even and of the odd values, in either half.
     __device__ __forceinline__ uint32_t largest() const {
+        const uint32_t* word = reinterpret_cast<const uint32_t*>(raw);
         uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, magnitude(at(j)));
+        for (int i = 0; i < 4 * kVectors; ++i)
+            m = sizeof(T) == 2 ? __vmaxu2(m, word[i] & 0x7fff7fffu) : max(m, word[i] & 0x7fffffffu);
         return m;
+    }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+        return sizeof(T) == 2 ? __vmaxu2(a, b) : max(a, b);
+    }
+    // What largest() found, as a number.
+    static __device__ __forceinline__ float value_of(uint32_t m) {
+        if (sizeof(T) == 4) return __uint_as_float(m);
+        const uint16_t h = (uint16_t)max(m & 0xffffu, m >> 16);
+        return as_float(*reinterpret_cast<const T*>(&h));
     }
 };
 
@@ -91,32 +112,35 @@ __device__ __forceinline__ void store_tail(uint8_t* dst, uint2 v, int64_t left) 
 // ---- rows: a scale for each 1 x 128 ----------------------------------------------------
 // 16 lanes per block, 8 neighbouring values each; every half warp takes kAhead blocks at a time, whose loads
 // are under way together.  HBM-bound: each value once in (2 or 4 bytes) and once out (1 byte).
-constexpr int kAhead = 4;
+constexpr int kAhead = 4;       // the lanes that divide (below) are as many
 
 template <typename T, bool E5M2, bool VEC>
 __global__ void __launch_bounds__(256)
-quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t width, int64_t blocks,
-                     uint8_t* __restrict__ q, float* __restrict__ scale) {
+quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int rows, int width, int blocks, uint8_t* __restrict__ q,
+                     float* __restrict__ scale) {
     const float type_max = E5M2 ? 57344.0f : 448.0f;
-    const int sub = threadIdx.x & 15;
-    const int64_t total = rows * blocks, stride = (int64_t)gridDim.x * 16;
-    const int64_t row_step = stride / blocks, block_step = stride - row_step * blocks;
+    const int lane = threadIdx.x & 31, sub = lane & 15;
+    const int64_t stride = (int64_t)gridDim.x * 16;
+    const int row_step = (int)(stride / blocks), block_step = (int)(stride - (int64_t)row_step * blocks);
     // half warp h of the grid takes blocks h, h + stride, ...; both halves of a warp run the loop equally often
     // (the shuffles below take all lanes)
-    int64_t i = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
-    int64_t row = i / blocks, block = i - row * blocks;
+    const int64_t half = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+    int64_t row = half / blocks;
+    int block = (int)(half - row * blocks);
+    const int64_t total = (int64_t)rows * blocks;
     for (int64_t first = (int64_t)blockIdx.x * 16 + threadIdx.x / 32 * 2; first < total; first += kAhead * stride) {
         Eight<T> v[kAhead];
-        int64_t at[kAhead], to[kAhead], left[kAhead];
+        int64_t rows_at[kAhead];
+        int blocks_at[kAhead];
+        uint32_t m[kAhead];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
-            const int64_t col = block * kBlock + sub * 8;
-            at[a] = i;
-            to[a] = row * width + col;
-            left[a] = i < total ? width - col : 0;
-            if (VEC && left[a] >= 8) v[a].load(x + row * ld + col);
-            else v[a].gather(x + row * ld + col, 1, left[a]);
-            i += stride;
+            const int col = block * kBlock + sub * 8;
+            rows_at[a] = row;
+            blocks_at[a] = block;
+            const int left = row < rows ? width - col : 0;
+            if (VEC && left >= 8) v[a].load(x + row * ld + col);
+            else v[a].gather(x + row * ld + col, 1, left);
             row += row_step;
             block += block_step;
             if (block >= blocks) {
@@ -126,17 +150,29 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t 
         }
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
-            uint32_t m = v[a].largest();
+            m[a] = v[a].largest();
 #pragma unroll
-            for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-            const Divider over(scale_of(m, type_max));
-            if (at[a] < total && sub == 0) scale[at[a]] = over.scale;
-            float f[8];
+            for (int d = 8; d; d >>= 1) m[a] = Eight<T>::larger(m[a], __shfl_xor_sync(0xffffffffu, m[a], d));
+        }
+        // the divisions of the four blocks side by side: lanes 0-3 of a half warp have one each
+        const uint32_t mine = (lane & 2) ? ((lane & 1) ? m[3] : m[2]) : ((lane & 1) ? m[1] : m[0]);
+        const Divider of_mine = divide_by(scale_of(Eight<T>::value_of(mine), type_max));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = v[a].at(j);
-            const uint2 out = round8<E5M2>(f, over);
-            if (VEC && left[a] >= 8) *reinterpret_cast<uint2*>(q + to[a]) = out;
-            else if (left[a] > 0) store_tail(q + to[a], out, left[a]);
+        for (int a = 0; a < kAhead; ++a) {
+            Divider over;
+            over.scale = __shfl_sync(0xffffffffu, of_mine.scale, a, 16);
+            over.reciprocal = __shfl_sync(0xffffffffu, of_mine.reciprocal, a, 16);
+            if (rows_at[a] < rows) {
+                const int col = blocks_at[a] * kBlock + sub * 8, left = width - col;
+                if (sub == 0) scale[rows_at[a] * blocks + blocks_at[a]] = over.scale;
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = v[a].at(j);
+                const uint2 out = round8<E5M2>(f, over);
+                uint8_t* to = q + rows_at[a] * width + col;
+                if (VEC && left >= 8) *reinterpret_cast<uint2*>(to) = out;
+                else if (left > 0) store_tail(to, out, left);
+            }
         }
     }
 }
@@ -148,7 +184,7 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t 
 // are.  Otherwise it has 8 neighbouring columns of 8 neighbouring depths, and the rounded block goes through
 // shared memory: column n, 8-byte piece k at piece k ^ (n / 8 mod 16), free of bank conflicts both ways.
 template <typename T, bool E5M2, bool DEPTH_INNER>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
 quantize_blocks_kernel(const T* __restrict__ w, int64_t sg, int64_t sk, int64_t sn, int64_t depth, int64_t cols,
                        int64_t k_blocks, int64_t n_blocks, bool vec, uint8_t* __restrict__ q,
                        float* __restrict__ scale) {
@@ -174,14 +210,14 @@ quantize_blocks_kernel(const T* __restrict__ w, int64_t sg, int64_t sk, int64_t 
         else v[j].gather(from, DEPTH_INNER ? sk : sn, o < others ? inner_left : 0);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, v[j].largest());
+    for (int j = 0; j < 8; ++j) m = Eight<T>::larger(m, v[j].largest());
 #pragma unroll
-    for (int d = 16; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    for (int d = 16; d; d >>= 1) m = Eight<T>::larger(m, __shfl_xor_sync(0xffffffffu, m, d));
     if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, largest[i]);
-    const Divider over(scale_of(m, type_max));
+    for (int i = 0; i < 8; ++i) m = Eight<T>::larger(m, largest[i]);
+    const Divider over = divide_by(scale_of(Eight<T>::value_of(m), type_max));
     if (threadIdx.x == 0) scale[blockIdx.x] = over.scale;
     uint8_t* dst = q + g * depth * cols + n0 * depth + k0;
     const bool wide = (depth & 7) == 0;
@@ -224,8 +260,8 @@ int launch_rows(const void* x, int64_t ld, int64_t rows, int64_t width, void* q,
     // 16-byte loads and 8-byte stores need every row to start on such a boundary
     const bool vec = (ld * (int64_t)sizeof(T)) % 16 == 0 && width % 8 == 0 &&
                      (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
-    if (vec) quantize_rows_kernel<T, E5M2, true><<<(unsigned)ctas, 256, 0, stream>>>((const T*)x, ld, rows, width, blocks, (uint8_t*)q, scale);
-    else quantize_rows_kernel<T, E5M2, false><<<(unsigned)ctas, 256, 0, stream>>>((const T*)x, ld, rows, width, blocks, (uint8_t*)q, scale);
+    if (vec) quantize_rows_kernel<T, E5M2, true><<<(unsigned)ctas, 256, 0, stream>>>((const T*)x, ld, (int)rows, (int)width, (int)blocks, (uint8_t*)q, scale);
+    else quantize_rows_kernel<T, E5M2, false><<<(unsigned)ctas, 256, 0, stream>>>((const T*)x, ld, (int)rows, (int)width, (int)blocks, (uint8_t*)q, scale);
     BSP_LAUNCH_CHECK();
     return BSP_OK;
 }
@@ -268,6 +304,7 @@ extern "C" int bsp_quantize_rows(const void* x, int64_t ld_x, int64_t rows, int6
                                  int type_q, float* scale, void* stream) {
     if (rows < 0 || width < 0 || ld_x < 0) return BSP_ERR_INVALID_ARG;
     if (rows == 0 || width == 0) return BSP_OK;
+    if (rows > 0x7fffffffLL || width > 0x7fffffffLL - 256) return BSP_ERR_UNSUPPORTED;
     if (!x || !q || !scale) return BSP_ERR_INVALID_ARG;
     return dispatch(dtype, type_q, [&](auto t, bool e5m2) {
         using T = decltype(t);
