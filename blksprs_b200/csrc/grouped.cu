@@ -32,16 +32,13 @@
 // BSP_ERR_DEVICE_TIMEOUT in the status word, all roles leave, copies and MMAs in flight are waited
 // for, tensor memory is freed.  Offsets that decrease or leave 0 .. T record BSP_ERR_DEVICE_RANGE and
 // are clamped, so every access stays in bounds whatever they hold.
-#include <stdio.h>
-
 #include <atomic>
 
-#include "common.cuh"
-#include "umma_common.cuh"
+#include "grouped_common.cuh"
 
 namespace bsp {
 
-using namespace umma;
+using namespace grouped;
 
 namespace {
 
@@ -49,7 +46,6 @@ constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
 constexpr int kTile = 256;            // M of a pair's tile (and N, 16 bits)
 constexpr int kHalf = 128;            // M in either CTA
-constexpr int kMaxGroups = 1024;      // bounded by the group table in shared memory
 constexpr int kScaleSlots = 4;        // groups of four steps whose scales are staged ahead
 constexpr int kScaleSlot = 4 * kHalf + 8;   // floats of a slot: four per row of the CTA's half, four of either block of w
 constexpr int kBand = 8;              // row tiles that are walked together for every column tile
@@ -74,24 +70,6 @@ struct Smem {
     static constexpr int kTotal = kData + kStaging + kTable + kScales + kBars + 1024;
 };
 
-struct Params {
-    const void* offsets;
-    int offsets_i64;
-    int groups;
-    int rows;        // T
-    int cols;        // extent of the output's contiguous dimension
-    int out_rows;    // weight gradient: rows of one group's output
-    int depth;       // rows product: contraction length
-    void* out;
-    int out_dtype;
-    uint32_t idesc;  // instruction descriptor without N
-    const float* scale_x;
-    int64_t sx_row, sx_block;
-    const float* scale_w;
-    int64_t sw_group, sw_k, sw_n;
-    int32_t* status;
-};
-
 struct Tile {
     int group;
     int r0, rows;    // first output row (of the whole output, or of the group's output), rows to store
@@ -102,28 +80,6 @@ struct Tile {
 };
 
 // ---- PTX of CTA pairs --------------------------------------------------------------
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Arrival on a barrier of either CTA.  The plain form publishes no writes to the other CTA (tensor-memory reads
-// are ordered by the tcgen05 fence before it): with release at cluster scope every arrival waited for all of the
-// warp's memory traffic, 2000 cycles per 8-bit step.
-__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
 // Copies into this CTA's shared memory that report to a barrier of either CTA of the pair.
 __device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile(
@@ -193,108 +149,10 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
         ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
-// mbar_wait without a call: a call would have the epilogue's sums saved around it.
-__device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
-                                             bool honor_abort = true) {
-    if (mbar_try_wait(bar, parity)) return true;
-    unsigned long long t0 = 0;
-    for (uint32_t it = 1;; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 0xff) == 0) {
-            if (honor_abort && *abort_flag) return false;
-            if (t0 == 0) {
-                t0 = global_timer();
-            } else if (global_timer() - t0 > kWaitLimitNs) {
-                *abort_flag = 1;
-                if (status) *status = BSP_ERR_DEVICE_TIMEOUT;
-                return false;
-            }
-        }
-    }
-}
-__device__ __forceinline__ void copy_async_4(uint32_t to, const float* from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
-}
-__device__ __forceinline__ float4 shared_float4(uint32_t at) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-    return v;
-}
-// A bounded wait of a whole warp: true only if it succeeded for every lane, so that the lanes go on or leave
-// together.  The first try is a straight line: 27 cycles on a barrier that is through, against 76 for the loop.
-__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    unsigned long long t0 = 0;
-    for (uint32_t it = 1;; ++it) {
-        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-        if ((it & 0xff) == 0) {
-            const unsigned long long now = global_timer();
-            if (t0 == 0) t0 = now;
-            const bool late = now - t0 > kWaitLimitNs && now > t0;
-            if (late) {
-                *abort_flag = 1;
-                if (status) *status = BSP_ERR_DEVICE_TIMEOUT;
-            }
-            if (__any_sync(0xffffffffu, late || *abort_flag)) return false;
-        }
-    }
-}
-// Orders what the other CTA wrote before its arrival (the barrier's wait acquires for this CTA only).
-__device__ __forceinline__ void acquire_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
-
-// A value all lanes of a converged warp hold, told to the compiler: MMA operands then live in uniform registers.
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
-
-__device__ __forceinline__ int round_up(int v, int to) { return (v + to - 1) / to * to; }
-
 // 16 bits: the rows of a group are cut into the fewest tiles of at most kTile rows, all of about the same height.
 __device__ __forceinline__ int tile_height(int m) {
     const int n = (m + kTile - 1) / kTile;
     return n == 0 ? 0 : round_up((m + n - 1) / n, 32);
-}
-
-// ---- epilogue pieces ----------------------------------------------------------------
-// A warp's staging area holds 32 output rows x 64 bytes; the 16-byte pieces of row r are permuted by
-// (r / 2) mod 4, which keeps both the writes below and the reads free of bank conflicts.
-__device__ __forceinline__ uint32_t staged_at(int row, int piece) { return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); }
-
-// Stores the staged rows: four lanes write the 64 bytes of a row, eight rows per instruction.
-__device__ __forceinline__ void store_staged(uint32_t staging, char* out, int64_t row_bytes, int rows, int bytes) {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = 8 * i + (lane >> 2), piece = lane & 3;
-        uint32_t v[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(staging + staged_at(row, piece)));
-        if (row < rows && piece * 16 < bytes) st_global_16B(out + row * row_bytes + piece * 16, v);
-    }
-    __syncwarp();
-}
-
-// v = 32 accumulator columns of one warp, lane = output column, column = output row: packs neighbouring
-// output columns (neighbouring lanes) into words; even lanes keep even rows, odd lanes odd rows.
-template <typename T>
-__device__ __forceinline__ void stage_transposed(uint32_t staging, const float* v) {
-    const int lane = threadIdx.x & 31, odd = lane & 1;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const uint32_t mine = pack2<T>(v[2 * j], v[2 * j + 1]);      // rows 2j, 2j + 1 of this column
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-        const uint32_t word = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
-        const int row = 2 * j + odd;
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(staging + staged_at(row, lane >> 3) + ((lane >> 1) & 3) * 4), "r"(word) : "memory");
-    }
-}
-
-// 64 bytes of one output row per lane.
-__device__ __forceinline__ void stage_row(uint32_t staging, const uint32_t* words) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                     ::"r"(staging + staged_at(lane, i)), "r"(words[4 * i]), "r"(words[4 * i + 1]), "r"(words[4 * i + 2]), "r"(words[4 * i + 3]) : "memory");
 }
 
 template <int MODE, bool A_MN>
@@ -778,55 +636,6 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 
 // ---- host side ---------------------------------------------------------------------
 
-int make_map(CUtensorMap* map, const void* base, int elem, int rank, const int64_t* dims, const int64_t* strides_bytes,
-             const int* box) {
-    EncodeTiledFn fn = get_encode_fn();
-    if (!fn) {
-        set_cuda_error(cudaErrorNotSupported, "cuTensorMapEncodeTiled entry point");
-        return BSP_ERR_CUDA;
-    }
-    cuuint64_t d[3], s[2];
-    cuuint32_t b[3], e[3] = {1, 1, 1};
-    for (int i = 0; i < rank; ++i) {
-        d[i] = (cuuint64_t)dims[i];
-        b[i] = (cuuint32_t)box[i];
-    }
-    for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)strides_bytes[i];
-    const CUtensorMapDataType type = elem == BSP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                   : elem == BSP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                      : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    const CUresult r = fn(map, type, rank, const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) {
-        char what[64];
-        snprintf(what, sizeof(what), "cuTensorMapEncodeTiled: CUresult %d", (int)r);
-        set_cuda_error(cudaErrorInvalidValue, what);
-        return BSP_ERR_CUDA;
-    }
-    return BSP_OK;
-}
-
-// The encoder is a driver call and needs the device's context current in this thread; a thread that has
-// made no runtime call yet (the first backward of a process runs in one) does not have it.
-int bind_context() {
-    int dev = 0;
-    BSP_CUDA_TRY(cudaGetDevice(&dev));
-    BSP_CUDA_TRY(cudaSetDevice(dev));
-    return BSP_OK;
-}
-
-bool is_f8(int type) { return type == BSP_E4M3 || type == BSP_E5M2; }
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-// Rows (T, depth) with a row stride of ld elements; boxes of 128 bytes x `box_rows`.
-int rows_map(CUtensorMap* map, const void* base, int elem, int64_t rows, int64_t width, int64_t ld, int box_rows) {
-    const int esize = is_f8(elem) ? 1 : 2;
-    const int64_t dims[2] = {width, rows}, strides[1] = {ld * esize};
-    const int box[2] = {128 / esize, box_rows};
-    return make_map(map, base, elem, 2, dims, strides, box);
-}
-
 template <int MODE, bool A_MN>
 int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mbs, const Params& p, int64_t most_tiles,
            cudaStream_t stream) {
@@ -901,8 +710,12 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
     const uint32_t fmt = dtype == BSP_BF16 ? 1u : 0u;
     p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((w_cols_inner ? 1u : 0u) << 15) | ((uint32_t)(kTile >> 4) << 24);
     p.status = status_word;
-    const int64_t tiles = most_row_tiles(rows, groups) * ceil_div(cols, kTile);
     cudaStream_t stream = (cudaStream_t)stream_;
+    if (few_applies(rows, groups)) {
+        p.idesc = (p.idesc & 0x00ffffffu) | (128u >> 4 << 24);
+        return launch_few(false, w_cols_inner != 0, ma, mbs, p, stream);
+    }
+    const int64_t tiles = most_row_tiles(rows, groups) * ceil_div(cols, kTile);
     return w_cols_inner ? launch<kRows16, true>(ma, mb, mbs, p, tiles, stream)
                         : launch<kRows16, false>(ma, mb, mbs, p, tiles, stream);
 }
@@ -962,7 +775,8 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
     const int box[3] = {128, Cfg<kRows8>::kN / 2, 1}, box_small[3] = {128, 32, 1};
     if ((st = make_map(&mb, w, type_w, 3, dims, strides, box)) != BSP_OK) return st;
     if ((st = make_map(&mbs, w, type_w, 3, dims, strides, box_small)) != BSP_OK) return st;
-    if ((st = rows_map(&ma, x, type_x, rows, depth, ld_x, kHalf)) != BSP_OK) return st;
+    const bool few = few_applies(rows, groups);
+    if ((st = rows_map(&ma, x, type_x, rows, depth, ld_x, few ? 32 : kHalf)) != BSP_OK) return st;
     Params p = {};
     p.offsets = offsets;
     p.offsets_i64 = offsets_i64;
@@ -982,6 +796,12 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
     p.sw_k = sw_k;
     p.sw_n = sw_n;
     p.status = status_word;
+    if (few) {
+        // the weights are A there
+        p.idesc = (1u << 4) | ((type_w == BSP_E5M2 ? 1u : 0u) << 7) | ((type_x == BSP_E5M2 ? 1u : 0u) << 10) |
+                  (128u >> 4 << 24);
+        return launch_few(true, false, mb, ma, p, (cudaStream_t)stream_);
+    }
     const int64_t tiles = most_row_tiles(rows, groups) * ceil_div(cols, Cfg<kRows8>::kN);
     return launch<kRows8, false>(ma, mb, mbs, p, tiles, (cudaStream_t)stream_);
 }

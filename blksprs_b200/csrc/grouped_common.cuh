@@ -1,0 +1,218 @@
+// Shared by the grouped products (grouped.cu: tiles of CTA pairs; grouped_few.cu: few rows per group): launch
+// parameters, bounded waits, cluster and epilogue pieces, tensor maps.
+#pragma once
+
+#include <stdio.h>
+
+#include "common.cuh"
+#include "umma_common.cuh"
+
+namespace bsp {
+namespace grouped {
+
+using namespace umma;
+
+constexpr int kMaxGroups = 1024;      // bounded by the group table in shared memory
+
+struct Params {
+    const void* offsets;
+    int offsets_i64;
+    int groups;
+    int rows;        // T
+    int cols;        // extent of the output's contiguous dimension
+    int out_rows;    // weight gradient: rows of one group's output
+    int depth;       // rows product: contraction length
+    void* out;
+    int out_dtype;
+    uint32_t idesc;  // instruction descriptor without N
+    const float* scale_x;
+    int64_t sx_row, sx_block;
+    const float* scale_w;
+    int64_t sw_group, sw_k, sw_n;
+    int32_t* status;
+};
+
+// ---- clusters ----------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrival on a barrier of either CTA.  The plain form publishes no writes to the other CTA (tensor-memory reads
+// are ordered by the tcgen05 fence before it): with release at cluster scope every arrival waited for all of the
+// warp's memory traffic, 2000 cycles per 8-bit step.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// mbar_wait without a call: a call would have the epilogue's sums saved around it.
+__device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
+                                             bool honor_abort = true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    unsigned long long t0 = 0;
+    for (uint32_t it = 1;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 0xff) == 0) {
+            if (honor_abort && *abort_flag) return false;
+            if (t0 == 0) {
+                t0 = global_timer();
+            } else if (global_timer() - t0 > kWaitLimitNs) {
+                *abort_flag = 1;
+                if (status) *status = BSP_ERR_DEVICE_TIMEOUT;
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ void copy_async_4(uint32_t to, const float* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ float shared_float(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 shared_float4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+// A bounded wait of a whole warp: true only if it succeeded for every lane, so that the lanes go on or leave
+// together.  The first try is a straight line: 27 cycles on a barrier that is through, against 76 for the loop.
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    unsigned long long t0 = 0;
+    for (uint32_t it = 1;; ++it) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if ((it & 0xff) == 0) {
+            const unsigned long long now = global_timer();
+            if (t0 == 0) t0 = now;
+            const bool late = now - t0 > kWaitLimitNs && now > t0;
+            if (late) {
+                *abort_flag = 1;
+                if (status) *status = BSP_ERR_DEVICE_TIMEOUT;
+            }
+            if (__any_sync(0xffffffffu, late || *abort_flag)) return false;
+        }
+    }
+}
+// Orders what the other CTA wrote before its arrival (the barrier's wait acquires for this CTA only).
+__device__ __forceinline__ void acquire_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+
+// A value all lanes of a converged warp hold, told to the compiler: MMA operands then live in uniform registers.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+__device__ __forceinline__ int round_up(int v, int to) { return (v + to - 1) / to * to; }
+
+// ---- epilogue pieces ----------------------------------------------------------------
+// A warp's staging area holds 32 output rows x 64 bytes; the 16-byte pieces of row r are permuted by
+// (r / 2) mod 4, which keeps both the writes below and the reads free of bank conflicts.
+__device__ __forceinline__ uint32_t staged_at(int row, int piece) { return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); }
+
+// Stores the staged rows: four lanes write the 64 bytes of a row, eight rows per instruction.
+__device__ __forceinline__ void store_staged(uint32_t staging, char* out, int64_t row_bytes, int rows, int bytes) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 8 * i + (lane >> 2), piece = lane & 3;
+        uint32_t v[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(staging + staged_at(row, piece)));
+        if (row < rows && piece * 16 < bytes) st_global_16B(out + row * row_bytes + piece * 16, v);
+    }
+    __syncwarp();
+}
+
+// v = 32 accumulator columns of one warp, lane = output column, column = output row: packs neighbouring
+// output columns (neighbouring lanes) into words; even lanes keep even rows, odd lanes odd rows.
+template <typename T>
+__device__ __forceinline__ void stage_transposed(uint32_t staging, const float* v) {
+    const int lane = threadIdx.x & 31, odd = lane & 1;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const uint32_t mine = pack2<T>(v[2 * j], v[2 * j + 1]);      // rows 2j, 2j + 1 of this column
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+        const uint32_t word = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+        const int row = 2 * j + odd;
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(staging + staged_at(row, lane >> 3) + ((lane >> 1) & 3) * 4), "r"(word) : "memory");
+    }
+}
+
+// 64 bytes of one output row per lane.
+__device__ __forceinline__ void stage_row(uint32_t staging, const uint32_t* words) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                     ::"r"(staging + staged_at(lane, i)), "r"(words[4 * i]), "r"(words[4 * i + 1]), "r"(words[4 * i + 2]), "r"(words[4 * i + 3]) : "memory");
+}
+
+// ---- host side ---------------------------------------------------------------------
+
+inline int make_map(CUtensorMap* map, const void* base, int elem, int rank, const int64_t* dims, const int64_t* strides_bytes,
+             const int* box) {
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn) {
+        set_cuda_error(cudaErrorNotSupported, "cuTensorMapEncodeTiled entry point");
+        return BSP_ERR_CUDA;
+    }
+    cuuint64_t d[3], s[2];
+    cuuint32_t b[3], e[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) {
+        d[i] = (cuuint64_t)dims[i];
+        b[i] = (cuuint32_t)box[i];
+    }
+    for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)strides_bytes[i];
+    const CUtensorMapDataType type = elem == BSP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                   : elem == BSP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const CUresult r = fn(map, type, rank, const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        char what[64];
+        snprintf(what, sizeof(what), "cuTensorMapEncodeTiled: CUresult %d", (int)r);
+        set_cuda_error(cudaErrorInvalidValue, what);
+        return BSP_ERR_CUDA;
+    }
+    return BSP_OK;
+}
+
+// The encoder is a driver call and needs the device's context current in this thread; a thread that has
+// made no runtime call yet (the first backward of a process runs in one) does not have it.
+inline int bind_context() {
+    int dev = 0;
+    BSP_CUDA_TRY(cudaGetDevice(&dev));
+    BSP_CUDA_TRY(cudaSetDevice(dev));
+    return BSP_OK;
+}
+
+inline bool is_f8(int type) { return type == BSP_E4M3 || type == BSP_E5M2; }
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Rows (T, depth) with a row stride of ld elements; boxes of 128 bytes x `box_rows`.
+inline int rows_map(CUtensorMap* map, const void* base, int elem, int64_t rows, int64_t width, int64_t ld, int box_rows) {
+    const int esize = is_f8(elem) ? 1 : 2;
+    const int64_t dims[2] = {width, rows}, strides[1] = {ld * esize};
+    const int box[2] = {128 / esize, box_rows};
+    return make_map(map, base, elem, 2, dims, strides, box);
+}
+
+// Product of few rows per group (grouped_few.cu); same operands as the products it stands in for.
+int launch_few(bool f8, bool a_mn, const CUtensorMap& weights, const CUtensorMap& rows_small, const Params& p,
+               cudaStream_t stream);
+bool few_applies(int64_t rows, int64_t groups);
+
+}  // namespace grouped
+}  // namespace bsp

@@ -1,0 +1,445 @@
+// Products grouped by expert where the groups are short (a decoding step: one to a few rows for each expert): the
+// rows product and the scaled product of grouped.cu, same operands, other shape.
+//
+// What bounds it is streaming the weights of the groups that have rows, and below a few tens of megabytes the
+// latency of a launch.  So the tiles are small (128 output features x up to 64 rows, one CTA each, two CTAs per SM
+// with 96 KiB of copies under way), and where there are too few of them to fill the GPU the contraction is split
+// over a cluster of 2, 4 or 8 CTAs: each leaves its partial sums in its own shared memory, and after a cluster
+// barrier each adds up a share of the rows over all of them, always in the same order.  No workspace, no atomics,
+// the same bits on every run.
+//
+// A = weights (M = 128 features, accumulator lanes), B = rows (N = their number rounded up to 16).  8 bits: the
+// scale of a step belongs to the accumulator's columns; 32 of them are read from shared memory as vectors.
+//
+// Warp 0 copies, warp 1 issues the MMAs and owns tensor memory, warps 2-5 are the epilogue, warp 6 stages scales.
+// Waits are bounded and offsets are clamped as in grouped.cu.
+#include <atomic>
+
+#include "grouped_common.cuh"
+
+namespace bsp {
+namespace grouped {
+
+namespace {
+
+constexpr int kFewThreads = 7 * 32;
+constexpr int kFewM = 128;
+constexpr int kFewN = 64;
+constexpr int kFewStages = 4;
+constexpr int kFewStageBytes = kFewM * 128 + kFewN * 128;
+constexpr int kFewAccs = 2;                    // 8 bits: one per step, 16 bits: the first one
+constexpr int kFewScaleSlots = 4;              // steps in groups of four
+constexpr int kFewScaleSlot = 4 * kFewN + 4;   // floats: one per step and row, one per step
+
+struct FewSmem {
+    static constexpr int kData = kFewStages * kFewStageBytes;   // afterwards the partial sums, 64 x 128 floats
+    static constexpr int kStaging = 4 * 2048;
+    static constexpr int kScales = kFewScaleSlots * kFewScaleSlot * 4;
+    static constexpr int kBars = (2 * kFewStages + 2 * kFewAccs + 1 + 2 * kFewScaleSlots) * 8;
+    static constexpr int kTotal = kData + kStaging + kScales + kBars + 1024;     // two CTAs per SM
+    static_assert(kFewN * kFewM * 4 <= kData, "partial sums reuse the ring");
+    static_assert((kMaxGroups + 1) * 4 <= kStaging, "the offsets lie in the staging area until the tile is known");
+    static_assert(2 * (kTotal + 64 + 1024) <= 228 * 1024, "two CTAs per SM");
+};
+
+template <bool F8>
+__device__ __forceinline__ void few_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    if (F8)
+        asm volatile(
+            "{\n\t.reg .pred p, e;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        tc_mma_f16_elect(d_tmem, adesc, bdesc, idesc, accumulate);
+}
+
+__device__ __forceinline__ void few_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    tma_load_2d(dst, map, x, y, bar);
+}
+__device__ __forceinline__ void few_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ float2 cluster_float2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+// grid: x = cluster rank (split of the contraction) + split * column tile, y = row tile.
+template <bool F8, bool A_MN>
+__global__ void __launch_bounds__(kFewThreads, 2)
+grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p,
+                   const int split) {
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw = smem_addr(smem_raw);
+    const uint32_t data = (raw + 1023u) & ~1023u;
+    unsigned char* data_ptr = smem_raw + (data - raw);
+    const uint32_t scales = data + FewSmem::kData + FewSmem::kStaging;
+    int* row_start = reinterpret_cast<int*>(data_ptr + FewSmem::kData);      // groups + 1
+    const uint32_t bars = scales + FewSmem::kScales;
+    const uint32_t full_bar = bars, empty_bar = full_bar + 8 * kFewStages, tfull_bar = empty_bar + 8 * kFewStages,
+                   tempty_bar = tfull_bar + 8 * kFewAccs, drain_bar = tempty_bar + 8 * kFewAccs,
+                   sfull_bar = drain_bar + 8, sempty_bar = sfull_bar + 8 * kFewScaleSlots;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word, issued_stages;
+    __shared__ int tile_s[5];              // group, first row, rows (0: nothing to do), rows before and behind all groups
+    volatile int* abort_flag = &abort_word;
+
+    constexpr int KE = F8 ? 128 : 64;
+    constexpr int KSTEP = F8 ? 32 : 16;
+    constexpr uint32_t kColumns = F8 ? 128 : 64;     // of tensor memory
+
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int rank = split > 1 ? (int)cluster_rank() : 0;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kFewStages; ++s) {
+            mbar_init(full_bar + 8 * s, 1);
+            mbar_init(empty_bar + 8 * s, 1);
+        }
+        for (int i = 0; i < kFewAccs; ++i) {
+            mbar_init(tfull_bar + 8 * i, 1);
+            mbar_init(tempty_bar + 8 * i, 4);
+        }
+        mbar_init(drain_bar, 1);
+        for (int i = 0; i < kFewScaleSlots; ++i) {
+            mbar_init(sfull_bar + 8 * i, 32);
+            mbar_init(sempty_bar + 8 * i, 4);
+        }
+        abort_word = issued_stages = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async;" ::: "memory");
+    }
+    for (int i = threadIdx.x; i <= p.groups; i += kFewThreads) {
+        const long long v = p.offsets_i64 ? reinterpret_cast<const long long*>(p.offsets)[i]
+                                          : (long long)reinterpret_cast<const int*>(p.offsets)[i];
+        const long long c = v < 0 ? 0 : v > p.rows ? p.rows : v;
+        if (c != v && p.status) *p.status = BSP_ERR_DEVICE_RANGE;
+        row_start[i] = (int)c;
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_addr(&tmem_slot)), "r"(kColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = uniform(tmem_slot);
+    if (warp == 0) {
+        // running maximum of the offsets; the group that row tile blockIdx.y falls into
+        int high = 0, before = 0;
+        const int want = (int)blockIdx.y;
+        if (lane < 5) tile_s[lane] = 0;
+        __syncwarp();
+        for (int base = 0; base <= p.groups; base += 32) {
+            const int i = base + lane;
+            int v = i <= p.groups ? row_start[i] : 0;
+            const int own = v;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, v, d);
+                if (lane >= d) v = max(v, o);
+            }
+            v = max(v, high);
+            if (i <= p.groups && v != own && p.status) *p.status = BSP_ERR_DEVICE_RANGE;
+            // group i - 1 ends at v and starts where the lane before is
+            int start = __shfl_up_sync(0xffffffffu, v, 1);
+            if (lane == 0) start = high;
+            const int tiles = i >= 1 && i <= p.groups ? (v - start + kFewN - 1) / kFewN : 0;
+            int sum = tiles;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, sum, d);
+                if (lane >= d) sum += o;
+            }
+            const int first = before + sum - tiles;
+            if (tiles > 0 && want >= first && want < first + tiles) {
+                tile_s[0] = i - 1;
+                tile_s[1] = start + (want - first) * kFewN;
+                tile_s[2] = min(kFewN, v - tile_s[1]);
+            }
+            if (i == 0) tile_s[3] = v;
+            if (i == p.groups) tile_s[4] = v;
+            before += __shfl_sync(0xffffffffu, sum, 31);
+            high = __shfl_sync(0xffffffffu, v, 31);
+        }
+    }
+    __syncthreads();
+    const int group = uniform(tile_s[0]), r0 = uniform(tile_s[1]), rows = uniform(tile_s[2]);
+    const int c0 = (int)(blockIdx.x / split) * kFewM;
+    const int n = round_up(rows, 16);
+    const int all_steps = (p.depth + KE - 1) / KE, share = (all_steps + split - 1) / split;
+    const int first_step = min(all_steps, rank * share);
+    const int steps = rows > 0 ? min(all_steps, first_step + share) - first_step : 0;
+    const int esize = p.out_dtype == BSP_F32 ? 4 : 2;
+    const int64_t row_bytes = (int64_t)p.cols * esize;
+
+    if (warp == 0) {
+        // ---------------- copies ----------------
+        if (lane == 0) {
+            const int b_bytes = (n + 31) / 32 * 4096;
+            for (int k = 0; k < steps; ++k) {
+                const int s = k % kFewStages;
+                if (k >= kFewStages && !bounded_wait(empty_bar + 8 * s, (k / kFewStages - 1) & 1, abort_flag, p.status)) break;
+                const uint32_t a = data + s * kFewStageBytes, b = a + kFewM * 128, bar = full_bar + 8 * s;
+                const int x0 = (first_step + k) * KE;
+                mbar_arrive_expect_tx(bar, kFewM * 128 + b_bytes);
+                issued_stages = k + 1;
+                if (A_MN) {
+                    few_load_3d(a, &map_w, c0, x0, group, bar);
+                    few_load_3d(a + 8192, &map_w, c0 + 64, x0, group, bar);
+                } else {
+                    few_load_3d(a, &map_w, x0, c0, group, bar);
+                }
+                for (int r = 0; r < n; r += 32) few_load_2d(b + r * 128, &map_x, x0, r0 + r, bar);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---------------- MMAs ----------------
+        const uint32_t idesc = p.idesc | ((uint32_t)(n >> 3) << 17);
+        bool alive = true;
+        for (int k = 0; k < steps; ++k) {
+            const int s = k % kFewStages;
+            if (F8 && k >= kFewAccs) {
+                alive = wait_all(tempty_bar + 8 * (k % kFewAccs), (k / kFewAccs - 1) & 1, abort_flag, p.status);
+                if (!alive) break;
+            }
+            alive = wait_all(full_bar + 8 * s, (k / kFewStages) & 1, abort_flag, p.status);
+            if (!alive) break;
+            tc_fence_after();
+            const uint32_t a = data + s * kFewStageBytes, b = a + kFewM * 128;
+            const int valid = min(KE, p.depth - (first_step + k) * KE), mmas = (valid + KSTEP - 1) / KSTEP;
+            const uint32_t d = tmem + (F8 ? k % kFewAccs * kFewN : 0);
+            const uint64_t ad = A_MN ? make_smem_desc(a, 8192, 1024) : make_smem_desc(a, 16, 1024);
+            const uint64_t bd = make_smem_desc(b, 16, 1024);
+            for (int kk = 0; kk < mmas; ++kk)
+                few_mma<F8>(d, ad + kk * (A_MN ? 128 : 2), bd + kk * 2, idesc, kk > 0 || (!F8 && k > 0));
+            tc_commit_elect(empty_bar + 8 * s);
+            if (F8) tc_commit_elect(tfull_bar + 8 * (k % kFewAccs));
+            else if (k == steps - 1) tc_commit_elect(tfull_bar);
+        }
+        if (!alive) {
+            // the MMAs issued so far finish before tensor memory is given back
+            tc_commit_elect(drain_bar);
+            bounded_wait(drain_bar, 0, abort_flag, nullptr, false);
+        }
+        __syncwarp();
+    } else if (warp == 6) {
+        // ---------------- scales of four steps at a time (8 bits) ----------------
+        if (F8) {
+            const float* sx = p.scale_x + (int64_t)r0 * p.sx_row;
+            const float* sw = p.scale_w + (int64_t)group * p.sw_group + (int64_t)(c0 / 128) * p.sw_n;
+            for (int k0 = 0, at = 0; k0 < steps; k0 += 4, ++at) {
+                const int slot = at % kFewScaleSlots;
+                if (at >= kFewScaleSlots &&
+                    !wait_all(sempty_bar + 8 * slot, (at / kFewScaleSlots - 1) & 1, abort_flag, p.status))
+                    break;
+                const uint32_t to = scales + slot * kFewScaleSlot * 4;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t k = first_step + k0 + j;
+                    if (k0 + j < steps) {
+                        for (int r = lane; r < rows; r += 32)
+                            copy_async_4(to + (j * kFewN + r) * 4, sx + r * p.sx_row + k * p.sx_block);
+                        if (lane == j) copy_async_4(to + (4 * kFewN + j) * 4, sw + k * p.sw_k);
+                    }
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sfull_bar + 8 * slot) : "memory");
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+        }
+    }
+
+    // ---------------- epilogue warps: lane = output column, accumulator column = output row ----------------
+    const int quarter = warp & 3;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    float sum[2][32];
+    bool complete = rows > 0;
+    if (warp >= 2 && warp < 6) {
+        // rows outside every group are zero
+        const int64_t ctas = (int64_t)gridDim.x * gridDim.y, cta = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+        const int64_t before = tile_s[3], behind = tile_s[4], pieces = row_bytes / 16;
+        const int64_t outside = before + (p.rows - behind);
+        for (int64_t i = cta * 128 + threadIdx.x - 64; i < outside * pieces; i += ctas * 128) {
+            const int64_t r = i / pieces, at = i - r * pieces;
+            const int64_t row = r < before ? r : behind + (r - before);
+            *reinterpret_cast<int4*>((char*)p.out + row * row_bytes + at * 16) = make_int4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[h][j] = 0.0f;
+        if (F8) {
+            for (int k = 0; k < steps; ++k) {
+                const int slot = k / 4 % kFewScaleSlots;
+                const uint32_t from = scales + slot * kFewScaleSlot * 4 + (k & 3) * kFewN * 4;
+                complete = ((k & 3) != 0 || wait_all(sfull_bar + 8 * slot, (k / 4 / kFewScaleSlots) & 1, abort_flag, p.status)) &&
+                           wait_all(tfull_bar + 8 * (k % kFewAccs), (k / kFewAccs) & 1, abort_flag, p.status);
+                if (!complete) break;
+                tc_fence_after();
+                const float w = shared_float(scales + slot * kFewScaleSlot * 4 + (4 * kFewN + (k & 3)) * 4);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h * 32 < n) {
+                        // columns behind n, and scales behind the rows, hold anything: they are not stored
+                        uint32_t v[32];
+                        tc_ld32(lanes + k % kFewAccs * kFewN + h * 32, v);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 s = shared_float4(from + (h * 32 + j) * 4);
+                            sum[h][j] = fmaf(__uint_as_float(v[j]), s.x * w, sum[h][j]);
+                            sum[h][j + 1] = fmaf(__uint_as_float(v[j + 1]), s.y * w, sum[h][j + 1]);
+                            sum[h][j + 2] = fmaf(__uint_as_float(v[j + 2]), s.z * w, sum[h][j + 2]);
+                            sum[h][j + 3] = fmaf(__uint_as_float(v[j + 3]), s.w * w, sum[h][j + 3]);
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(tempty_bar + 8 * (k % kFewAccs));
+                    if ((k & 3) == 3 || k == steps - 1) mbar_arrive(sempty_bar + 8 * slot);
+                }
+            }
+        } else if (steps > 0) {
+            complete = wait_all(tfull_bar, 0, abort_flag, p.status);
+            if (complete) {
+                tc_fence_after();
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h * 32 < n) {
+                        uint32_t v[32];
+                        tc_ld32(lanes + h * 32, v);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[h][j] = __uint_as_float(v[j]);
+                    }
+                }
+                tc_fence_before();
+            }
+        }
+        if (split == 1 && complete) {
+            const uint32_t staging = data + FewSmem::kData + (warp - 2) * 2048;
+            const int c = c0 + quarter * 32;
+            char* out = (char*)p.out + r0 * row_bytes + (int64_t)c * esize;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h * 32 < rows) {
+                    if (p.out_dtype == BSP_F32) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (h * 32 + j < rows && c + lane < p.cols)
+                                *reinterpret_cast<float*>(out + (h * 32 + j) * row_bytes + lane * 4) = sum[h][j];
+                    } else {
+                        if (p.out_dtype == BSP_F16) stage_transposed<__half>(staging, sum[h]);
+                        else stage_transposed<__nv_bfloat16>(staging, sum[h]);
+                        store_staged(staging, out + h * 32 * row_bytes, row_bytes, rows - h * 32, (p.cols - c) * 2);
+                    }
+                }
+            }
+        }
+    }
+
+    // ---------------- teardown ----------------
+    tc_fence_before();
+    __syncthreads();
+    if (abort_word && threadIdx.x == 0) {
+        // copies in flight land before the block may leave (or its shared memory is used again)
+        const int last = issued_stages;
+        for (int i = last > kFewStages ? last - kFewStages : 0; i < last; ++i)
+            bounded_wait(full_bar + 8 * (i % kFewStages), (i / kFewStages) & 1, abort_flag, nullptr, false);
+    }
+    __syncthreads();
+    if (split > 1) {
+        // partial sums [row][column] over the ring, which every copy and MMA is through with
+        if (warp >= 2 && warp < 6) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (h * 32 + j < rows)
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(data + ((h * 32 + j) * kFewM + quarter * 32 + lane) * 4), "f"(sum[h][j]) : "memory");
+        }
+        cluster_sync();
+        const int pair = threadIdx.x & 63;                       // two columns of one row per thread
+        const int c = c0 + 2 * pair;
+        if (threadIdx.x < 192 && c < p.cols) {
+            for (int r = rank * 3 + (threadIdx.x >> 6); r < rows; r += split * 3) {
+                float2 total = make_float2(0.0f, 0.0f);
+                for (int q = 0; q < split; ++q) {
+                    const float2 part = cluster_float2(map_to_rank(data + (r * kFewM + 2 * pair) * 4, q));
+                    total.x += part.x;
+                    total.y += part.y;
+                }
+                char* out = (char*)p.out + (r0 + r) * row_bytes + (int64_t)c * esize;
+                if (p.out_dtype == BSP_F32) *reinterpret_cast<float2*>(out) = total;
+                else *reinterpret_cast<uint32_t*>(out) = p.out_dtype == BSP_F16 ? pack2<__half>(total.x, total.y)
+                                                                                : pack2<__nv_bfloat16>(total.x, total.y);
+            }
+        }
+        cluster_sync();      // no CTA leaves while another still reads its sums
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
+    }
+}
+
+template <bool F8, bool A_MN>
+int launch_kernel(const CUtensorMap& weights, const CUtensorMap& rows_small, const Params& p, cudaStream_t stream) {
+    auto kern = grouped_few_kernel<F8, A_MN>;
+    static std::atomic<uint64_t> opted_in{0};
+    int dev = 0;
+    BSP_CUDA_TRY(cudaGetDevice(&dev));
+    const uint64_t dev_bit = dev >= 0 && dev < 64 ? (1ull << dev) : 0;
+    if (!(opted_in.load(std::memory_order_acquire) & dev_bit)) {
+        BSP_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FewSmem::kTotal));
+        opted_in.fetch_or(dev_bit, std::memory_order_release);
+    }
+    const int sms = num_sms();
+    if (sms <= 0) return BSP_ERR_CUDA;
+    const int64_t c_tiles = ceil_div(p.cols, kFewM);
+    const int64_t hit = p.groups < p.rows ? p.groups : p.rows;
+    const int64_t row_tiles = p.rows / kFewN + hit;              // at most
+    if (c_tiles * 8 > 0x7fffffffLL || row_tiles > 65535) return BSP_ERR_UNSUPPORTED;
+    // Split the contraction while all CTAs fit the GPU at once (two per SM) and each keeps four steps.
+    const int64_t steps = ceil_div(p.depth, F8 ? 128 : 64);
+    int split = 1;
+    while (split < 8 && c_tiles * hit * split * 2 <= 2 * sms && steps >= 8 * split) split *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(c_tiles * split), (unsigned)row_tiles);
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = FewSmem::kTotal;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    BSP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, weights, rows_small, p, split));
+    return BSP_OK;
+}
+
+}  // namespace
+
+bool few_applies(int64_t rows, int64_t groups) {
+    const int64_t hit = groups < rows ? groups : rows;
+    return rows <= 32 * hit && rows / kFewN + hit <= 65535;
+}
+
+int launch_few(bool f8, bool a_mn, const CUtensorMap& weights, const CUtensorMap& rows_small, const Params& p,
+               cudaStream_t stream) {
+    if (f8) return launch_kernel<true, false>(weights, rows_small, p, stream);
+    return a_mn ? launch_kernel<false, true>(weights, rows_small, p, stream)
+                : launch_kernel<false, false>(weights, rows_small, p, stream);
+}
+
+}  // namespace grouped
+}  // namespace bsp

@@ -9,6 +9,7 @@
 #include <cuda_fp8.h>
 
 #include "common.cuh"
+#include "umma_common.cuh"
 
 namespace bsp {
 namespace {
@@ -110,37 +111,44 @@ __device__ __forceinline__ void store_tail(uint8_t* dst, uint2 v, int64_t left) 
 }
 
 // ---- rows: a scale for each 1 x 128 ----------------------------------------------------
-// 16 lanes per block, 8 neighbouring values each; every half warp takes kAhead blocks at a time, whose loads
-// are under way together.  HBM-bound: each value once in (2 or 4 bytes) and once out (1 byte).
+// 8 lanes per block, 16 neighbouring values each (37 us on 16384 x 4096 bf16, 5.4 TB/s; with 16 lanes of 8 values
+// 49 us: more shuffles and index arithmetic per value); every quarter warp takes kAhead blocks at a time, whose loads are under way together.
+// HBM-bound: each value once in (2 or 4 bytes) and once out (1 byte).
 constexpr int kAhead = 4;       // the lanes that divide (below) are as many
 
 template <typename T, bool E5M2, bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
 quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int rows, int width, int blocks, uint8_t* __restrict__ q,
                      float* __restrict__ scale) {
     const float type_max = E5M2 ? 57344.0f : 448.0f;
-    const int lane = threadIdx.x & 31, sub = lane & 15;
-    const int64_t stride = (int64_t)gridDim.x * 16;
+    const int lane = threadIdx.x & 31, sub = lane & 7;
+    const int64_t stride = (int64_t)gridDim.x * 32;
     const int row_step = (int)(stride / blocks), block_step = (int)(stride - (int64_t)row_step * blocks);
-    // half warp h of the grid takes blocks h, h + stride, ...; both halves of a warp run the loop equally often
-    // (the shuffles below take all lanes)
-    const int64_t half = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
-    int64_t row = half / blocks;
-    int block = (int)(half - row * blocks);
+    // quarter warp h of the grid takes blocks h, h + stride, ...; all quarters of a warp run the loop equally
+    // often (the shuffles below take all lanes)
+    const int64_t quarter = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
+    int64_t row = quarter / blocks;
+    int block = (int)(quarter - row * blocks);
     const int64_t total = (int64_t)rows * blocks;
-    for (int64_t first = (int64_t)blockIdx.x * 16 + threadIdx.x / 32 * 2; first < total; first += kAhead * stride) {
-        Eight<T> v[kAhead];
+    for (int64_t first = (int64_t)blockIdx.x * 32 + threadIdx.x / 32 * 4; first < total; first += kAhead * stride) {
+        Eight<T> v[kAhead][2];
         int64_t rows_at[kAhead];
         int blocks_at[kAhead];
         uint32_t m[kAhead];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
-            const int col = block * kBlock + sub * 8;
+            const int col = block * kBlock + sub * 16;
             rows_at[a] = row;
             blocks_at[a] = block;
             const int left = row < rows ? width - col : 0;
-            if (VEC && left >= 8) v[a].load(x + row * ld + col);
-            else v[a].gather(x + row * ld + col, 1, left);
+            const T* from = x + row * ld + col;
+            if (VEC && left >= 16) {
+                v[a][0].load(from);
+                v[a][1].load(from + 8);
+            } else {
+                v[a][0].gather(from, 1, left);
+                v[a][1].gather(from + 8, 1, left - 8);
+            }
             row += row_step;
             block += block_step;
             if (block >= blocks) {
@@ -150,28 +158,36 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int rows, int width, i
         }
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
-            m[a] = v[a].largest();
+            m[a] = Eight<T>::larger(v[a][0].largest(), v[a][1].largest());
 #pragma unroll
-            for (int d = 8; d; d >>= 1) m[a] = Eight<T>::larger(m[a], __shfl_xor_sync(0xffffffffu, m[a], d));
+            for (int d = 4; d; d >>= 1) m[a] = Eight<T>::larger(m[a], __shfl_xor_sync(0xffffffffu, m[a], d));
         }
-        // the divisions of the four blocks side by side: lanes 0-3 of a half warp have one each
+        // the divisions of the four blocks side by side: lanes 0-3 of a quarter warp have one each
         const uint32_t mine = (lane & 2) ? ((lane & 1) ? m[3] : m[2]) : ((lane & 1) ? m[1] : m[0]);
         const Divider of_mine = divide_by(scale_of(Eight<T>::value_of(mine), type_max));
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
             Divider over;
-            over.scale = __shfl_sync(0xffffffffu, of_mine.scale, a, 16);
-            over.reciprocal = __shfl_sync(0xffffffffu, of_mine.reciprocal, a, 16);
+            over.scale = __shfl_sync(0xffffffffu, of_mine.scale, a, 8);
+            over.reciprocal = __shfl_sync(0xffffffffu, of_mine.reciprocal, a, 8);
             if (rows_at[a] < rows) {
-                const int col = blocks_at[a] * kBlock + sub * 8, left = width - col;
+                const int col = blocks_at[a] * kBlock + sub * 16, left = width - col;
                 if (sub == 0) scale[rows_at[a] * blocks + blocks_at[a]] = over.scale;
-                float f[8];
+                uint2 out[2];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] = v[a].at(j);
-                const uint2 out = round8<E5M2>(f, over);
+                for (int h = 0; h < 2; ++h) {
+                    float f[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] = v[a][h].at(j);
+                    out[h] = round8<E5M2>(f, over);
+                }
                 uint8_t* to = q + rows_at[a] * width + col;
-                if (VEC && left >= 8) *reinterpret_cast<uint2*>(to) = out;
-                else if (left > 0) store_tail(to, out, left);
+                if (VEC && left >= 16) {
+                    *reinterpret_cast<uint4*>(to) = make_uint4(out[0].x, out[0].y, out[1].x, out[1].y);
+                } else if (left > 0) {
+                    store_tail(to, out[0], left);
+                    store_tail(to + 8, out[1], left - 8);
+                }
             }
         }
     }
@@ -255,11 +271,13 @@ quantize_blocks_kernel(const T* __restrict__ w, int64_t sg, int64_t sk, int64_t 
 template <typename T, bool E5M2>
 int launch_rows(const void* x, int64_t ld, int64_t rows, int64_t width, void* q, float* scale, cudaStream_t stream) {
     const int64_t blocks = ceil_div(width, kBlock), total = rows * blocks;
-    int64_t ctas = ceil_div(total, 16);
-    if (ctas > 148 * 8) ctas = 148 * 8;
-    // 16-byte loads and 8-byte stores need every row to start on such a boundary
-    const bool vec = (ld * (int64_t)sizeof(T)) % 16 == 0 && width % 8 == 0 &&
-                     (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+    int64_t ctas = ceil_div(total, 32);
+    const int sms = umma::num_sms();
+    if (sms <= 0) return BSP_ERR_CUDA;
+    if (ctas > sms * 3) ctas = sms * 3;       // what is resident at once (37 us; 24 per SM in waves: 44 us)
+    // 16-byte loads and stores need every row to start on such a boundary
+    const bool vec = (ld * (int64_t)sizeof(T)) % 16 == 0 && width % 16 == 0 &&
+                     (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
     if (vec) quantize_rows_kernel<T, E5M2, true><<<(unsigned)ctas, 256, 0, stream>>>((const T*)x, ld, (int)rows, (int)width, (int)blocks, (uint8_t*)q, scale);
     else quantize_rows_kernel<T, E5M2, false><<<(unsigned)ctas, 256, 0, stream>>>((const T*)x, ld, (int)rows, (int)width, (int)blocks, (uint8_t*)q, scale);
     BSP_LAUNCH_CHECK();

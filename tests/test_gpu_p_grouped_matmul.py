@@ -101,6 +101,21 @@ def test_odd_depths_and_columns(depth, cols):
     check_training(*make([37, 0, 300], depth, cols, FP16, seed=cols, stored="nk"))
 
 
+@pytest.mark.parametrize("stored", ["kn", "nk"])
+@pytest.mark.parametrize("depth,cols", [(512, 136), (1032, 200), (2048, 128), (4160, 72)])
+@pytest.mark.parametrize("sizes", [[1], [0, 2, 0, 1], [30, 0, 64, 1, 65], [0] * 40 + [33]], ids=str)
+def test_few_rows_split_over_the_depth(sizes, depth, cols, stored):
+    """Few tiles and a long contraction: the sums of a tile are split over two to eight thread blocks."""
+    check_training(*make(sizes, depth, cols, BF16, seed=depth, stored=stored, before=1, behind=2))
+
+
+@pytest.mark.parametrize("out_dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("depth,cols", [(1024, 136), (2064, 200), (4096, 128), (8320, 72)])
+@pytest.mark.parametrize("sizes", [[1], [0, 2, 0, 1], [30, 0, 64, 1, 65], [0] * 40 + [33]], ids=str)
+def test_scaled_few_rows_split_over_the_depth(sizes, depth, cols, out_dtype):
+    check_scaled(*make_scaled(sizes, depth, cols, seed=depth, before=1, behind=2), out_dtype)
+
+
 @pytest.mark.parametrize("before,behind", [(0, 7), (5, 0), (130, 300), (1, 1)])
 @pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=["int32", "int64"])
 def test_rows_of_no_group_are_zero(before, behind, index):
