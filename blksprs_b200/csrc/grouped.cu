@@ -690,13 +690,13 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
     if ((depth & 7) || (cols & 7) || (ld_x & 7) || (ld_w & 7) || (group_stride_w & 7) || ld_x < depth || ld_w < inner ||
         group_stride_w < 0 || (groups > 1 && group_stride_w < 8))
         return BSP_ERR_INVALID_ARG;
-    if ((st = bind_context()) != BSP_OK) return st;
     CUtensorMap ma, mb, mbs;
     const int64_t dims[3] = {inner, outer, groups};
     const int64_t strides[2] = {ld_w * 2, (groups > 1 ? group_stride_w : outer * ld_w) * 2};
     const int box[3] = {64, w_cols_inner ? 64 : kHalf, 1};
     if ((st = make_map(&ma, w, dtype, 3, dims, strides, box)) != BSP_OK) return st;
-    if ((st = rows_map(&mb, x, dtype, rows, depth, ld_x, kHalf)) != BSP_OK) return st;
+    const bool few = few_applies(rows, groups);
+    if (!few && (st = rows_map(&mb, x, dtype, rows, depth, ld_x, kHalf)) != BSP_OK) return st;
     if ((st = rows_map(&mbs, x, dtype, rows, depth, ld_x, 32)) != BSP_OK) return st;
     Params p = {};
     p.offsets = offsets;
@@ -711,7 +711,7 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
     p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((w_cols_inner ? 1u : 0u) << 15) | ((uint32_t)(kTile >> 4) << 24);
     p.status = status_word;
     cudaStream_t stream = (cudaStream_t)stream_;
-    if (few_applies(rows, groups)) {
+    if (few) {
         p.idesc = (p.idesc & 0x00ffffffu) | (128u >> 4 << 24);
         return launch_few(false, w_cols_inner != 0, ma, mbs, p, stream);
     }
@@ -733,7 +733,6 @@ extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* 
         return BSP_ERR_INVALID_ARG;
     const int64_t tiles = groups * ceil_div(depth, kTile) * ceil_div(cols, kTile);
     if (tiles > 0x7fffffffLL - 65536) return BSP_ERR_UNSUPPORTED;
-    if ((st = bind_context()) != BSP_OK) return st;
     CUtensorMap ma, mb;
     if ((st = rows_map(&ma, grad, dtype, rows, cols, ld_grad, 64)) != BSP_OK) return st;
     if ((st = rows_map(&mb, x, dtype, rows, depth, ld_x, 64)) != BSP_OK) return st;
@@ -768,14 +767,13 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
     if ((depth & 15) || (cols & 7) || (ld_x & 15) || (ld_w & 15) || (group_stride_w & 15) || ld_x < depth ||
         ld_w < depth || group_stride_w < 0 || (groups > 1 && group_stride_w < 16))
         return BSP_ERR_INVALID_ARG;
-    if ((st = bind_context()) != BSP_OK) return st;
     CUtensorMap ma, mb, mbs;
     const int64_t dims[3] = {depth, cols, groups};
     const int64_t strides[2] = {ld_w, groups > 1 ? group_stride_w : cols * ld_w};
     const int box[3] = {128, Cfg<kRows8>::kN / 2, 1}, box_small[3] = {128, 32, 1};
     if ((st = make_map(&mb, w, type_w, 3, dims, strides, box)) != BSP_OK) return st;
-    if ((st = make_map(&mbs, w, type_w, 3, dims, strides, box_small)) != BSP_OK) return st;
     const bool few = few_applies(rows, groups);
+    if (!few && (st = make_map(&mbs, w, type_w, 3, dims, strides, box_small)) != BSP_OK) return st;
     if ((st = rows_map(&ma, x, type_x, rows, depth, ld_x, few ? 32 : kHalf)) != BSP_OK) return st;
     Params p = {};
     p.offsets = offsets;

@@ -177,24 +177,25 @@ inline int make_map(CUtensorMap* map, const void* base, int elem, int rank, cons
     const CUtensorMapDataType type = elem == BSP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                    : elem == BSP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                       : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    const CUresult r = fn(map, type, rank, const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&] {
+        return fn(map, type, rank, const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
+        // the encoder is a driver call and needs the device's context current in this thread; a thread that has made
+        // no runtime call yet (the first backward of a process runs in one) does not have it
+        int dev = 0;
+        BSP_CUDA_TRY(cudaGetDevice(&dev));
+        BSP_CUDA_TRY(cudaSetDevice(dev));
+        r = encode();
+    }
     if (r != CUDA_SUCCESS) {
         char what[64];
         snprintf(what, sizeof(what), "cuTensorMapEncodeTiled: CUresult %d", (int)r);
         set_cuda_error(cudaErrorInvalidValue, what);
         return BSP_ERR_CUDA;
     }
-    return BSP_OK;
-}
-
-// The encoder is a driver call and needs the device's context current in this thread; a thread that has
-// made no runtime call yet (the first backward of a process runs in one) does not have it.
-inline int bind_context() {
-    int dev = 0;
-    BSP_CUDA_TRY(cudaGetDevice(&dev));
-    BSP_CUDA_TRY(cudaSetDevice(dev));
     return BSP_OK;
 }
 

@@ -78,8 +78,24 @@ def _validate_groups(x: Tensor, w: Tensor, group_offsets: Tensor, vector: int) -
         raise ValueError(f"Inner dimension must be divisible by {vector} and columns by 8")
 
 
+_INDEX_DTYPES = (torch.int32, torch.int64)
+
+
+def _groups_fit(x: Tensor, w: Tensor, group_offsets: Tensor, vector: int) -> bool:
+    """All of the group checks at once; the named errors are sorted out only if this fails (a call on a few rows
+    takes the GPU about as long as the checks one by one take the host)."""
+    (_, depth), (groups, w_depth, cols) = x.shape, w.shape
+    device = x.device
+    return (depth == w_depth and group_offsets.shape == (groups + 1,) and group_offsets.dtype in _INDEX_DTYPES
+            and groups <= MAX_GROUPS and depth % vector == 0 and cols % 8 == 0 and group_offsets.is_contiguous()
+            and x.is_cuda and w.device == device and group_offsets.device == device)
+
+
 def _validate(x: Tensor, w: Tensor, group_offsets: Tensor) -> None:
     if not validation_enabled():
+        return
+    if (x.dim() == 2 and w.dim() == 3 and x.dtype in _16_BIT and w.dtype is x.dtype
+            and _groups_fit(x, w, group_offsets, 8)):
         return
     validate_dimensions(x, dims=2)
     validate_dimensions(w)
@@ -101,7 +117,7 @@ def _rows_product(x: Tensor, w: Tensor, group_offsets: Tensor) -> Tensor:
     w, group_stride, ld_w, columns_inner = _weight_operand(w)
     device = x.device
     with _cabi.device_guard(device):
-        out = torch.empty((rows, cols), dtype=x.dtype, device=device)
+        out = x.new_empty((rows, cols))
         _cabi.check(_cabi.lib().bsp_grouped_matmul(
             x.data_ptr(), ld_x, w.data_ptr(), group_stride, ld_w, columns_inner, group_offsets.data_ptr(),
             group_offsets.dtype == torch.int64, rows, groups, depth, cols, out.data_ptr(),
@@ -168,7 +184,6 @@ def _grouped_matmul_eager(x, w, group_offsets):
 _grouped_matmul_no_compile = torch.compiler.disable(_grouped_matmul_eager)
 
 
-@torch.amp.custom_fwd(device_type="cuda")
 def grouped_matmul(x: Tensor, w: Tensor, group_offsets: Tensor) -> Tensor:
     """Multiplies the rows of every group with that group's matrix.
 
@@ -199,6 +214,14 @@ def _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype) -> None:
     if out_dtype not in _OUT_DTYPES:
         raise ValueError("Output dtype must be float16, bfloat16, or float32")
     if not validation_enabled():
+        return
+    if (x.dim() == 2 and w.dim() == 3 and x.dtype in _cabi.EIGHT_BIT_DTYPE_CODES
+            and w.dtype in _cabi.EIGHT_BIT_DTYPE_CODES and scale_x.dtype is torch.float32
+            and scale_w.dtype is torch.float32 and _groups_fit(x, w, group_offsets, 16)
+            and scale_x.shape == (x.size(0), _blocks_of(x.size(1)))
+            and scale_w.shape == (w.size(0), _blocks_of(w.size(1)), _blocks_of(w.size(2)))
+            and scale_x.device == x.device and scale_w.device == x.device
+            and not (scale_x.requires_grad or scale_w.requires_grad or x.requires_grad or w.requires_grad)):
         return
     validate_dimensions(x, scale_x, dims=2)
     validate_dimensions(w, scale_w)

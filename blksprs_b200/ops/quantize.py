@@ -21,6 +21,8 @@ def _validate(t: Tensor, dtype: torch.dtype, dims: int) -> None:
         raise ValueError("Output dtype must be float8_e4m3fn or float8_e5m2")
     if not validation_enabled():
         return
+    if t.dim() == dims and t.dtype in _cabi.DATA_DTYPE_CODES and t.is_cuda and not t.requires_grad:
+        return
     validate_dimensions(t, dims=dims)
     if t.dtype not in _cabi.DATA_DTYPE_CODES:
         raise ValueError("Tensor must have either float16, bfloat16, or float32 dtype")
@@ -39,8 +41,8 @@ def _quantize_rows_eager(x: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]
         x = x.contiguous()
     device = x.device
     with _cabi.device_guard(device):
-        q = torch.empty((rows, width), dtype=dtype, device=device)
-        scale = torch.empty((rows, -(-width // SCALE_BLOCK)), dtype=torch.float32, device=device)
+        q = x.new_empty((rows, width), dtype=dtype)
+        scale = x.new_empty((rows, -(-width // SCALE_BLOCK)), dtype=torch.float32)
         _cabi.check(_cabi.lib().bsp_quantize_rows(
             x.data_ptr(), x.stride(0), rows, width, _cabi.DATA_DTYPE_CODES[x.dtype], q.data_ptr(),
             _cabi.EIGHT_BIT_DTYPE_CODES[dtype], scale.data_ptr(), _cabi.stream_handle(device)), "bsp_quantize_rows")
