@@ -405,10 +405,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         // rows of the next group inside the last 16: zero them in every 64-wide atom
                         const int pieces = (mmas * KSTEP - valid) * 8;     // 16-byte pieces per atom
                         const int atoms = 2 + (n / 2 + 63) / 64;
-                        for (int i = lane; i < atoms * pieces; i += 32) {
-                            const int atom = i / pieces, at = i - atom * pieces;
-                            const uint32_t dst = (atom < 2 ? a + atom * 8192 : b + (atom - 2) * 8192) + valid * 128 + at * 16;
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+                        for (int atom = 0; atom < atoms; ++atom) {
+                            const uint32_t dst = (atom < 2 ? a + atom * 8192 : b + (atom - 2) * 8192) + valid * 128;
+                            for (int i = lane; i < pieces; i += 32)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + i * 16), "r"(0) : "memory");
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
@@ -590,7 +590,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 for (int c32 = part * 32; c32 < o.n; c32 += 64) {
                     uint32_t v[32];
                     if (computed) {
-                        tc_ld32(lanes + acc % kAccs * kN + c32, v);
+                        const uint32_t from = lanes + acc % kAccs * kN + c32;
+                        tc_ld16x32(from, v);
+                        tc_ld16x32(from + (16u << 16), v + 16);
                         tc_wait_ld();
                     } else {
 #pragma unroll

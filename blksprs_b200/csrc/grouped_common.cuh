@@ -134,18 +134,31 @@ __device__ __forceinline__ void store_staged(uint32_t staging, char* out, int64_
     __syncwarp();
 }
 
-// v = 32 accumulator columns of one warp, lane = output column, column = output row: packs neighbouring
-// output columns (neighbouring lanes) into words; even lanes keep even rows, odd lanes odd rows.
+// 16 lanes x 32 columns of tensor memory as four 8-column groups: r[4g], r[4g + 1] = lane t / 4, columns
+// 8g + 2 (t mod 4) + {0, 1}; r[4g + 2], r[4g + 3] = lane t / 4 + 8, same columns.
+__device__ __forceinline__ void tc_ld16x32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
+
+// 32 lanes (output columns) x 32 accumulator columns (output rows) as two tc_ld16x32 deliver them: the pairs a thread
+// holds are 8 x 8 matrices of neighbouring rows, stored transposed, so that a staged row is 32 neighbouring output
+// columns.  (Exchanging words between lanes and storing them one by one took 40 instead of 12 shared-memory and
+// shuffle instructions for the same 2 KiB.)
 template <typename T>
 __device__ __forceinline__ void stage_transposed(uint32_t staging, const float* v) {
-    const int lane = threadIdx.x & 31, odd = lane & 1;
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const uint32_t mine = pack2<T>(v[2 * j], v[2 * j + 1]);      // rows 2j, 2j + 1 of this column
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-        const uint32_t word = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
-        const int row = 2 * j + odd;
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(staging + staged_at(row, lane >> 3) + ((lane >> 1) & 3) * 4), "r"(word) : "memory");
+    for (int g = 0; g < 4; ++g) {
+        const uint32_t at = staging + staged_at(8 * g + (lane & 7), lane >> 3);
+        asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+                     ::"r"(at), "r"(pack2<T>(v[4 * g], v[4 * g + 1])), "r"(pack2<T>(v[4 * g + 2], v[4 * g + 3])),
+                       "r"(pack2<T>(v[16 + 4 * g], v[16 + 4 * g + 1])), "r"(pack2<T>(v[16 + 4 * g + 2], v[16 + 4 * g + 3]))
+                     : "memory");
     }
 }
 

@@ -313,8 +313,14 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (h * 32 < n) {
+                        // stored by this CTA: as stage_transposed takes them; else a column per lane
                         uint32_t v[32];
-                        tc_ld32(lanes + h * 32, v);
+                        if (split == 1) {
+                            tc_ld16x32(lanes + h * 32, v);
+                            tc_ld16x32(lanes + h * 32 + (16u << 16), v + 16);
+                        } else {
+                            tc_ld32(lanes + h * 32, v);
+                        }
                         tc_wait_ld();
 #pragma unroll
                         for (int j = 0; j < 32; ++j) sum[h][j] = __uint_as_float(v[j]);
@@ -330,11 +336,17 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (h * 32 < rows) {
-                    if (p.out_dtype == BSP_F32) {
+                    if (F8) {
+                        // a column per lane: 64 bytes (fp32: 128) of a row per warp and store
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (h * 32 + j < rows && c + lane < p.cols)
-                                *reinterpret_cast<float*>(out + (h * 32 + j) * row_bytes + lane * 4) = sum[h][j];
+                        for (int j = 0; j < 32; ++j) {
+                            char* at = out + (h * 32 + j) * row_bytes + lane * esize;
+                            if (h * 32 + j < rows && c + lane < p.cols) {
+                                if (p.out_dtype == BSP_F32) *reinterpret_cast<float*>(at) = sum[h][j];
+                                else if (p.out_dtype == BSP_F16) *reinterpret_cast<__half*>(at) = __float2half_rn(sum[h][j]);
+                                else *reinterpret_cast<__nv_bfloat16*>(at) = __float2bfloat16_rn(sum[h][j]);
+                            }
+                        }
                     } else {
                         if (p.out_dtype == BSP_F16) stage_transposed<__half>(staging, sum[h]);
                         else stage_transposed<__nv_bfloat16>(staging, sum[h]);
