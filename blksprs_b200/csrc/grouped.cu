@@ -44,7 +44,7 @@ namespace {
 
 constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
-constexpr int kTile = 256;            // M of a pair's tile (and N, 16 bits)
+constexpr int kTile = 256;            // M of a pair's tile, and most of an MMA's N
 constexpr int kHalf = 128;            // M in either CTA
 constexpr int kScaleSlots = 4;        // groups of four steps whose scales are staged ahead
 constexpr int kScaleSlot = 4 * kHalf + 8;   // floats of a slot: four per row of the CTA's half, four of either block of w
@@ -52,21 +52,22 @@ constexpr int kBand = 8;              // row tiles that are walked together for 
 
 enum Mode { kRows16, kGrad16, kRows8 };
 
-// N of a tile, accumulators in tensor memory (512 columns in all), ring stages.  (8 bits with four accumulators of
+// N of an MMA, accumulators in tensor memory (512 columns in all), the most of them a tile takes, ring stages.  (8 bits with four accumulators of
 // N = 128 instead: 389 against 310 us on 16 groups of 1024 rows, 4096 x 4096; the hand-over of an accumulator
 // costs about the same whatever its width.)
-template <int MODE> struct Cfg { static constexpr int kN = 256, kAccs = 2, kStages = 6; };
+constexpr int kN = 256, kAccs = 2;
+constexpr int ring_stages(int halves) { return halves == 2 ? 4 : 6; }
 
-template <int MODE>
+template <int MODE, int HALVES>
 struct Smem {
-    static constexpr int kStages = Cfg<MODE>::kStages;
-    static constexpr int kABytes = kHalf * 128, kBBytes = Cfg<MODE>::kN / 2 * 128;
-    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kStages = ring_stages(HALVES);
+    static constexpr int kABytes = kHalf * 128, kBBytes = kN / 2 * 128;       // of one half
+    static constexpr int kStageBytes = kABytes + HALVES * kBBytes;
     static constexpr int kData = kStages * kStageBytes;
     static constexpr int kStaging = kEpiWarps * 2048;
     static constexpr int kTable = (2 * (kMaxGroups + 1) * 4 + 7) & ~7;
     static constexpr int kScales = MODE == kRows8 ? kScaleSlots * kScaleSlot * 4 : 0;
-    static constexpr int kBars = (3 * kStages + 2 * Cfg<MODE>::kAccs + 1 + 2 * kScaleSlots) * 8;
+    static constexpr int kBars = (3 * kStages + 2 * kAccs + 1 + 2 * kScaleSlots) * 8;
     static constexpr int kTotal = kData + kStaging + kTable + kScales + kBars + 1024;
 };
 
@@ -74,7 +75,7 @@ struct Tile {
     int group;
     int r0, rows;    // first output row (of the whole output, or of the group's output), rows to store
     int c0, cols;    // first output column, columns to store
-    int n;           // N of the MMA
+    int n;           // accumulator columns, in two halves if more than kTile
     int t0;          // weight gradient: first contraction row
     int depth;       // contraction length
 };
@@ -98,10 +99,11 @@ __device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* ma
 // STEP_A / STEP_B: descriptor distance (16-byte units) of neighbouring MMAs.
 #define BSP_PAIR_MMA(KIND)                                                                                     \
     asm volatile(                                                                                              \
-        "{\n\t.reg .pred p, t, e, f;\n\t.reg .b64 a, b;\n\t"                                                 \
+        "{\n\t.reg .pred p, t, e, f, r;\n\t.reg .b64 a, b;\n\t"                                                 \
         "elect.sync _|e, 0xffffffff;\n\t"                                                                     \
         "setp.ne.b32 p, %4, 0;\n\t"                                                                           \
         "setp.ne.and.b32 f, %7, 0, e;\n\t"                                                                    \
+        "setp.ne.and.b32 r, %11, 0, e;\n\t"                                                                   \
         "setp.eq.b32 t, 0, 0;\n\t"                                                                            \
         "@e tcgen05.mma.cta_group::2.kind::" KIND " [%0], %1, %2, %3, p;\n\t"                                 \
         "add.s64 a, %1, %8;\n\tadd.s64 b, %2, %9;\n\t"                                                       \
@@ -110,14 +112,14 @@ __device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* ma
         "@e tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %3, t;\n\t"                                   \
         "add.s64 a, a, %8;\n\tadd.s64 b, b, %9;\n\t"                                                         \
         "@e tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %3, t;\n\t"                                   \
-        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], %10;\n\t" \
+        "@r tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], %10;\n\t" \
         "@f tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%6], %10;\n\t}" \
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(release_bar), "r"(done_bar),   \
-          "r"(done), "n"(STEP_A), "n"(STEP_B), "h"((uint16_t)3) : "memory")
+          "r"(done), "n"(STEP_A), "n"(STEP_B), "h"((uint16_t)3), "r"(release) : "memory")
 template <bool F8, int STEP_A, int STEP_B>
 __device__ __forceinline__ void pair_mma_entry(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                               uint32_t accumulate, uint32_t release_bar, uint32_t done_bar,
-                                               uint32_t done) {
+                                               uint32_t accumulate, uint32_t release_bar, uint32_t release,
+                                               uint32_t done_bar, uint32_t done) {
     if (F8) BSP_PAIR_MMA("f8f6f4");
     else BSP_PAIR_MMA("f16");
 }
@@ -149,19 +151,25 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
         ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
-// 16 bits: the rows of a group are cut into the fewest tiles of at most kTile rows, all of about the same height.
-__device__ __forceinline__ int tile_height(int m) {
-    const int n = (m + kTile - 1) / kTile;
+// 16 bits: the rows of a group are cut into the fewest tiles of at most `most` rows, all of about the same height.
+__device__ __forceinline__ int tile_height(int m, int most) {
+    const int n = (m + most - 1) / most;
     return n == 0 ? 0 : round_up((m + n - 1) / n, 32);
 }
+// N of either half's MMAs.
+__device__ __forceinline__ int half_n(int n, int half) {
+    const int first = n <= kTile ? n : round_up(n / 2, 32);
+    return half ? n - first : first;
+}
 
-template <int MODE, bool A_MN>
+// HALVES: accumulators a tile may take (16 bits: 256 or 512 rows; 8 bits: one).
+template <int MODE, bool A_MN, int HALVES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CUtensorMap map_b_small, const Params p) {
-    using L = Smem<MODE>;
+    using L = Smem<MODE, HALVES>;
+    constexpr int kHalves = HALVES;
     constexpr int kStages = L::kStages, kStageBytes = L::kStageBytes, kABytes = L::kABytes, kBBytes = L::kBBytes;
-    constexpr int kN = Cfg<MODE>::kN, kAccs = Cfg<MODE>::kAccs;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
     const uint32_t data = (raw + 1023u) & ~1023u;
@@ -226,6 +234,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const uint32_t tmem = uniform(tmem_slot);
     constexpr int kTileCols = MODE == kRows8 ? kN : kTile;       // of the output
     const int c_tiles = (p.cols + kTileCols - 1) / kTileCols;
+    constexpr int tile_rows = HALVES * kTile;
     if (warp == 0) {
         int high = 0, before = 0;
         for (int base = 0; base <= p.groups; base += 32) {
@@ -246,7 +255,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             for (int base = 0; base < p.groups; base += 32) {
                 const int i = base + lane;
                 int n = 0;
-                if (i < p.groups) n = (row_start[i + 1] - row_start[i] + kTile - 1) / kTile * c_tiles;
+                if (i < p.groups) n = (row_start[i + 1] - row_start[i] + tile_rows - 1) / tile_rows * c_tiles;
                 const int own = n;
                 for (int d = 1; d < 32; d <<= 1) {
                     const int o = __shfl_up_sync(0xffffffffu, n, d);
@@ -261,7 +270,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     __syncthreads();
     cluster_sync();      // the other CTA's barriers and tensor memory are ready
 
-    const int r_tiles_all = (p.out_rows + kTile - 1) / kTile;
+    const int r_tiles_all = (p.out_rows + tile_rows - 1) / tile_rows;
     const int n_tiles = uniform(MODE != kGrad16 ? tile_start[p.groups] : p.groups * c_tiles * r_tiles_all);
     const int first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
 
@@ -276,7 +285,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             }
             o.group = lo;
             local = t - tile_start[lo];
-            r_tiles = (row_start[lo + 1] - row_start[lo] + kTile - 1) / kTile;
+            r_tiles = (row_start[lo + 1] - row_start[lo] + tile_rows - 1) / tile_rows;
         } else {
             r_tiles = r_tiles_all;
             o.group = t / (c_tiles * r_tiles);
@@ -290,12 +299,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         o.cols = min(kTileCols, p.cols - o.c0);
         const int first = row_start[o.group], m = row_start[o.group + 1] - first;
         if (MODE == kGrad16) {
-            o.r0 = r * kTile;
-            o.rows = min(kTile, p.out_rows - o.r0);
+            const int h = tile_height(p.out_rows, tile_rows);
+            o.r0 = r * h;
+            o.rows = min(h, p.out_rows - o.r0);
             o.t0 = first;
             o.depth = m;
         } else {
-            const int h = MODE == kRows16 ? tile_height(m) : kTile;
+            const int h = MODE == kRows16 ? tile_height(m, tile_rows) : kTile;
             o.r0 = first + r * h;
             o.rows = min(h, m - r * h);
             o.t0 = 0;
@@ -316,10 +326,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 bool alive = true;
                 for (int t = first_tile; t < n_tiles && alive; t += tile_step) {
                     const Tile o = tile_at(t);
-                    const int half = o.n / 2;
                     const int steps = (o.depth + KE - 1) / KE;
-                    // bytes of B one CTA copies
-                    const int b_bytes = B_MN ? (half + 63) / 64 * 8192 : half == kN / 2 ? kBBytes : (half + 31) / 32 * 4096;
+                    // rows of B one CTA copies for either half, and their bytes
+                    const int share[2] = {half_n(o.n, 0) / 2, half_n(o.n, 1) / 2};
+                    int b_bytes = 0;
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h)
+                        b_bytes += B_MN ? (share[h] + 63) / 64 * 8192 : share[h] == kN / 2 ? kBBytes : (share[h] + 31) / 32 * 4096;
                     for (int k = 0; k < steps; ++k, ++it) {
                         const uint32_t s = it % kStages;
                         if (it >= kStages &&
@@ -340,32 +353,32 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                             mbar_arrive_expect_tx(full_bar + 8 * s, kABytes + b_bytes);
                             ++issued_tails[s];
                         }
-                        if (MODE == kRows16) {
-                            const int m0 = o.c0 + rank * kHalf, n0 = o.r0 + rank * half;
-                            if (A_MN) {
-                                pair_load_3d(a, &map_a, m0, k * KE, o.group, bar);
-                                pair_load_3d(a + 8192, &map_a, m0 + 64, k * KE, o.group, bar);
-                            } else {
-                                pair_load_3d(a, &map_a, k * KE, m0, o.group, bar);
-                            }
-                            if (half == kN / 2) {
-                                pair_load_2d(b, &map_b, k * KE, n0, bar);
-                            } else {
-                                for (int r = 0; r < half; r += 32) pair_load_2d(b + r * 128, &map_b_small, k * KE, n0 + r, bar);
-                            }
-                        } else if (MODE == kRows8) {
-                            const int m0 = o.r0 + rank * kHalf, n0 = o.c0 + rank * half;
-                            pair_load_2d(a, &map_a, k * KE, m0, bar);
-                            if (half == kN / 2) {
-                                pair_load_3d(b, &map_b, k * KE, n0, o.group, bar);
-                            } else {
-                                for (int r = 0; r < half; r += 32) pair_load_3d(b + r * 128, &map_b_small, k * KE, n0 + r, o.group, bar);
-                            }
+                        if (MODE == kRows8) {
+                            pair_load_2d(a, &map_a, k * KE, o.r0 + rank * kHalf, bar);
+                        } else if (MODE == kGrad16) {
+                            pair_load_2d(a, &map_a, o.c0 + rank * kHalf, o.t0 + k * KE, bar);
+                            pair_load_2d(a + 8192, &map_a, o.c0 + rank * kHalf + 64, o.t0 + k * KE, bar);
+                        } else if (A_MN) {
+                            pair_load_3d(a, &map_a, o.c0 + rank * kHalf, k * KE, o.group, bar);
+                            pair_load_3d(a + 8192, &map_a, o.c0 + rank * kHalf + 64, k * KE, o.group, bar);
                         } else {
-                            const int m0 = o.c0 + rank * kHalf, n0 = o.r0 + rank * half, t0 = o.t0 + k * KE;
-                            pair_load_2d(a, &map_a, m0, t0, bar);
-                            pair_load_2d(a + 8192, &map_a, m0 + 64, t0, bar);
-                            for (int r = 0; r < half; r += 64) pair_load_2d(b + r * 128, &map_b, n0 + r, t0, bar);
+                            pair_load_3d(a, &map_a, k * KE, o.c0 + rank * kHalf, o.group, bar);
+                        }
+#pragma unroll
+                        for (int h = 0; h < kHalves; ++h) {
+                            const uint32_t to = b + h * kBBytes;
+                            const int from = (MODE == kRows8 ? o.c0 : o.r0) + (h ? 2 * share[0] : 0) + rank * share[h];
+                            if (B_MN) {
+                                for (int r = 0; r < share[h]; r += 64) pair_load_2d(to + r * 128, &map_b, from + r, o.t0 + k * KE, bar);
+                            } else if (MODE == kRows8) {
+                                if (share[h] == kN / 2) pair_load_3d(to, &map_b, k * KE, from, o.group, bar);
+                                else
+                                    for (int r = 0; r < share[h]; r += 32) pair_load_3d(to + r * 128, &map_b_small, k * KE, from + r, o.group, bar);
+                            } else {
+                                if (share[h] == kN / 2) pair_load_2d(to, &map_b, k * KE, from, bar);
+                                else
+                                    for (int r = 0; r < share[h]; r += 32) pair_load_2d(to + r * 128, &map_b_small, k * KE, from + r, bar);
+                            }
                         }
                     }
                 }
@@ -383,7 +396,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 const Tile o = tile_at(t);
                 const int depth = uniform(o.depth), n = uniform(o.n);
                 const int steps = (depth + KE - 1) / KE;
-                const uint32_t idesc = p.idesc | ((uint32_t)(n >> 3) << 17);
+                const int halves = kHalves > 1 && n > kTile ? 2 : 1;
                 for (int k = 0; k < steps; ++k, ++it) {
                     const uint32_t s = it % kStages;
                     const uint32_t a = data + s * kStageBytes, b = a + kABytes;
@@ -391,11 +404,6 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     const int mmas = (valid + KSTEP - 1) / KSTEP;
                     const bool zero_rows = MODE == kGrad16 && (valid & (KSTEP - 1));
                     if (rank == 0) {
-                        // a new accumulator: per tile, and for 8-bit operands per step (every step has its own scales)
-                        if (F8 || k == 0) {
-                            alive = acc < kAccs || wait_all(tempty_bar + 8 * (acc % kAccs), (acc / kAccs - 1) & 1, abort_flag, p.status);
-                            if (!alive) break;
-                        }
                         alive = wait_all(full_bar + 8 * s, (it / kStages) & 1, abort_flag, p.status);
                     } else if (zero_rows) {
                         alive = wait_all(full_bar + 8 * s, (tail_parity >> s) & 1, abort_flag, p.status);
@@ -404,40 +412,53 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     if (zero_rows) {
                         // rows of the next group inside the last 16: zero them in every 64-wide atom
                         const int pieces = (mmas * KSTEP - valid) * 8;     // 16-byte pieces per atom
-                        const int atoms = 2 + (n / 2 + 63) / 64;
-                        for (int atom = 0; atom < atoms; ++atom) {
-                            const uint32_t dst = (atom < 2 ? a + atom * 8192 : b + (atom - 2) * 8192) + valid * 128;
+                        const int atoms = 2 + (half_n(n, 0) / 2 + 63) / 64, more = (half_n(n, 1) / 2 + 63) / 64;
+                        for (int atom = 0; atom < atoms + more; ++atom) {
+                            const uint32_t dst = (atom < 2 ? a + atom * 8192 : atom < atoms ? b + (atom - 2) * 8192
+                                                                                             : b + kBBytes + (atom - atoms) * 8192) + valid * 128;
                             for (int i = lane; i < pieces; i += 32)
                                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + i * 16), "r"(0) : "memory");
                         }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        // what is zeroed here is read by this SM's tensor core only: visible to it after the proxy fence,
+                        // and the first CTA issues the MMA after this CTA's arrival
+                        asm volatile("fence.proxy.async;" ::: "memory");
                         __syncwarp();
                         if (rank == 1) {
-                            if (lane == 0) mbar_arrive_release_cluster(map_to_rank(zeroed_bar + 8 * s, 0));
+                            if (lane == 0) mbar_arrive_pair(map_to_rank(zeroed_bar + 8 * s, 0));
                         } else {
                             alive = wait_all(zeroed_bar + 8 * s, (tail_parity >> s) & 1, abort_flag, p.status);
                             if (!alive) break;
-                            acquire_cluster();
                         }
                         tail_parity ^= 1u << s;
                     }
                     if (rank == 0) {
-                        tc_fence_after();
-                        const uint32_t d = tmem + acc % kAccs * kN;
                         const uint64_t ad = A_MN ? make_smem_desc(a, 8192, 1024) : make_smem_desc(a, 16, 1024);
-                        const uint64_t bd = B_MN ? make_smem_desc(b, 8192, 1024) : make_smem_desc(b, 16, 1024);
                         constexpr int STEP_A = A_MN ? 128 : 2, STEP_B = B_MN ? 128 : 2;
                         const bool done = F8 || k == steps - 1;
-                        if (mmas == 4) {
-                            pair_mma_entry<F8, STEP_A, STEP_B>(d, ad, bd, idesc, !F8 && k > 0, empty_bar + 8 * s,
-                                                               tfull_bar + 8 * (acc % kAccs), done);
-                        } else {
-                            for (int kk = 0; kk < mmas; ++kk)
-                                pair_mma<F8>(d, ad + kk * STEP_A, bd + kk * STEP_B, idesc, kk > 0 || (!F8 && k > 0));
-                            pair_commit(empty_bar + 8 * s);
-                            if (done) pair_commit(tfull_bar + 8 * (acc % kAccs));
+                        for (int h = 0; h < halves; ++h) {
+                            // a new accumulator: per tile, and for 8-bit operands per step (every step has its own scales)
+                            const uint32_t at = acc + h, slot = at % kAccs;
+                            if (F8 || k == 0) {
+                                alive = at < kAccs || wait_all(tempty_bar + 8 * slot, (at / kAccs - 1) & 1, abort_flag, p.status);
+                                if (!alive) break;
+                            }
+                            tc_fence_after();
+                            const uint32_t d = tmem + slot * kN, bh = b + h * kBBytes;
+                            const uint32_t idesc = p.idesc | ((uint32_t)(half_n(n, h) >> 3) << 17);
+                            const uint64_t bd = B_MN ? make_smem_desc(bh, 8192, 1024) : make_smem_desc(bh, 16, 1024);
+                            const bool last = h == halves - 1;
+                            if (mmas == 4) {
+                                pair_mma_entry<F8, STEP_A, STEP_B>(d, ad, bd, idesc, !F8 && k > 0, empty_bar + 8 * s, last,
+                                                                   tfull_bar + 8 * slot, done);
+                            } else {
+                                for (int kk = 0; kk < mmas; ++kk)
+                                    pair_mma<F8>(d, ad + kk * STEP_A, bd + kk * STEP_B, idesc, kk > 0 || (!F8 && k > 0));
+                                if (last) pair_commit(empty_bar + 8 * s);
+                                if (done) pair_commit(tfull_bar + 8 * slot);
+                            }
                         }
-                        if (F8 || k == steps - 1) ++acc;
+                        if (!alive) break;
+                        if (done) acc += halves;
                     }
                 }
             }
@@ -581,33 +602,53 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 char* out = (char*)p.out + first * row_bytes + (int64_t)c * 2;
                 const int bytes = (p.cols - c) * 2;
                 const bool computed = steps > 0;    // a group without rows has a gradient of zero
-                if (computed) {
-                    alive = wait_all(tfull_bar + 8 * (acc % kAccs), (acc / kAccs) & 1, abort_flag, p.status);
-                    if (!alive) break;
-                    tc_fence_after();
-                }
 #pragma unroll 1
-                for (int c32 = part * 32; c32 < o.n; c32 += 64) {
-                    uint32_t v[32];
+                for (int h = 0; h < kHalves; ++h) {
+                    const int n = half_n(o.n, h), above = h ? half_n(o.n, 0) : 0;
+                    if (n == 0) break;
+                    // first everything out of tensor memory, as packed words, so that the accumulator is free again
+                    // (the next tile's MMAs wait for it); then through the staging area into rows
+                    uint32_t words[4][16];
                     if (computed) {
-                        const uint32_t from = lanes + acc % kAccs * kN + c32;
-                        tc_ld16x32(from, v);
-                        tc_ld16x32(from + (16u << 16), v + 16);
-                        tc_wait_ld();
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = 0;
+                        alive = wait_all(tfull_bar + 8 * (acc % kAccs), (acc / kAccs) & 1, abort_flag, p.status);
+                        if (!alive) break;
+                        tc_fence_after();
                     }
-                    const float* f = reinterpret_cast<const float*>(v);
-                    if (p.out_dtype == BSP_F16) stage_transposed<__half>(staging, f);
-                    else stage_transposed<__nv_bfloat16>(staging, f);
-                    store_staged(staging, out + c32 * row_bytes, row_bytes, o.rows - c32, bytes);
-                }
-                if (computed) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_pair(tempty_first + 8 * (acc % kAccs));
-                    ++acc;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int c32 = part * 32 + i * 64;
+                        if (c32 < n) {
+                            uint32_t v[32];
+                            if (computed) {
+                                const uint32_t from = lanes + acc % kAccs * kN + c32;
+                                tc_ld16x32(from, v);
+                                tc_ld16x32(from + (16u << 16), v + 16);
+                                tc_wait_ld();
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) v[j] = 0;
+                            }
+                            const float* f = reinterpret_cast<const float*>(v);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                words[i][j] = p.out_dtype == BSP_F16 ? pack2<__half>(f[2 * j], f[2 * j + 1])
+                                                                     : pack2<__nv_bfloat16>(f[2 * j], f[2 * j + 1]);
+                        }
+                    }
+                    if (computed) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_pair(tempty_first + 8 * (acc % kAccs));
+                        ++acc;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int c32 = part * 32 + i * 64;
+                        if (c32 < n) {
+                            stage_transposed(staging, words[i]);
+                            store_staged(staging, out + (above + c32) * row_bytes, row_bytes, o.rows - above - c32, bytes);
+                        }
+                    }
                 }
             }
         }
@@ -638,30 +679,38 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 
 // ---- host side ---------------------------------------------------------------------
 
-template <int MODE, bool A_MN>
+template <int MODE, bool A_MN, int HALVES>
 int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mbs, const Params& p, int64_t most_tiles,
            cudaStream_t stream) {
-    auto kern = grouped_kernel<MODE, A_MN>;
+    auto kern = grouped_kernel<MODE, A_MN, HALVES>;
     static std::atomic<uint64_t> opted_in{0};
     int dev = 0;
     BSP_CUDA_TRY(cudaGetDevice(&dev));
     const uint64_t dev_bit = dev >= 0 && dev < 64 ? (1ull << dev) : 0;
     if (!(opted_in.load(std::memory_order_acquire) & dev_bit)) {
-        BSP_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<MODE>::kTotal));
+        BSP_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<MODE, HALVES>::kTotal));
         opted_in.fetch_or(dev_bit, std::memory_order_release);
     }
     const int pairs = num_sms() / 2;
     if (pairs <= 0) return BSP_ERR_CUDA;
     const int ctas = 2 * (int)(most_tiles < pairs ? (most_tiles < 1 ? 1 : most_tiles) : pairs);
-    kern<<<ctas, kThreads, Smem<MODE>::kTotal, stream>>>(ma, mb, mbs, p);
+    kern<<<ctas, kThreads, Smem<MODE, HALVES>::kTotal, stream>>>(ma, mb, mbs, p);
     BSP_LAUNCH_CHECK();
     return BSP_OK;
 }
 
-// Tiles of a rows product: a group of m rows has ceil(m / kTile) <= m / kTile + 1 row tiles, and no more
-// groups than rows have any.
-int64_t most_row_tiles(int64_t rows, int64_t groups) {
-    return rows / kTile + (groups < rows ? groups : rows);
+// Tiles of a rows product: a group of m rows has ceil(m / height) <= m / height + 1 row tiles, and no more groups
+// than rows have any.
+int64_t most_row_tiles(int64_t rows, int64_t groups, int64_t height) {
+    return rows / height + (groups < rows ? groups : rows);
+}
+
+// Accumulators of a 16-bit tile.  Two: A is staged once for both, 24 KiB per CTA and 512 cycles of MMAs instead of
+// 32 (what L2 delivers, about 55 bytes per cycle and SM, is what bounds the ring); one where two would leave the
+// pairs fewer than four tiles each, or where the mean group would not fill them (192 rows: 71 / 81 us).  Measured, one / two: 16 groups of 1024 rows, 2048 x 4096: 248 / 239 us; weight
+// gradient of 8 groups of 2048 rows, 4096 x 4096: 534 / 415 us; 33 groups of 60 rows, 1032 x 1496: 39 / 43 us.
+int tile_halves(int64_t tiles_of_two, int64_t rows, int64_t groups) {
+    return tiles_of_two >= 4 * (num_sms() / 2) && rows >= 384 * (groups < rows ? groups : rows) ? 2 : 1;
 }
 
 int check_sizes(int64_t rows, int64_t groups, int64_t depth, int64_t cols, const void* offsets) {
@@ -697,7 +746,7 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
     const int64_t strides[2] = {ld_w * 2, (groups > 1 ? group_stride_w : outer * ld_w) * 2};
     const int box[3] = {64, w_cols_inner ? 64 : kHalf, 1};
     if ((st = make_map(&ma, w, dtype, 3, dims, strides, box)) != BSP_OK) return st;
-    const bool few = few_applies(rows, groups);
+    const bool few = few_applies(rows, groups, cols);
     if (!few && (st = rows_map(&mb, x, dtype, rows, depth, ld_x, kHalf)) != BSP_OK) return st;
     if ((st = rows_map(&mbs, x, dtype, rows, depth, ld_x, 32)) != BSP_OK) return st;
     Params p = {};
@@ -717,9 +766,13 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
         p.idesc = (p.idesc & 0x00ffffffu) | (128u >> 4 << 24);
         return launch_few(false, w_cols_inner != 0, ma, mbs, p, stream);
     }
-    const int64_t tiles = most_row_tiles(rows, groups) * ceil_div(cols, kTile);
-    return w_cols_inner ? launch<kRows16, true>(ma, mb, mbs, p, tiles, stream)
-                        : launch<kRows16, false>(ma, mb, mbs, p, tiles, stream);
+    const int halves = tile_halves(most_row_tiles(rows, groups, 2 * kTile) * ceil_div(cols, kTile), rows, groups);
+    const int64_t tiles = most_row_tiles(rows, groups, halves * kTile) * ceil_div(cols, kTile);
+    if (w_cols_inner)
+        return halves == 2 ? launch<kRows16, true, 2>(ma, mb, mbs, p, tiles, stream)
+                           : launch<kRows16, true, 1>(ma, mb, mbs, p, tiles, stream);
+    return halves == 2 ? launch<kRows16, false, 2>(ma, mb, mbs, p, tiles, stream)
+                       : launch<kRows16, false, 1>(ma, mb, mbs, p, tiles, stream);
 }
 
 extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* grad, int64_t ld_grad,
@@ -750,7 +803,9 @@ extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* 
     const uint32_t fmt = dtype == BSP_BF16 ? 1u : 0u;
     p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(kTile >> 4) << 24);
     p.status = status_word;
-    return launch<kGrad16, true>(ma, mb, mb, p, tiles, (cudaStream_t)stream_);
+    const bool two = tile_halves(groups * ceil_div(depth, 2 * kTile) * ceil_div(cols, kTile), rows, groups) == 2;
+    return two ? launch<kGrad16, true, 2>(ma, mb, mb, p, tiles, (cudaStream_t)stream_)
+               : launch<kGrad16, true, 1>(ma, mb, mb, p, tiles, (cudaStream_t)stream_);
 }
 
 extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x, const float* scale_x,
@@ -772,9 +827,9 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
     CUtensorMap ma, mb, mbs;
     const int64_t dims[3] = {depth, cols, groups};
     const int64_t strides[2] = {ld_w, groups > 1 ? group_stride_w : cols * ld_w};
-    const int box[3] = {128, Cfg<kRows8>::kN / 2, 1}, box_small[3] = {128, 32, 1};
+    const int box[3] = {128, kN / 2, 1}, box_small[3] = {128, 32, 1};
     if ((st = make_map(&mb, w, type_w, 3, dims, strides, box)) != BSP_OK) return st;
-    const bool few = few_applies(rows, groups);
+    const bool few = few_applies(rows, groups, cols);
     if (!few && (st = make_map(&mbs, w, type_w, 3, dims, strides, box_small)) != BSP_OK) return st;
     if ((st = rows_map(&ma, x, type_x, rows, depth, ld_x, few ? 32 : kHalf)) != BSP_OK) return st;
     Params p = {};
@@ -802,6 +857,6 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
                   (128u >> 4 << 24);
         return launch_few(true, false, mb, ma, p, (cudaStream_t)stream_);
     }
-    const int64_t tiles = most_row_tiles(rows, groups) * ceil_div(cols, Cfg<kRows8>::kN);
-    return launch<kRows8, false>(ma, mb, mbs, p, tiles, (cudaStream_t)stream_);
+    const int64_t tiles = most_row_tiles(rows, groups, kTile) * ceil_div(cols, kN);
+    return launch<kRows8, false, 1>(ma, mb, mbs, p, tiles, (cudaStream_t)stream_);
 }

@@ -52,9 +52,6 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
 // mbar_wait without a call: a call would have the epilogue's sums saved around it.
 __device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
                                              bool honor_abort = true) {
@@ -106,9 +103,6 @@ __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile
         }
     }
 }
-// Orders what the other CTA wrote before its arrival (the barrier's wait acquires for this CTA only).
-__device__ __forceinline__ void acquire_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
-
 // A value all lanes of a converged warp hold, told to the compiler: MMA operands then live in uniform registers.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
@@ -149,15 +143,14 @@ __device__ __forceinline__ void tc_ld16x32(uint32_t taddr, uint32_t* r) {
 // holds are 8 x 8 matrices of neighbouring rows, stored transposed, so that a staged row is 32 neighbouring output
 // columns.  (Exchanging words between lanes and storing them one by one took 40 instead of 12 shared-memory and
 // shuffle instructions for the same 2 KiB.)
-template <typename T>
-__device__ __forceinline__ void stage_transposed(uint32_t staging, const float* v) {
+// words: v[2j], v[2j + 1] packed, in that order.
+__device__ __forceinline__ void stage_transposed(uint32_t staging, const uint32_t* words) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         const uint32_t at = staging + staged_at(8 * g + (lane & 7), lane >> 3);
         asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
-                     ::"r"(at), "r"(pack2<T>(v[4 * g], v[4 * g + 1])), "r"(pack2<T>(v[4 * g + 2], v[4 * g + 3])),
-                       "r"(pack2<T>(v[16 + 4 * g], v[16 + 4 * g + 1])), "r"(pack2<T>(v[16 + 4 * g + 2], v[16 + 4 * g + 3]))
+                     ::"r"(at), "r"(words[2 * g]), "r"(words[2 * g + 1]), "r"(words[8 + 2 * g]), "r"(words[8 + 2 * g + 1])
                      : "memory");
     }
 }
@@ -226,7 +219,7 @@ inline int rows_map(CUtensorMap* map, const void* base, int elem, int64_t rows, 
 // Product of few rows per group (grouped_few.cu); same operands as the products it stands in for.
 int launch_few(bool f8, bool a_mn, const CUtensorMap& weights, const CUtensorMap& rows_small, const Params& p,
                cudaStream_t stream);
-bool few_applies(int64_t rows, int64_t groups);
+bool few_applies(int64_t rows, int64_t groups, int64_t cols);
 
 }  // namespace grouped
 }  // namespace bsp

@@ -348,8 +348,12 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                             }
                         }
                     } else {
-                        if (p.out_dtype == BSP_F16) stage_transposed<__half>(staging, sum[h]);
-                        else stage_transposed<__nv_bfloat16>(staging, sum[h]);
+                        uint32_t words[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            words[j] = p.out_dtype == BSP_F16 ? pack2<__half>(sum[h][2 * j], sum[h][2 * j + 1])
+                                                              : pack2<__nv_bfloat16>(sum[h][2 * j], sum[h][2 * j + 1]);
+                        stage_transposed(staging, words);
                         store_staged(staging, out + h * 32 * row_bytes, row_bytes, rows - h * 32, (p.cols - c) * 2);
                     }
                 }
@@ -441,9 +445,14 @@ int launch_kernel(const CUtensorMap& weights, const CUtensorMap& rows_small, con
 
 }  // namespace
 
-bool few_applies(int64_t rows, int64_t groups) {
+// Which of the two: by the mean rows of the groups that can have rows.  Measured (us, few / pairs; 2048 x 1024 bf16, 64
+// groups): 48 rows 52 / 61, 64 rows 57 / 65, 96 rows 68 / 66; 32 groups of 1024 x 2048: 48 rows 33 / 35, 64 rows 35 / 36, 96
+// rows 42 / 37; 8 groups of 2048 x 2048: 32 rows 19 / 20, 48 rows 23 / 20.  Where the pairs would have less than half a
+// tile each, splitting the depth pays longer: one group of 4096 x 4096: 64 rows 15 / 29, 96 rows 22 / 34 (8 bits 20 / 20).
+bool few_applies(int64_t rows, int64_t groups, int64_t cols) {
     const int64_t hit = groups < rows ? groups : rows;
-    return rows <= 32 * hit && rows / kFewN + hit <= 65535;
+    if (rows / kFewN + hit > 65535) return false;
+    return rows <= 40 * hit || (rows <= 96 * hit && 4 * hit * ceil_div(cols, 256) <= num_sms());
 }
 
 int launch_few(bool f8, bool a_mn, const CUtensorMap& weights, const CUtensorMap& rows_small, const Params& p,

@@ -172,16 +172,18 @@ class _GroupedMatmul(torch.autograd.Function):
         return grad_x, grad_w, None
 
 
-@plain_dispatch
 def _grouped_matmul_eager(x, w, group_offsets):
-    x, w = cast_for_autocast(x, w)
+    if torch.is_autocast_enabled():
+        x, w = cast_for_autocast(x, w)
     _validate(x, w, group_offsets)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         return _GroupedMatmul.apply(x, w, group_offsets)
     return _rows_product(x, w, group_offsets)
 
 
-_grouped_matmul_no_compile = torch.compiler.disable(_grouped_matmul_eager)
+_PLAIN = (Tensor, torch.nn.Parameter)
+_grouped_matmul_plain = plain_dispatch(_grouped_matmul_eager)
+_grouped_matmul_no_compile = torch.compiler.disable(_grouped_matmul_plain)
 
 
 def grouped_matmul(x: Tensor, w: Tensor, group_offsets: Tensor) -> Tensor:
@@ -202,7 +204,10 @@ def grouped_matmul(x: Tensor, w: Tensor, group_offsets: Tensor) -> Tensor:
     Returns:
         Tensor: The products ``(T, N)``.
     """
-    impl = _grouped_matmul_no_compile if torch.compiler.is_compiling() else _grouped_matmul_eager
+    if torch.compiler.is_compiling():
+        return _grouped_matmul_no_compile(x, w, group_offsets)
+    # only other tensor subclasses need their dispatch switched off
+    impl = _grouped_matmul_eager if type(x) in _PLAIN and type(w) in _PLAIN else _grouped_matmul_plain
     return impl(x, w, group_offsets)
 
 
@@ -244,7 +249,6 @@ def _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype) -> None:
     validate_device(x, scale_x, w, scale_w, group_offsets)
 
 
-@plain_dispatch
 def _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtype):
     _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype)
     rows, depth = x.shape
@@ -265,7 +269,8 @@ def _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtyp
     return out
 
 
-_grouped_matmul_scaled_no_compile = torch.compiler.disable(_grouped_matmul_scaled_eager)
+_grouped_matmul_scaled_plain = plain_dispatch(_grouped_matmul_scaled_eager)
+_grouped_matmul_scaled_no_compile = torch.compiler.disable(_grouped_matmul_scaled_plain)
 
 
 def grouped_matmul_scaled(x: Tensor, scale_x: Tensor, w: Tensor, scale_w: Tensor, group_offsets: Tensor,
@@ -288,5 +293,7 @@ def grouped_matmul_scaled(x: Tensor, scale_x: Tensor, w: Tensor, scale_w: Tensor
     Returns:
         Tensor: The products ``(T, N)``; rows of no group are zero.
     """
-    impl = _grouped_matmul_scaled_no_compile if torch.compiler.is_compiling() else _grouped_matmul_scaled_eager
+    if torch.compiler.is_compiling():
+        return _grouped_matmul_scaled_no_compile(x, scale_x, w, scale_w, group_offsets, out_dtype)
+    impl = _grouped_matmul_scaled_eager if type(x) is Tensor and type(w) in _PLAIN else _grouped_matmul_scaled_plain
     return impl(x, scale_x, w, scale_w, group_offsets, out_dtype)

@@ -264,6 +264,17 @@ def test_autocast_and_no_grad():
         assert not bs.ops.grouped_matmul(x, w.to(BF16), offsets).requires_grad
 
 
+def test_marked_tensors_and_compiled_calls():
+    """Tensor subclasses (the compressed-tensor marker) and calls from a compiled function give the same values."""
+    import blksprs_b200 as bs
+    x, w, grad, offsets = make([10, 30], 64, 72, BF16)
+    want = bs.ops.grouped_matmul(x, w, offsets)
+    got = bs.ops.grouped_matmul(bs.BlksprsTensor.wrap(x), torch.nn.Parameter(w), offsets)
+    assert type(got) is torch.Tensor and torch.equal(got, want)
+    compiled = torch.compile(lambda a, b, c: bs.ops.grouped_matmul(a + 0, b, c) + 0, backend="eager")
+    assert torch.equal(compiled(x, w, offsets), want)
+
+
 def test_same_inputs_same_bits():
     import blksprs_b200 as bs
     x, w, grad, offsets = make([500, 3, 1000, 41], 520, 264, BF16)
