@@ -102,6 +102,19 @@ def test_odd_depths_and_columns(depth, cols):
 
 
 @pytest.mark.parametrize("stored", ["kn", "nk"])
+@pytest.mark.parametrize("sizes", [[4097, 4999], [8191, 1, 0, 800], [9729]], ids=str)
+def test_long_groups(sizes, stored):
+    """Enough tiles for the tall ones (up to 512 rows), heights that do not divide."""
+    check_training(*make(sizes, 72, 4104, BF16, seed=len(sizes), stored=stored, before=3, behind=30))
+
+
+@pytest.mark.parametrize("stored", ["kn", "nk"])
+def test_weight_gradient_of_large_weights(stored):
+    """Tall tiles of the weight gradient: contractions whose last rows are and are not a multiple of 16."""
+    check_training(*make([403, 512, 0, 700, 385, 416], 2056, 4104, FP16, seed=11, stored=stored, behind=5))
+
+
+@pytest.mark.parametrize("stored", ["kn", "nk"])
 @pytest.mark.parametrize("depth,cols", [(512, 136), (1032, 200), (2048, 128), (4160, 72)])
 @pytest.mark.parametrize("sizes", [[1], [0, 2, 0, 1], [30, 0, 64, 1, 65], [0] * 40 + [33]], ids=str)
 def test_few_rows_split_over_the_depth(sizes, depth, cols, stored):
@@ -253,6 +266,71 @@ def test_other_stream_and_graph_replay():
     assert not torch.equal(replayed, want)
 
 
+def test_two_streams_at_once():
+    import blksprs_b200 as bs
+    cases = [make([10, 300, 0, 77], 520, 1032, BF16, seed=1), make([2, 0, 1, 3], 2048, 512, FP16, seed=2, stored="nk"),
+             make([2000, 1, 999], 264, 520, BF16, seed=3, behind=9)]
+    for x, w, _, _ in cases:
+        x.requires_grad_(True), w.requires_grad_(True)
+
+    def step(x, w, grad, offsets):
+        out = bs.ops.grouped_matmul(x, w, offsets)
+        return (out.detach(), *torch.autograd.grad(out, (x, w), grad))
+    want = [step(*case) for case in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[] for _ in cases]
+    for _ in range(5):
+        for stream, case, results in zip(streams, cases, got):
+            with torch.cuda.stream(stream):
+                results.append(step(*case))
+    torch.cuda.synchronize()
+    for results, wanted in zip(got, want):
+        for result in results:
+            assert all(torch.equal(a, b) for a, b in zip(result, wanted))
+
+
+def test_output_beyond_32_bit_offsets():
+    """2.3e9 output elements: the last rows and columns, from both ends of the offsets."""
+    import blksprs_b200 as bs
+    gen = torch.Generator().manual_seed(12)
+    rows, cols = 70001, 32776
+    x, w = values(rows, 64, dtype=BF16, gen=gen), values(2, 64, cols, dtype=BF16, gen=gen, scale=0.125)
+    offsets = bounds_of([69990, 9], 1).to(DEV)
+    out = bs.ops.grouped_matmul(x, w, offsets)
+    for part, e in ((slice(1, 9), 0), (slice(65530, 65545), 0), (slice(69985, 69991), 0), (slice(69991, 70000), 1)):
+        assert_near(out[part], x[part].double() @ w[e].double(), x[part].double().abs() @ w[e].double().abs(), 64)
+    assert not out[0].any() and not out[70000].any()
+
+
+def test_layer_of_experts_with_its_gradients():
+    """Two products with an activation between, forward and backward, on whole numbers small enough that fp16 holds
+    every product, sum and gradient exactly: all of them have to be equal."""
+    import blksprs_b200 as bs
+    gen = torch.Generator().manual_seed(13)
+    offsets = bounds_of([7, 0, 5, 4], 2).to(DEV)
+
+    def small(*shape):
+        return torch.randint(-1, 2, shape, generator=gen).to(FP16).to(DEV)
+
+    x, up, down, grad = small(20, 32), small(4, 32, 40), small(4, 40, 24), small(20, 24)
+
+    def gradients(product, dtype):
+        leaves = [t.to(dtype).requires_grad_(True) for t in (x, up, down)]
+        hidden = torch.relu(product(leaves[0], leaves[1]))
+        out = product(hidden, leaves[2])
+        return [out, *torch.autograd.grad(out, leaves, grad.to(dtype))]
+
+    def by_mask(a, b):
+        row = torch.arange(20, device=DEV)
+        group = (row[:, None] >= offsets[None, :-1]) & (row[:, None] < offsets[None, 1:])
+        return torch.einsum("te,tk,ekn->tn", group.to(a.dtype), a, b)
+
+    for got, want in zip(gradients(lambda a, b: bs.ops.grouped_matmul(a, b, offsets), FP16),
+                         gradients(by_mask, torch.float64)):
+        assert torch.equal(got.double(), want)
+
+
 def test_autocast_and_no_grad():
     import blksprs_b200 as bs
     x, w, grad, offsets = make([10, 30], 64, 72, FP32)
@@ -326,6 +404,21 @@ def check_scaled(x, sx, w, sw, offsets, out_dtype):
 @pytest.mark.parametrize("sizes", [[1], [31, 0, 33], [257, 1, 255, 0, 256], [700]], ids=str)
 def test_scaled_sizes_of_groups(sizes, out_dtype):
     check_scaled(*make_scaled(sizes, 272, 136, seed=len(sizes), before=2, behind=3), out_dtype)
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_random_sizes(seed):
+    """Sizes, strides of storage and types by chance, over both kernels of either product."""
+    import random
+    rng = random.Random(seed)
+    groups = rng.choice((1, 2, 5, 17, 64))
+    mean = rng.choice((1, 3, 20, 45, 70, 200, 600))
+    sizes = [rng.choice((0, 1, rng.randint(0, 2 * mean))) for _ in range(groups)]
+    before, behind = rng.choice((0, 1, 37)), rng.choice((0, 1, 260))
+    depth, cols = 8 * rng.randint(1, 150), 8 * rng.randint(1, 150)
+    check_training(*make(sizes, depth, cols, rng.choice((BF16, FP16)), seed, before, behind, rng.choice(("kn", "nk"))))
+    check_scaled(*make_scaled(sizes, 16 * rng.randint(1, 75), cols, rng.choice((E4M3, E5M2)), rng.choice((E4M3, E5M2)),
+                              seed, before, behind), rng.choice((BF16, FP16, FP32)))
 
 
 @pytest.mark.parametrize("tx,tw", [(E4M3, E4M3), (E5M2, E4M3), (E4M3, E5M2), (E5M2, E5M2)],
