@@ -327,12 +327,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 for (int t = first_tile; t < n_tiles && alive; t += tile_step) {
                     const Tile o = tile_at(t);
                     const int steps = (o.depth + KE - 1) / KE;
-                    // rows of B one CTA copies for either half, and their bytes
+                    // rows of B one CTA copies for either half, and their bytes (32 at a time, from 97 on all 128 at once)
                     const int share[2] = {half_n(o.n, 0) / 2, half_n(o.n, 1) / 2};
                     int b_bytes = 0;
 #pragma unroll
                     for (int h = 0; h < kHalves; ++h)
-                        b_bytes += B_MN ? (share[h] + 63) / 64 * 8192 : share[h] == kN / 2 ? kBBytes : (share[h] + 31) / 32 * 4096;
+                        b_bytes += B_MN ? (share[h] + 63) / 64 * 8192 : (share[h] + 31) / 32 * 4096;
                     for (int k = 0; k < steps; ++k, ++it) {
                         const uint32_t s = it % kStages;
                         if (it >= kStages &&
@@ -371,11 +371,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                             if (B_MN) {
                                 for (int r = 0; r < share[h]; r += 64) pair_load_2d(to + r * 128, &map_b, from + r, o.t0 + k * KE, bar);
                             } else if (MODE == kRows8) {
-                                if (share[h] == kN / 2) pair_load_3d(to, &map_b, k * KE, from, o.group, bar);
+                                if (share[h] > kN / 2 - 32) pair_load_3d(to, &map_b, k * KE, from, o.group, bar);
                                 else
                                     for (int r = 0; r < share[h]; r += 32) pair_load_3d(to + r * 128, &map_b_small, k * KE, from + r, o.group, bar);
                             } else {
-                                if (share[h] == kN / 2) pair_load_2d(to, &map_b, k * KE, from, bar);
+                                if (share[h] > kN / 2 - 32) pair_load_2d(to, &map_b, k * KE, from, bar);
                                 else
                                     for (int r = 0; r < share[h]; r += 32) pair_load_2d(to + r * 128, &map_b_small, k * KE, from + r, bar);
                             }
