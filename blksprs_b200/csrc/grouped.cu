@@ -164,7 +164,7 @@ __device__ __forceinline__ int half_n(int n, int half) {
 
 // HALVES: accumulators a tile may take (16 bits: 256 or 512 rows; 8 bits: one).
 template <int MODE, bool A_MN, int HALVES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CUtensorMap map_b_small, const Params p) {
     using L = Smem<MODE, HALVES>;
@@ -194,6 +194,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 
     const uint32_t rank = cluster_rank();
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    let_next_launch();
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full_bar + 8 * s, 1);
@@ -215,6 +216,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async;" ::: "memory");
     }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;"
+                     ::"r"(smem_addr(&tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    wait_for_previous_launch();
     // group table: clamped offsets, then (warp 0) their running maximum and the tiles before each group
     for (int i = threadIdx.x; i <= p.groups; i += kThreads) {
         const long long v = p.offsets_i64 ? reinterpret_cast<const long long*>(p.offsets)[i]
@@ -222,11 +229,6 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const long long c = v < 0 ? 0 : v > p.rows ? p.rows : v;
         if (c != v && p.status) *p.status = BSP_ERR_DEVICE_RANGE;
         row_start[i] = (int)c;
-    }
-    if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;"
-                     ::"r"(smem_addr(&tmem_slot)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
@@ -694,9 +696,7 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mbs,
     const int pairs = num_sms() / 2;
     if (pairs <= 0) return BSP_ERR_CUDA;
     const int ctas = 2 * (int)(most_tiles < pairs ? (most_tiles < 1 ? 1 : most_tiles) : pairs);
-    kern<<<ctas, kThreads, Smem<MODE, HALVES>::kTotal, stream>>>(ma, mb, mbs, p);
-    BSP_LAUNCH_CHECK();
-    return BSP_OK;
+    return launch_overlapped(kern, dim3(ctas), kThreads, Smem<MODE, HALVES>::kTotal, 2, stream, ma, mb, mbs, p);
 }
 
 // Tiles of a rows product: a group of m rows has ceil(m / height) <= m / height + 1 row tiles, and no more groups

@@ -108,6 +108,11 @@ __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, 
 
 __device__ __forceinline__ int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
+// Programmatic dependent launch: the next launch of the stream may set up (barriers, tensor memory) on SMs this one
+// leaves; no launch touches global memory before the one before it has finished.
+__device__ __forceinline__ void let_next_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- epilogue pieces ----------------------------------------------------------------
 // A warp's staging area holds 32 output rows x 64 bytes; the 16-byte pieces of row r are permuted by
 // (r / 2) mod 4, which keeps both the writes below and the reads free of bank conflicts.
@@ -202,6 +207,27 @@ inline int make_map(CUtensorMap* map, const void* base, int elem, int rank, cons
         set_cuda_error(cudaErrorInvalidValue, what);
         return BSP_ERR_CUDA;
     }
+    return BSP_OK;
+}
+
+// A launch in clusters of `cluster` CTAs whose set-up overlaps the end of the launch before it.
+template <typename K, typename... Args>
+inline int launch_overlapped(K kernel, dim3 grid, int threads, int smem, int cluster, cudaStream_t stream, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    BSP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
     return BSP_OK;
 }
 

@@ -95,6 +95,7 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int rank = split > 1 ? (int)cluster_rank() : 0;
+    let_next_launch();
     if (threadIdx.x == 0) {
         for (int s = 0; s < kFewStages; ++s) {
             mbar_init(full_bar + 8 * s, 1);
@@ -113,17 +114,18 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async;" ::: "memory");
     }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_addr(&tmem_slot)), "r"(kColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    wait_for_previous_launch();
     for (int i = threadIdx.x; i <= p.groups; i += kFewThreads) {
         const long long v = p.offsets_i64 ? reinterpret_cast<const long long*>(p.offsets)[i]
                                           : (long long)reinterpret_cast<const int*>(p.offsets)[i];
         const long long c = v < 0 ? 0 : v > p.rows ? p.rows : v;
         if (c != v && p.status) *p.status = BSP_ERR_DEVICE_RANGE;
         row_start[i] = (int)c;
-    }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_addr(&tmem_slot)), "r"(kColumns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
@@ -427,20 +429,8 @@ int launch_kernel(const CUtensorMap& weights, const CUtensorMap& rows_small, con
     const int64_t steps = ceil_div(p.depth, F8 ? 128 : 64);
     int split = 1;
     while (split < 8 && c_tiles * hit * split * 2 <= 2 * sms && steps >= 8 * split) split *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(c_tiles * split), (unsigned)row_tiles);
-    cfg.blockDim = dim3(kFewThreads);
-    cfg.dynamicSmemBytes = FewSmem::kTotal;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    BSP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, weights, rows_small, p, split));
-    return BSP_OK;
+    return launch_overlapped(kern, dim3((unsigned)(c_tiles * split), (unsigned)row_tiles), kFewThreads, FewSmem::kTotal,
+                             split, stream, weights, rows_small, p, split);
 }
 
 }  // namespace
@@ -452,6 +442,7 @@ int launch_kernel(const CUtensorMap& weights, const CUtensorMap& rows_small, con
 bool few_applies(int64_t rows, int64_t groups, int64_t cols) {
     const int64_t hit = groups < rows ? groups : rows;
     if (rows / kFewN + hit > 65535) return false;
+    if (rows <= 72 * hit && hit * ceil_div(cols, kFewM) >= 512) return true;
     return rows <= 40 * hit || (rows <= 96 * hit && 4 * hit * ceil_div(cols, 256) <= num_sms());
 }
 
