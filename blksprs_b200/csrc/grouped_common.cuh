@@ -226,7 +226,7 @@ inline int launch_overlapped(K kernel, dim3 grid, int threads, int smem, int clu
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     BSP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
     return BSP_OK;
 }

@@ -19,6 +19,8 @@ from ..utils.tools import cast_for_autocast, plain_dispatch
 from ..utils.validation import contiguous_enabled, validate_device, validate_dimensions, validation_enabled
 
 _16_BIT = (torch.float16, torch.bfloat16)
+_8_BIT = tuple(_cabi.EIGHT_BIT_DTYPE_CODES)
+_INDEX_DTYPES = (torch.int32, torch.int64)
 _OUT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 SCALE_BLOCK = 128
 MAX_GROUPS = 1024
@@ -78,24 +80,26 @@ def _validate_groups(x: Tensor, w: Tensor, group_offsets: Tensor, vector: int) -
         raise ValueError(f"Inner dimension must be divisible by {vector} and columns by 8")
 
 
-_INDEX_DTYPES = (torch.int32, torch.int64)
-
-
-def _groups_fit(x: Tensor, w: Tensor, group_offsets: Tensor, vector: int) -> bool:
+def _groups_fit(x_shape, w_shape, group_offsets: Tensor, vector: int, device: torch.device, others) -> bool:
     """All of the group checks at once; the named errors are sorted out only if this fails (a call on a few rows
     takes the GPU about as long as the checks one by one take the host)."""
-    (_, depth), (groups, w_depth, cols) = x.shape, w.shape
-    device = x.device
-    return (depth == w_depth and group_offsets.shape == (groups + 1,) and group_offsets.dtype in _INDEX_DTYPES
-            and groups <= MAX_GROUPS and depth % vector == 0 and cols % 8 == 0 and group_offsets.is_contiguous()
-            and x.is_cuda and w.device == device and group_offsets.device == device)
+    groups, depth, cols = w_shape
+    if (x_shape[1] != depth or groups > MAX_GROUPS or depth % vector or cols % 8 or device.type != "cuda"
+            or group_offsets.dtype not in _INDEX_DTYPES or group_offsets.shape != (groups + 1,)
+            or not group_offsets.is_contiguous() or group_offsets.device != device):
+        return False
+    for t in others:
+        if t.device != device:
+            return False
+    return True
 
 
 def _validate(x: Tensor, w: Tensor, group_offsets: Tensor) -> None:
     if not validation_enabled():
         return
-    if (x.dim() == 2 and w.dim() == 3 and x.dtype in _16_BIT and w.dtype is x.dtype
-            and _groups_fit(x, w, group_offsets, 8)):
+    x_shape, w_shape, dtype = x.shape, w.shape, x.dtype
+    if (len(x_shape) == 2 and len(w_shape) == 3 and dtype in _16_BIT and w.dtype is dtype
+            and _groups_fit(x_shape, w_shape, group_offsets, 8, x.device, (w,))):
         return
     validate_dimensions(x, dims=2)
     validate_dimensions(w)
@@ -220,12 +224,12 @@ def _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype) -> None:
         raise ValueError("Output dtype must be float16, bfloat16, or float32")
     if not validation_enabled():
         return
-    if (x.dim() == 2 and w.dim() == 3 and x.dtype in _cabi.EIGHT_BIT_DTYPE_CODES
-            and w.dtype in _cabi.EIGHT_BIT_DTYPE_CODES and scale_x.dtype is torch.float32
-            and scale_w.dtype is torch.float32 and _groups_fit(x, w, group_offsets, 16)
-            and scale_x.shape == (x.size(0), _blocks_of(x.size(1)))
-            and scale_w.shape == (w.size(0), _blocks_of(w.size(1)), _blocks_of(w.size(2)))
-            and scale_x.device == x.device and scale_w.device == x.device
+    x_shape, w_shape = x.shape, w.shape
+    if (len(x_shape) == 2 and len(w_shape) == 3 and x.dtype in _8_BIT and w.dtype in _8_BIT
+            and scale_x.dtype is torch.float32 and scale_w.dtype is torch.float32
+            and scale_x.shape == (x_shape[0], -(-x_shape[1] // SCALE_BLOCK))
+            and scale_w.shape == (w_shape[0], -(-w_shape[1] // SCALE_BLOCK), -(-w_shape[2] // SCALE_BLOCK))
+            and _groups_fit(x_shape, w_shape, group_offsets, 16, x.device, (w, scale_x, scale_w))
             and not (scale_x.requires_grad or scale_w.requires_grad or x.requires_grad or w.requires_grad)):
         return
     validate_dimensions(x, scale_x, dims=2)
@@ -259,7 +263,7 @@ def _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtyp
     w, group_stride, ld_w, _ = _weight_operand(w, columns_inner=False)
     device = x.device
     with _cabi.device_guard(device):
-        out = torch.empty((rows, cols), dtype=out_dtype, device=device)
+        out = x.new_empty((rows, cols), dtype=out_dtype)
         _cabi.check(_cabi.lib().bsp_grouped_matmul_scaled(
             x.data_ptr(), ld_x, _cabi.EIGHT_BIT_DTYPE_CODES[x.dtype], scale_x.data_ptr(), *scale_x.stride(),
             w.data_ptr(), group_stride, ld_w, _cabi.EIGHT_BIT_DTYPE_CODES[w.dtype], scale_w.data_ptr(),
