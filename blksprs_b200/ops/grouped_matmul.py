@@ -16,7 +16,7 @@ from torch import Tensor
 from .. import _cabi
 from ..plan import status_word
 from ..utils.tools import cast_for_autocast, plain_dispatch
-from ..utils.validation import contiguous_enabled, validate_device, validate_dimensions, validation_enabled
+from ..utils.validation import contiguous_enabled
 
 _16_BIT = (torch.float16, torch.bfloat16)
 _8_BIT = tuple(_cabi.EIGHT_BIT_DTYPE_CODES)
@@ -26,15 +26,31 @@ SCALE_BLOCK = 128
 MAX_GROUPS = 1024
 
 
-def _copied(t: Tensor) -> Tensor:
-    if not contiguous_enabled():
+# The checks below do not go by the validation switch: they read nothing from the device and cost a microsecond or
+# two, and operands that do not fit together would be read out of bounds.
+
+def check_dimensions(dims: int, *tensors: Tensor) -> None:
+    if any(t.dim() != dims for t in tensors):
+        raise ValueError(f"Tensor must have {dims} dimensions")
+
+
+def check_device(*tensors: Tensor) -> None:
+    if tensors[0].device.type != "cuda":
+        raise ValueError("Tensors must be on GPU")
+    if any(t.device != tensors[0].device for t in tensors[1:]):
+        raise ValueError("Tensors must be on same device")
+
+
+def _copied(t: Tensor, in_backward: bool = False) -> Tensor:
+    if not (in_backward or contiguous_enabled()):
         raise ValueError("Tensor must be contiguous")
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _row_operand(t: Tensor) -> tuple[Tensor, int]:
+def _row_operand(t: Tensor, in_backward: bool = False) -> tuple[Tensor, int]:
     """``t`` (rows, width) and its row stride as the kernels read it: contiguous rows that start on 16-byte
-    boundaries, any stride between them; a copy where ``t`` is not like that."""
+    boundaries, any stride between them; a copy where ``t`` is not like that (what a backward pass gets is copied
+    whatever the switch for inputs says)."""
     rows, width = t.shape
     vector = 16 // t.element_size()
     if t.stride(1) == 1 and t.data_ptr() % 16 == 0:
@@ -43,10 +59,11 @@ def _row_operand(t: Tensor) -> tuple[Tensor, int]:
         ld = t.stride(0)
         if ld >= width and ld % vector == 0:
             return t, ld
-    return _copied(t), width
+    return _copied(t, in_backward), width
 
 
-def _weight_operand(w: Tensor, columns_inner: bool = True) -> tuple[Tensor, int, int, bool]:
+def _weight_operand(w: Tensor, columns_inner: bool = True,
+                    in_backward: bool = False) -> tuple[Tensor, int, int, bool]:
     """``w`` (groups, depth, columns), group stride, stride of the outer of the two matrix dimensions and whether
     the columns are the inner one.  Both storage orders are read in place; anything else is copied.
     ``columns_inner`` = False: only the depth may be the inner dimension (8-bit operands)."""
@@ -61,7 +78,7 @@ def _weight_operand(w: Tensor, columns_inner: bool = True) -> tuple[Tensor, int,
         if sk == 1 and sn >= depth and sn % vector == 0:
             return w, sg, sn, False
     if columns_inner:
-        return _copied(w), depth * cols, cols, True
+        return _copied(w, in_backward), depth * cols, cols, True
     return _copied(w.transpose(1, 2)).transpose(1, 2), depth * cols, depth, False
 
 
@@ -95,30 +112,28 @@ def _groups_fit(x_shape, w_shape, group_offsets: Tensor, vector: int, device: to
 
 
 def _validate(x: Tensor, w: Tensor, group_offsets: Tensor) -> None:
-    if not validation_enabled():
-        return
     x_shape, w_shape, dtype = x.shape, w.shape, x.dtype
     if (len(x_shape) == 2 and len(w_shape) == 3 and dtype in _16_BIT and w.dtype is dtype
             and _groups_fit(x_shape, w_shape, group_offsets, 8, x.device, (w,))):
         return
-    validate_dimensions(x, dims=2)
-    validate_dimensions(w)
+    check_dimensions(2, x)
+    check_dimensions(3, w)
     if x.dtype not in _16_BIT:
         raise ValueError("Tensor must have either float16 or bfloat16 dtype")
     if w.dtype != x.dtype:
         raise ValueError("Tensors must have same dtype")
     _validate_groups(x, w, group_offsets, 8)
-    validate_device(x, w, group_offsets)
+    check_device(x, w, group_offsets)
 
 
-def _rows_product(x: Tensor, w: Tensor, group_offsets: Tensor) -> Tensor:
+def _rows_product(x: Tensor, w: Tensor, group_offsets: Tensor, in_backward: bool = False) -> Tensor:
     """``out[t] = x[t] @ w[group of t]``, zero for rows of no group."""
     rows, depth = x.shape
     groups, _, cols = w.shape
     if rows == 0 or cols == 0 or depth == 0 or groups == 0:
         return torch.zeros((rows, cols), dtype=x.dtype, device=x.device)
-    x, ld_x = _row_operand(x)
-    w, group_stride, ld_w, columns_inner = _weight_operand(w)
+    x, ld_x = _row_operand(x, in_backward)
+    w, group_stride, ld_w, columns_inner = _weight_operand(w, in_backward=in_backward)
     device = x.device
     with _cabi.device_guard(device):
         out = x.new_empty((rows, cols))
@@ -136,8 +151,8 @@ def _weight_gradient(x: Tensor, grad: Tensor, group_offsets: Tensor, groups: int
     cols = grad.size(1)
     if rows == 0 or cols == 0 or depth == 0 or groups == 0:
         return torch.zeros((groups, depth, cols), dtype=x.dtype, device=x.device)
-    x, ld_x = _row_operand(x)
-    grad, ld_grad = _row_operand(grad)
+    x, ld_x = _row_operand(x, True)
+    grad, ld_grad = _row_operand(grad, True)
     device = x.device
     with _cabi.device_guard(device):
         out = torch.empty((groups, depth, cols), dtype=x.dtype, device=device)
@@ -166,7 +181,7 @@ class _GroupedMatmul(torch.autograd.Function):
             grad_output = grad_output.to(x.dtype)
         grad_x = grad_w = None
         if ctx.needs_input_grad[0]:
-            grad_x = _rows_product(grad_output, w.transpose(1, 2), group_offsets)
+            grad_x = _rows_product(grad_output, w.transpose(1, 2), group_offsets, True)
         if ctx.needs_input_grad[1]:
             if w.stride(1) == 1 and w.stride(2) != 1:
                 # weights stored with the depth innermost get their gradient in the same order
@@ -222,18 +237,17 @@ def _blocks_of(size: int) -> int:
 def _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype) -> None:
     if out_dtype not in _OUT_DTYPES:
         raise ValueError("Output dtype must be float16, bfloat16, or float32")
-    if not validation_enabled():
-        return
     x_shape, w_shape = x.shape, w.shape
     if (len(x_shape) == 2 and len(w_shape) == 3 and x.dtype in _8_BIT and w.dtype in _8_BIT
             and scale_x.dtype is torch.float32 and scale_w.dtype is torch.float32
             and scale_x.shape == (x_shape[0], -(-x_shape[1] // SCALE_BLOCK))
             and scale_w.shape == (w_shape[0], -(-w_shape[1] // SCALE_BLOCK), -(-w_shape[2] // SCALE_BLOCK))
             and _groups_fit(x_shape, w_shape, group_offsets, 16, x.device, (w, scale_x, scale_w))
-            and not (scale_x.requires_grad or scale_w.requires_grad or x.requires_grad or w.requires_grad)):
+            and not (torch.is_grad_enabled() and (scale_x.requires_grad or scale_w.requires_grad or x.requires_grad
+                                                  or w.requires_grad))):
         return
-    validate_dimensions(x, scale_x, dims=2)
-    validate_dimensions(w, scale_w)
+    check_dimensions(2, x, scale_x)
+    check_dimensions(3, w, scale_w)
     for t in (x, w):
         if t.dtype not in _cabi.EIGHT_BIT_DTYPE_CODES:
             raise ValueError("Tensor must have either float8_e4m3fn or float8_e5m2 dtype")
@@ -250,7 +264,7 @@ def _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype) -> None:
     if torch.is_grad_enabled() and (scale_x.requires_grad or scale_w.requires_grad or x.requires_grad
                                     or w.requires_grad):
         raise ValueError("The scaled product has no gradient")
-    validate_device(x, scale_x, w, scale_w, group_offsets)
+    check_device(x, scale_x, w, scale_w, group_offsets)
 
 
 def _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtype):

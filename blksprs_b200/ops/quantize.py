@@ -11,24 +11,19 @@ from torch import Tensor
 
 from .. import _cabi
 from ..utils.tools import plain_dispatch
-from ..utils.validation import contiguous_enabled, validate_device, validate_dimensions, validation_enabled
-
-SCALE_BLOCK = 128
+from ..utils.validation import contiguous_enabled
+from .grouped_matmul import SCALE_BLOCK, check_device, check_dimensions
 
 
 def _validate(t: Tensor, dtype: torch.dtype, dims: int) -> None:
     if dtype not in _cabi.EIGHT_BIT_DTYPE_CODES:
         raise ValueError("Output dtype must be float8_e4m3fn or float8_e5m2")
-    if not validation_enabled():
-        return
-    if t.dim() == dims and t.dtype in _cabi.DATA_DTYPE_CODES and t.is_cuda and not t.requires_grad:
-        return
-    validate_dimensions(t, dims=dims)
+    check_dimensions(dims, t)
     if t.dtype not in _cabi.DATA_DTYPE_CODES:
         raise ValueError("Tensor must have either float16, bfloat16, or float32 dtype")
-    if torch.is_grad_enabled() and t.requires_grad:
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("Rounding to 8 bits has no gradient")
-    validate_device(t)
+    check_device(t)
 
 
 @plain_dispatch

@@ -266,6 +266,58 @@ def test_other_stream_and_graph_replay():
     assert not torch.equal(replayed, want)
 
 
+def test_recorded_training_step_and_serving_call():
+    """A training step (gradients of leaves that no eager graph holds) and a serving call, recorded and replayed on
+    other values, bounds and scales in the same buffers."""
+    import blksprs_b200 as bs
+    x, w, grad, offsets = make([10, 300, 0, 77], 144, 136, BF16, behind=5)
+
+    def training(a, b):
+        out = bs.ops.grouped_matmul(a, b, offsets)
+        return (out.detach(), *torch.autograd.grad(out, (a, b), grad))
+
+    def serving():
+        xq, sx = bs.ops.quantize_rows(x)
+        wq, sw = bs.ops.quantize_blocks(w)
+        return (bs.ops.grouped_matmul_scaled(xq, sx, wq, sw, offsets), sx, sw)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        training(x.detach().requires_grad_(True), w.detach().requires_grad_(True))
+        serving()
+        side.synchronize()
+        leaves = [t.detach().requires_grad_(True) for t in (x, w)]
+        with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+            recorded = (*training(*leaves), *serving())
+    for shift in (0, 1):
+        if shift:
+            x.copy_(x.flip(0)), w.copy_(w.flip(0)), grad.copy_(grad.flip(1))
+            offsets.copy_(bounds_of([200, 1, 100, 80], 3).to(DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in recorded]
+        want = (*training(x.detach().requires_grad_(True), w.detach().requires_grad_(True)), *serving())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_backward_copies_whatever_the_switch_for_inputs_says():
+    import blksprs_b200 as bs
+    x, w, grad, offsets = make([10, 30], 64, 72, BF16)
+    bs.utils.disable_contiguous()
+    try:
+        with pytest.raises(ValueError, match="contiguous"):
+            bs.ops.grouped_matmul(x[:, 4:60], w[:, 4:60], offsets)
+        w.requires_grad_(True)
+        out = bs.ops.grouped_matmul(x, w, offsets)
+        got, = torch.autograd.grad(out, w, grad[:, :1].expand(-1, 72))
+    finally:
+        bs.utils.enable_contiguous()
+    want, = torch.autograd.grad(bs.ops.grouped_matmul(x, w, offsets), w, grad[:, :1].repeat(1, 72))
+    assert torch.equal(got, want)
+
+
 def test_two_streams_at_once():
     import blksprs_b200 as bs
     cases = [make([10, 300, 0, 77], 520, 1032, BF16, seed=1), make([2, 0, 1, 3], 2048, 512, FP16, seed=2, stored="nk"),
@@ -499,6 +551,25 @@ def test_quantize_blocks(depth, cols, order, dtype, to):
     assert torch.equal(scale, want)
     want_q = plain_quantize(w, LARGEST[to], blocked(want, (1, 2))[:, :depth, :cols], to)
     assert torch.equal(q.contiguous().view(torch.uint8), want_q.contiguous().view(torch.uint8))
+
+
+@pytest.mark.parametrize("to", [E4M3, E5M2], ids=["e4m3", "e5m2"])
+def test_quantize_all_magnitudes(to):
+    """Blocks from the smallest to the largest fp32 magnitudes, values of a block down to 2^-40 of its largest: the
+    quotient is the correctly rounded one on both ways to it."""
+    import blksprs_b200 as bs
+    gen = torch.Generator().manual_seed(21)
+    exponent = torch.arange(-149, 127).repeat_interleave(4).double()
+    x = torch.randn((exponent.numel(), 128), generator=gen).clamp(-1.9, 1.9).double()
+    x = x * 2.0 ** (exponent[:, None] - 40.0 * torch.rand(x.shape, generator=gen).double() ** 3)
+    x = x.to(FP32).to(DEV)
+    q, scale = bs.ops.quantize_rows(x, to)
+    want = plain_scale(x.abs().amax(1, keepdim=True), to)
+    assert torch.equal(scale, want)
+    assert torch.equal(q.view(torch.uint8), plain_quantize(x, LARGEST[to], want, to).view(torch.uint8))
+    q, scale = bs.ops.quantize_blocks(x.reshape(-1, 128, 1), to)
+    assert torch.equal(scale.reshape(-1, 1), want)
+    assert torch.equal(q.reshape(x.shape).view(torch.uint8), plain_quantize(x, LARGEST[to], want, to).view(torch.uint8))
 
 
 def test_quantize_edge_values():

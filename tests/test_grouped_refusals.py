@@ -60,6 +60,32 @@ def test_grouped_matmul_scaled_refuses(change, message):
         bs.ops.grouped_matmul_scaled(*arguments)
 
 
+def test_switched_off_validation_still_refuses_what_would_be_read_out_of_bounds():
+    x, w, offsets = operands()
+    bs.utils.disable_validation()
+    try:
+        for bad in ((x[:, :8], w, offsets), (x, w, offsets[:-1]), (x, w.half(), offsets), (x, w[0], offsets),
+                    (x, w, offsets), (x[0], w, offsets), (x, w, offsets.float())):
+            with pytest.raises(ValueError):
+                bs.ops.grouped_matmul(*bad)
+        arguments = scaled_operands()
+        for at, bad in ((1, arguments[1][:, :1]), (3, arguments[3][:1]), (0, arguments[0][:, :16]), (4, offsets)):
+            with pytest.raises(ValueError):
+                bs.ops.grouped_matmul_scaled(*arguments[:at], bad, *arguments[at + 1:])
+        for op, t in ((bs.ops.quantize_rows, torch.zeros((4, 40))), (bs.ops.quantize_blocks, torch.zeros((2, 4, 40)))):
+            for bad in (t, t[0], t.double()):
+                with pytest.raises(ValueError):
+                    op(bad)
+    finally:
+        bs.utils.enable_validation()
+
+
+def test_group_limit_is_the_library_s():
+    from blksprs_b200.ops import grouped_matmul  # noqa: F401  (the module's name is the function's too)
+    import sys
+    assert sys.modules["blksprs_b200.ops.grouped_matmul"].MAX_GROUPS == _cabi.lib().bsp_grouped_max_groups()
+
+
 def test_grouped_matmul_scaled_refuses_output_types():
     with pytest.raises(ValueError, match="Output dtype"):
         bs.ops.grouped_matmul_scaled(*scaled_operands(), out_dtype=torch.float64)
