@@ -161,8 +161,11 @@ class _NoGuard:
 _NO_GUARD = _NoGuard()
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def device_guard(device: torch.device):
     """Context that makes ``device`` the current CUDA device; free when it already is."""
-    if device.index is not None and torch.cuda.current_device() == device.index:
+    if device.index is not None and _current_device() == device.index:
         return _NO_GUARD
     return torch.cuda.device(device)

@@ -155,7 +155,7 @@ def _weight_gradient(x: Tensor, grad: Tensor, group_offsets: Tensor, groups: int
     grad, ld_grad = _row_operand(grad, True)
     device = x.device
     with _cabi.device_guard(device):
-        out = torch.empty((groups, depth, cols), dtype=x.dtype, device=device)
+        out = x.new_empty((groups, depth, cols))
         _cabi.check(_cabi.lib().bsp_grouped_weight_grad(
             x.data_ptr(), ld_x, grad.data_ptr(), ld_grad, group_offsets.data_ptr(),
             group_offsets.dtype == torch.int64, rows, groups, depth, cols, out.data_ptr(),
