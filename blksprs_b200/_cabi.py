@@ -161,11 +161,12 @@ class _NoGuard:
 _NO_GUARD = _NoGuard()
 
 
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+# index of the calling thread's current CUDA device
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def device_guard(device: torch.device):
     """Context that makes ``device`` the current CUDA device; free when it already is."""
-    if device.index is not None and _current_device() == device.index:
+    if device.index is not None and current_device() == device.index:
         return _NO_GUARD
     return torch.cuda.device(device)

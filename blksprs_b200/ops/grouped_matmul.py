@@ -18,10 +18,10 @@ from ..plan import status_word
 from ..utils.tools import cast_for_autocast, plain_dispatch
 from ..utils.validation import contiguous_enabled
 
-_16_BIT = (torch.float16, torch.bfloat16)
-_8_BIT = tuple(_cabi.EIGHT_BIT_DTYPE_CODES)
+_16_BIT = {t: _cabi.DATA_DTYPE_CODES[t] for t in (torch.float16, torch.bfloat16)}
+_8_BIT = _cabi.EIGHT_BIT_DTYPE_CODES
 _INDEX_DTYPES = (torch.int32, torch.int64)
-_OUT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+_OUT_DTYPES = {t: _cabi.DATA_DTYPE_CODES[t] for t in (torch.float16, torch.bfloat16, torch.float32)}
 SCALE_BLOCK = 128
 MAX_GROUPS = 1024
 
@@ -47,39 +47,36 @@ def _copied(t: Tensor, in_backward: bool = False) -> Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _row_operand(t: Tensor, in_backward: bool = False) -> tuple[Tensor, int]:
-    """``t`` (rows, width) and its row stride as the kernels read it: contiguous rows that start on 16-byte
-    boundaries, any stride between them; a copy where ``t`` is not like that (what a backward pass gets is copied
-    whatever the switch for inputs says)."""
+# What the kernels read in place: rows, and matrices with either of their dimensions contiguous, that start on 16-byte
+# boundaries; anything else is copied.  (A call on a few rows takes the GPU about as long as Python takes for a few dozen
+# of its steps, so these and the checks are written as straight lines.)
+
+def _row_stride(t: Tensor, mask: int) -> int:
+    """Row stride of ``t`` (rows, width) if it is read in place, else 0; ``mask`` = elements of 16 bytes, less one."""
+    ld, inner = t.stride()
+    if inner != 1 or t.data_ptr() & 15:
+        return 0
     rows, width = t.shape
-    vector = 16 // t.element_size()
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0:
-        if rows == 1:
-            return t, width
-        ld = t.stride(0)
-        if ld >= width and ld % vector == 0:
-            return t, ld
-    return _copied(t, in_backward), width
+    if rows == 1:
+        return width
+    return 0 if ld < width or ld & mask else ld
 
 
-def _weight_operand(w: Tensor, columns_inner: bool = True,
-                    in_backward: bool = False) -> tuple[Tensor, int, int, bool]:
-    """``w`` (groups, depth, columns), group stride, stride of the outer of the two matrix dimensions and whether
-    the columns are the inner one.  Both storage orders are read in place; anything else is copied.
-    ``columns_inner`` = False: only the depth may be the inner dimension (8-bit operands)."""
-    groups, depth, cols = w.shape
-    vector = 16 // w.element_size()
+def _group_and_outer_stride(w: Tensor, mask: int) -> tuple[int, int, bool]:
+    """Group stride, stride of the outer matrix dimension and whether the columns are the inner one, of ``w``
+    (groups, depth, columns) if it is read in place; else the second is 0."""
     sg, sk, sn = w.stride()
-    if w.data_ptr() % 16 == 0 and (groups == 1 or (sg >= vector and sg % vector == 0)):
-        if groups == 1:
-            sg = depth * cols
-        if columns_inner and sn == 1 and sk >= cols and sk % vector == 0:
-            return w, sg, sk, True
-        if sk == 1 and sn >= depth and sn % vector == 0:
-            return w, sg, sn, False
-    if columns_inner:
-        return _copied(w, in_backward), depth * cols, cols, True
-    return _copied(w.transpose(1, 2)).transpose(1, 2), depth * cols, depth, False
+    groups, depth, cols = w.shape
+    if groups == 1:
+        sg = depth * cols
+    elif sg <= mask or sg & mask:
+        return sg, 0, True
+    if not w.data_ptr() & 15:
+        if sn == 1 and sk >= cols and not sk & mask:
+            return sg, sk, True
+        if sk == 1 and sn >= depth and not sn & mask:
+            return sg, sn, False
+    return sg, 0, True
 
 
 def _validate_groups(x: Tensor, w: Tensor, group_offsets: Tensor, vector: int) -> None:
@@ -97,25 +94,16 @@ def _validate_groups(x: Tensor, w: Tensor, group_offsets: Tensor, vector: int) -
         raise ValueError(f"Inner dimension must be divisible by {vector} and columns by 8")
 
 
-def _groups_fit(x_shape, w_shape, group_offsets: Tensor, vector: int, device: torch.device, others) -> bool:
-    """All of the group checks at once; the named errors are sorted out only if this fails (a call on a few rows
-    takes the GPU about as long as the checks one by one take the host)."""
-    groups, depth, cols = w_shape
-    if (x_shape[1] != depth or groups > MAX_GROUPS or depth % vector or cols % 8 or device.type != "cuda"
-            or group_offsets.dtype not in _INDEX_DTYPES or group_offsets.shape != (groups + 1,)
-            or not group_offsets.is_contiguous() or group_offsets.device != device):
-        return False
-    for t in others:
-        if t.device != device:
-            return False
-    return True
-
-
 def _validate(x: Tensor, w: Tensor, group_offsets: Tensor) -> None:
-    x_shape, w_shape, dtype = x.shape, w.shape, x.dtype
-    if (len(x_shape) == 2 and len(w_shape) == 3 and dtype in _16_BIT and w.dtype is dtype
-            and _groups_fit(x_shape, w_shape, group_offsets, 8, x.device, (w,))):
-        return
+    x_shape, w_shape, dtype, device = x.shape, w.shape, x.dtype, x.device
+    # all at once; which one it was is sorted out only if this fails
+    if len(x_shape) == 2 and len(w_shape) == 3:
+        groups, depth, cols = w_shape
+        if (x_shape[1] == depth and dtype in _16_BIT and w.dtype is dtype and groups <= MAX_GROUPS and not depth & 7
+                and not cols & 7 and group_offsets.dtype in _INDEX_DTYPES and group_offsets.shape == (groups + 1,)
+                and group_offsets.is_contiguous() and device.type == "cuda" and w.device == device
+                and group_offsets.device == device):
+            return
     check_dimensions(2, x)
     check_dimensions(3, w)
     if x.dtype not in _16_BIT:
@@ -130,18 +118,25 @@ def _rows_product(x: Tensor, w: Tensor, group_offsets: Tensor, in_backward: bool
     """``out[t] = x[t] @ w[group of t]``, zero for rows of no group."""
     rows, depth = x.shape
     groups, _, cols = w.shape
-    if rows == 0 or cols == 0 or depth == 0 or groups == 0:
-        return torch.zeros((rows, cols), dtype=x.dtype, device=x.device)
-    x, ld_x = _row_operand(x, in_backward)
-    w, group_stride, ld_w, columns_inner = _weight_operand(w, in_backward=in_backward)
     device = x.device
-    with _cabi.device_guard(device):
-        out = x.new_empty((rows, cols))
-        _cabi.check(_cabi.lib().bsp_grouped_matmul(
-            x.data_ptr(), ld_x, w.data_ptr(), group_stride, ld_w, columns_inner, group_offsets.data_ptr(),
-            group_offsets.dtype == torch.int64, rows, groups, depth, cols, out.data_ptr(),
-            _cabi.DATA_DTYPE_CODES[x.dtype], status_word(device).data_ptr(), _cabi.stream_handle(device)),
-            "bsp_grouped_matmul")
+    if not (rows and cols and depth and groups):
+        return torch.zeros((rows, cols), dtype=x.dtype, device=device)
+    if _cabi.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _rows_product(x, w, group_offsets, in_backward)
+    ld_x = _row_stride(x, 7)
+    if not ld_x:
+        x, ld_x = _copied(x, in_backward), depth
+    group_stride, ld_w, columns_inner = _group_and_outer_stride(w, 7)
+    if not ld_w:
+        w, group_stride, ld_w, columns_inner = _copied(w, in_backward), depth * cols, cols, True
+    out = x.new_empty((rows, cols))
+    status = _cabi.lib().bsp_grouped_matmul(
+        x.data_ptr(), ld_x, w.data_ptr(), group_stride, ld_w, columns_inner, group_offsets.data_ptr(),
+        group_offsets.dtype is torch.int64, rows, groups, depth, cols, out.data_ptr(), _16_BIT[x.dtype],
+        status_word(device).data_ptr(), _cabi.stream_handle(device))
+    if status:
+        _cabi.check(status, "bsp_grouped_matmul")
     return out
 
 
@@ -149,18 +144,24 @@ def _weight_gradient(x: Tensor, grad: Tensor, group_offsets: Tensor, groups: int
     """``out[e] = x[rows of e]^T @ grad[rows of e]``, zero for groups without rows."""
     rows, depth = x.shape
     cols = grad.size(1)
-    if rows == 0 or cols == 0 or depth == 0 or groups == 0:
-        return torch.zeros((groups, depth, cols), dtype=x.dtype, device=x.device)
-    x, ld_x = _row_operand(x, True)
-    grad, ld_grad = _row_operand(grad, True)
     device = x.device
-    with _cabi.device_guard(device):
-        out = x.new_empty((groups, depth, cols))
-        _cabi.check(_cabi.lib().bsp_grouped_weight_grad(
-            x.data_ptr(), ld_x, grad.data_ptr(), ld_grad, group_offsets.data_ptr(),
-            group_offsets.dtype == torch.int64, rows, groups, depth, cols, out.data_ptr(),
-            _cabi.DATA_DTYPE_CODES[x.dtype], status_word(device).data_ptr(), _cabi.stream_handle(device)),
-            "bsp_grouped_weight_grad")
+    if not (rows and cols and depth and groups):
+        return torch.zeros((groups, depth, cols), dtype=x.dtype, device=device)
+    if _cabi.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _weight_gradient(x, grad, group_offsets, groups)
+    ld_x, ld_grad = _row_stride(x, 7), _row_stride(grad, 7)
+    if not ld_x:
+        x, ld_x = _copied(x, True), depth
+    if not ld_grad:
+        grad, ld_grad = _copied(grad, True), cols
+    out = x.new_empty((groups, depth, cols))
+    status = _cabi.lib().bsp_grouped_weight_grad(
+        x.data_ptr(), ld_x, grad.data_ptr(), ld_grad, group_offsets.data_ptr(), group_offsets.dtype is torch.int64,
+        rows, groups, depth, cols, out.data_ptr(), _16_BIT[x.dtype], status_word(device).data_ptr(),
+        _cabi.stream_handle(device))
+    if status:
+        _cabi.check(status, "bsp_grouped_weight_grad")
     return out
 
 
@@ -237,15 +238,20 @@ def _blocks_of(size: int) -> int:
 def _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype) -> None:
     if out_dtype not in _OUT_DTYPES:
         raise ValueError("Output dtype must be float16, bfloat16, or float32")
-    x_shape, w_shape = x.shape, w.shape
-    if (len(x_shape) == 2 and len(w_shape) == 3 and x.dtype in _8_BIT and w.dtype in _8_BIT
-            and scale_x.dtype is torch.float32 and scale_w.dtype is torch.float32
-            and scale_x.shape == (x_shape[0], -(-x_shape[1] // SCALE_BLOCK))
-            and scale_w.shape == (w_shape[0], -(-w_shape[1] // SCALE_BLOCK), -(-w_shape[2] // SCALE_BLOCK))
-            and _groups_fit(x_shape, w_shape, group_offsets, 16, x.device, (w, scale_x, scale_w))
-            and not (torch.is_grad_enabled() and (scale_x.requires_grad or scale_w.requires_grad or x.requires_grad
-                                                  or w.requires_grad))):
-        return
+    x_shape, w_shape, device = x.shape, w.shape, x.device
+    if len(x_shape) == 2 and len(w_shape) == 3:
+        groups, depth, cols = w_shape
+        blocks = -(-depth // SCALE_BLOCK)
+        if (x_shape[1] == depth and x.dtype in _8_BIT and w.dtype in _8_BIT and groups <= MAX_GROUPS
+                and not depth & 15 and not cols & 7 and scale_x.dtype is torch.float32
+                and scale_w.dtype is torch.float32 and scale_x.shape == (x_shape[0], blocks)
+                and scale_w.shape == (groups, blocks, -(-cols // SCALE_BLOCK))
+                and group_offsets.dtype in _INDEX_DTYPES and group_offsets.shape == (groups + 1,)
+                and group_offsets.is_contiguous() and device.type == "cuda" and w.device == device
+                and scale_x.device == device and scale_w.device == device and group_offsets.device == device
+                and not ((scale_x.requires_grad or scale_w.requires_grad or x.requires_grad or w.requires_grad)
+                         and torch.is_grad_enabled())):
+            return
     check_dimensions(2, x, scale_x)
     check_dimensions(3, w, scale_w)
     for t in (x, w):
@@ -271,19 +277,26 @@ def _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtyp
     _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype)
     rows, depth = x.shape
     groups, _, cols = w.shape
-    if rows == 0 or cols == 0 or depth == 0 or groups == 0:
-        return torch.zeros((rows, cols), dtype=out_dtype, device=x.device)
-    x, ld_x = _row_operand(x)
-    w, group_stride, ld_w, _ = _weight_operand(w, columns_inner=False)
     device = x.device
-    with _cabi.device_guard(device):
-        out = x.new_empty((rows, cols), dtype=out_dtype)
-        _cabi.check(_cabi.lib().bsp_grouped_matmul_scaled(
-            x.data_ptr(), ld_x, _cabi.EIGHT_BIT_DTYPE_CODES[x.dtype], scale_x.data_ptr(), *scale_x.stride(),
-            w.data_ptr(), group_stride, ld_w, _cabi.EIGHT_BIT_DTYPE_CODES[w.dtype], scale_w.data_ptr(),
-            *scale_w.stride(), group_offsets.data_ptr(), group_offsets.dtype == torch.int64, rows, groups, depth,
-            cols, out.data_ptr(), _cabi.DATA_DTYPE_CODES[out_dtype], status_word(device).data_ptr(),
-            _cabi.stream_handle(device)), "bsp_grouped_matmul_scaled")
+    if not (rows and cols and depth and groups):
+        return torch.zeros((rows, cols), dtype=out_dtype, device=device)
+    if _cabi.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtype)
+    ld_x = _row_stride(x, 15)
+    if not ld_x:
+        x, ld_x = _copied(x), depth
+    group_stride, ld_w, columns_inner = _group_and_outer_stride(w, 15)
+    if not ld_w or columns_inner:
+        w, group_stride, ld_w = _copied(w.transpose(1, 2)).transpose(1, 2), depth * cols, depth
+    out = x.new_empty((rows, cols), dtype=out_dtype)
+    status = _cabi.lib().bsp_grouped_matmul_scaled(
+        x.data_ptr(), ld_x, _8_BIT[x.dtype], scale_x.data_ptr(), *scale_x.stride(), w.data_ptr(), group_stride, ld_w,
+        _8_BIT[w.dtype], scale_w.data_ptr(), *scale_w.stride(), group_offsets.data_ptr(),
+        group_offsets.dtype is torch.int64, rows, groups, depth, cols, out.data_ptr(), _OUT_DTYPES[out_dtype],
+        status_word(device).data_ptr(), _cabi.stream_handle(device))
+    if status:
+        _cabi.check(status, "bsp_grouped_matmul_scaled")
     return out
 
 
