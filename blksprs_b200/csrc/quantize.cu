@@ -1,7 +1,8 @@
 // 8-bit values with a scale for each block of 128: the operands of the scaled product.
 //
-//   scale = max(a / F, 2^-126), a the block's largest magnitude, F the type's largest value
-//   q     = value / scale, rounded to nearest even (a / scale is F within one rounding, so nothing saturates)
+//   scale = max(a * (1 / F), 2^-126), a the block's largest magnitude, F the type's largest value, its reciprocal
+//           rounded (a product, as elementwise libraries divide by a constant: the same scales to the last bit)
+//   q     = value / scale, rounded to nearest even (a / scale is F within two roundings, so nothing saturates)
 //
 // The floor of 2^-126 keeps the quotient finite for blocks of zeros and of subnormal magnitudes.
 // Magnitudes are compared as bit patterns: NaN > infinity > any finite value, so that one NaN or
@@ -21,8 +22,8 @@ __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-__device__ __forceinline__ float scale_of(float largest, float type_max) {
-    const float s = largest / type_max;
+__device__ __forceinline__ float scale_of(float largest, float reciprocal_of_max) {
+    const float s = largest * reciprocal_of_max;
     return s < kSmallestScale ? kSmallestScale : s;      // a NaN stays
 }
 
@@ -120,7 +121,7 @@ template <typename T, bool E5M2, bool VEC>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
 quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int rows, int width, int blocks, uint8_t* __restrict__ q,
                      float* __restrict__ scale) {
-    const float type_max = E5M2 ? 57344.0f : 448.0f;
+    constexpr float reciprocal_of_max = E5M2 ? 1.0f / 57344.0f : 1.0f / 448.0f;
     const int lane = threadIdx.x & 31, sub = lane & 7;
     const int64_t stride = (int64_t)gridDim.x * 32;
     const int row_step = (int)(stride / blocks), block_step = (int)(stride - (int64_t)row_step * blocks);
@@ -164,7 +165,7 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int rows, int width, i
         }
         // the divisions of the four blocks side by side: lanes 0-3 of a quarter warp have one each
         const uint32_t mine = (lane & 2) ? ((lane & 1) ? m[3] : m[2]) : ((lane & 1) ? m[1] : m[0]);
-        const Divider of_mine = divide_by(scale_of(Eight<T>::value_of(mine), type_max));
+        const Divider of_mine = divide_by(scale_of(Eight<T>::value_of(mine), reciprocal_of_max));
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
             Divider over;
@@ -207,7 +208,7 @@ quantize_blocks_kernel(const T* __restrict__ w, int64_t sg, int64_t sk, int64_t 
                        float* __restrict__ scale) {
     __shared__ uint2 staged[DEPTH_INNER ? 1 : kBlock * 16];
     __shared__ uint32_t largest[8];
-    const float type_max = E5M2 ? 57344.0f : 448.0f;
+    constexpr float reciprocal_of_max = E5M2 ? 1.0f / 57344.0f : 1.0f / 448.0f;
     const int64_t per_group = k_blocks * n_blocks;
     const int64_t g = blockIdx.x / per_group, block = blockIdx.x - g * per_group;
     const int64_t k0 = block / n_blocks * kBlock, n0 = block % n_blocks * kBlock;
@@ -234,7 +235,7 @@ quantize_blocks_kernel(const T* __restrict__ w, int64_t sg, int64_t sk, int64_t 
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = Eight<T>::larger(m, largest[i]);
-    const Divider over = divide_by(scale_of(Eight<T>::value_of(m), type_max));
+    const Divider over = divide_by(scale_of(Eight<T>::value_of(m), reciprocal_of_max));
     if (threadIdx.x == 0) scale[blockIdx.x] = over.scale;
     uint8_t* dst = q + g * depth * cols + n0 * depth + k0;
     const bool wide = (depth & 7) == 0;

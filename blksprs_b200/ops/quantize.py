@@ -1,7 +1,7 @@
 """8-bit values with a scale for each block of 128: the operands of ``grouped_matmul_scaled``.
 
-``scale = max(largest magnitude of the block / largest value of the type, 2**-126)``, ``q = value / scale`` rounded
-to nearest even.  A block that holds an infinity or a NaN has a scale that is not finite and multiplies out to NaN;
+``scale = max(largest magnitude of the block / largest value of the type, 2**-126)`` (the quotient as a product with the
+rounded reciprocal, as torch divides by a number), ``q = value / scale`` rounded to nearest even.  A block that holds an infinity or a NaN has a scale that is not finite and multiplies out to NaN;
 other blocks are not touched by it.  No counterpart in the blksprs library.
 """
 from __future__ import annotations
@@ -26,7 +26,6 @@ def _validate(t: Tensor, dtype: torch.dtype, dims: int) -> None:
     check_device(t)
 
 
-@plain_dispatch
 def _quantize_rows_eager(x: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
     _validate(x, dtype, 2)
     rows, width = x.shape
@@ -35,16 +34,19 @@ def _quantize_rows_eager(x: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]
             raise ValueError("Tensor must be contiguous")
         x = x.contiguous()
     device = x.device
-    with _cabi.device_guard(device):
-        q = x.new_empty((rows, width), dtype=dtype)
-        scale = x.new_empty((rows, -(-width // SCALE_BLOCK)), dtype=torch.float32)
-        _cabi.check(_cabi.lib().bsp_quantize_rows(
-            x.data_ptr(), x.stride(0), rows, width, _cabi.DATA_DTYPE_CODES[x.dtype], q.data_ptr(),
-            _cabi.EIGHT_BIT_DTYPE_CODES[dtype], scale.data_ptr(), _cabi.stream_handle(device)), "bsp_quantize_rows")
+    if _cabi.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _quantize_rows_eager(x, dtype)
+    q = x.new_empty((rows, width), dtype=dtype)
+    scale = x.new_empty((rows, -(-width // SCALE_BLOCK)), dtype=torch.float32)
+    status = _cabi.lib().bsp_quantize_rows(
+        x.data_ptr(), x.stride(0), rows, width, _cabi.DATA_DTYPE_CODES[x.dtype], q.data_ptr(),
+        _cabi.EIGHT_BIT_DTYPE_CODES[dtype], scale.data_ptr(), _cabi.stream_handle(device))
+    if status:
+        _cabi.check(status, "bsp_quantize_rows")
     return q, scale
 
 
-@plain_dispatch
 def _quantize_blocks_eager(w: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
     _validate(w, dtype, 3)
     groups, depth, cols = w.shape
@@ -59,8 +61,9 @@ def _quantize_blocks_eager(w: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tenso
     return q, scale
 
 
-_quantize_rows_no_compile = torch.compiler.disable(_quantize_rows_eager)
-_quantize_blocks_no_compile = torch.compiler.disable(_quantize_blocks_eager)
+_quantize_rows_plain, _quantize_blocks_plain = plain_dispatch(_quantize_rows_eager), plain_dispatch(_quantize_blocks_eager)
+_quantize_rows_no_compile = torch.compiler.disable(_quantize_rows_plain)
+_quantize_blocks_no_compile = torch.compiler.disable(_quantize_blocks_plain)
 
 
 def quantize_rows(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[Tensor, Tensor]:
@@ -73,7 +76,9 @@ def quantize_rows(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[
     Returns:
         tuple[Tensor, Tensor]: The rounded rows ``(T, K)`` and the scales, float32 ``(T, ceil(K / 128))``.
     """
-    return (_quantize_rows_no_compile if torch.compiler.is_compiling() else _quantize_rows_eager)(x, dtype)
+    if torch.compiler.is_compiling():
+        return _quantize_rows_no_compile(x, dtype)
+    return (_quantize_rows_eager if type(x) is Tensor else _quantize_rows_plain)(x, dtype)
 
 
 def quantize_blocks(w: Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[Tensor, Tensor]:
@@ -88,4 +93,6 @@ def quantize_blocks(w: Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tupl
         tuple[Tensor, Tensor]: The rounded matrices ``(E, K, N)``, stored with ``K`` contiguous as
         ``grouped_matmul_scaled`` reads them, and the scales, float32 ``(E, ceil(K / 128), ceil(N / 128))``.
     """
-    return (_quantize_blocks_no_compile if torch.compiler.is_compiling() else _quantize_blocks_eager)(w, dtype)
+    if torch.compiler.is_compiling():
+        return _quantize_blocks_no_compile(w, dtype)
+    return (_quantize_blocks_eager if type(w) is Tensor else _quantize_blocks_plain)(w, dtype)

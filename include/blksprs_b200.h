@@ -455,8 +455,8 @@ int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x, const flo
                               int64_t cols, void* out, int out_dtype, int32_t* status_word, void* stream);
 
 /* ---- 8-bit values with a scale for each block of 128 ----------------------
- * scale = max(largest magnitude of the block / largest value of the type,
- * 2^-126), q = value / scale rounded to nearest even.  A block that holds an
+ * scale = max(largest magnitude of the block * rounded reciprocal of the
+ * type's largest value, 2^-126), q = value / scale rounded to nearest even.  A block that holds an
  * infinity has an infinite scale, one that holds a NaN a NaN scale (both are
  * NaN when multiplied out).  Input fp16 / bf16 / fp32. */
 

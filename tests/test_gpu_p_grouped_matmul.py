@@ -501,8 +501,9 @@ def test_scaled_non_finite_scale_stays_in_its_row():
 
 
 def plain_scale(largest, to):
-    """The quotient rounded once: a division by a Python number would multiply by its rounded reciprocal."""
-    return (largest / torch.full_like(largest, LARGEST[to])).clamp(min=2.0 ** -126)
+    """The product with the reciprocal of the type's largest value, each rounded once."""
+    reciprocal = torch.tensor(1.0 / LARGEST[to], dtype=torch.float32, device=largest.device)
+    return (largest * reciprocal).clamp(min=2.0 ** -126)
 
 
 def plain_quantize(t, largest, scale, dtype):
