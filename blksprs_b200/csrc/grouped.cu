@@ -171,11 +171,14 @@ __device__ __forceinline__ int half_n(int n, int half) {
     return half ? n - first : first;
 }
 
+// Rows of the copy that brings `share` rows of B.
+__device__ __forceinline__ int copied_rows(int share) { return share > 64 ? 128 : share > 32 ? 64 : share > 0 ? 32 : 0; }
+
 // HALVES: accumulators a tile may take (16 bits: 256 or 512 rows; 8 bits: one).
 template <int MODE, bool A_MN, int HALVES>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-               const __grid_constant__ CUtensorMap map_b_small, const Params p) {
+               const __grid_constant__ CUtensorMap map_b_64, const __grid_constant__ CUtensorMap map_b_32, const Params p) {
     using L = Smem<MODE, HALVES>;
     constexpr int kHalves = HALVES;
     constexpr int kStages = L::kStages, kStageBytes = L::kStageBytes, kABytes = L::kABytes, kBBytes = L::kBBytes;
@@ -338,12 +341,14 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 for (int t = first_tile; t < n_tiles && alive; t += tile_step) {
                     const Tile o = tile_at(t);
                     const int steps = (o.depth + KE - 1) / KE;
-                    // rows of B one CTA copies for either half, and their bytes (32 at a time, from 97 on all 128 at once)
+                    // rows of B one CTA copies for either half, and their bytes.  One copy of 32, 64 or 128 rows, also where that
+                    // brings rows that no accumulator column takes: 96 rows in three copies kept a step at 1100 cycles, 128 in one
+                    // let it go at the MMAs' 770.
                     const int share[2] = {half_n(o.n, 0) / 2, half_n(o.n, 1) / 2};
                     int b_bytes = 0;
 #pragma unroll
                     for (int h = 0; h < kHalves; ++h)
-                        b_bytes += B_MN ? (share[h] + 63) / 64 * 8192 : (share[h] + 31) / 32 * 4096;
+                        b_bytes += B_MN ? (share[h] + 63) / 64 * 8192 : copied_rows(share[h]) * 128;
                     for (int k = 0; k < steps; ++k, ++it) {
                         const uint32_t s = it % kStages;
                         if (it >= kStages &&
@@ -381,14 +386,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                             const int from = (MODE == kRows8 ? o.c0 : o.r0) + (h ? 2 * share[0] : 0) + rank * share[h];
                             if (B_MN) {
                                 for (int r = 0; r < share[h]; r += 64) pair_load_2d(to + r * 128, &map_b, from + r, o.t0 + k * KE, bar);
-                            } else if (MODE == kRows8) {
-                                if (share[h] > kN / 2 - 32) pair_load_3d(to, &map_b, k * KE, from, o.group, bar);
-                                else
-                                    for (int r = 0; r < share[h]; r += 32) pair_load_3d(to + r * 128, &map_b_small, k * KE, from + r, o.group, bar);
-                            } else {
-                                if (share[h] > kN / 2 - 32) pair_load_2d(to, &map_b, k * KE, from, bar);
-                                else
-                                    for (int r = 0; r < share[h]; r += 32) pair_load_2d(to + r * 128, &map_b_small, k * KE, from + r, bar);
+                            } else if (share[h] > 0) {
+                                const CUtensorMap* map = share[h] > 64 ? &map_b : share[h] > 32 ? &map_b_64 : &map_b_32;
+                                if (MODE == kRows8) pair_load_3d(to, map, k * KE, from, o.group, bar);
+                                else pair_load_2d(to, map, k * KE, from, bar);
                             }
                         }
                     }
@@ -691,7 +692,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 // ---- host side ---------------------------------------------------------------------
 
 template <int MODE, bool A_MN, int HALVES>
-int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mbs, const Params& p, int64_t most_tiles,
+int launch(const CUtensorMap& ma, const CUtensorMap (&mb)[3], const Params& p, int64_t most_tiles,
            cudaStream_t stream) {
     auto kern = grouped_kernel<MODE, A_MN, HALVES>;
     static std::atomic<uint64_t> opted_in{0};
@@ -705,7 +706,7 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mbs,
     const int pairs = num_sms() / 2;
     if (pairs <= 0) return BSP_ERR_CUDA;
     const int ctas = 2 * (int)(most_tiles < pairs ? (most_tiles < 1 ? 1 : most_tiles) : pairs);
-    return launch_overlapped(kern, dim3(ctas), kThreads, Smem<MODE, HALVES>::kTotal, 2, stream, ma, mb, mbs, p);
+    return launch_overlapped(kern, dim3(ctas), kThreads, Smem<MODE, HALVES>::kTotal, 2, stream, ma, mb[0], mb[1], mb[2], p);
 }
 
 // Tiles of a rows product: a group of m rows has ceil(m / height) <= m / height + 1 row tiles, and no more groups
@@ -750,14 +751,14 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
     if ((depth & 7) || (cols & 7) || (ld_x & 7) || (ld_w & 7) || (group_stride_w & 7) || ld_x < depth || ld_w < inner ||
         group_stride_w < 0 || (groups > 1 && group_stride_w < 8))
         return BSP_ERR_INVALID_ARG;
-    CUtensorMap ma, mb, mbs;
+    CUtensorMap ma, mb[3];
     const int64_t dims[3] = {inner, outer, groups};
     const int64_t strides[2] = {ld_w * 2, (groups > 1 ? group_stride_w : outer * ld_w) * 2};
     const int box[3] = {64, w_cols_inner ? 64 : kHalf, 1};
     if ((st = make_map(&ma, w, dtype, 3, dims, strides, box)) != BSP_OK) return st;
     const bool few = few_applies(rows, groups, cols);
-    if (!few && (st = rows_map(&mb, x, dtype, rows, depth, ld_x, kHalf)) != BSP_OK) return st;
-    if ((st = rows_map(&mbs, x, dtype, rows, depth, ld_x, 32)) != BSP_OK) return st;
+    for (int i = few ? 2 : 0; i < 3; ++i)
+        if ((st = rows_map(&mb[i], x, dtype, rows, depth, ld_x, 128 >> i)) != BSP_OK) return st;
     Params p = {};
     p.offsets = offsets;
     p.offsets_i64 = offsets_i64;
@@ -773,15 +774,15 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
     cudaStream_t stream = (cudaStream_t)stream_;
     if (few) {
         p.idesc = (p.idesc & 0x00ffffffu) | (128u >> 4 << 24);
-        return launch_few(false, w_cols_inner != 0, ma, mbs, p, stream);
+        return launch_few(false, w_cols_inner != 0, ma, mb[2], p, stream);
     }
     const int halves = tile_halves(most_row_tiles(rows, groups, 2 * kTile) * ceil_div(cols, kTile), rows, groups);
     const int64_t tiles = most_row_tiles(rows, groups, halves * kTile) * ceil_div(cols, kTile);
     if (w_cols_inner)
-        return halves == 2 ? launch<kRows16, true, 2>(ma, mb, mbs, p, tiles, stream)
-                           : launch<kRows16, true, 1>(ma, mb, mbs, p, tiles, stream);
-    return halves == 2 ? launch<kRows16, false, 2>(ma, mb, mbs, p, tiles, stream)
-                       : launch<kRows16, false, 1>(ma, mb, mbs, p, tiles, stream);
+        return halves == 2 ? launch<kRows16, true, 2>(ma, mb, p, tiles, stream)
+                           : launch<kRows16, true, 1>(ma, mb, p, tiles, stream);
+    return halves == 2 ? launch<kRows16, false, 2>(ma, mb, p, tiles, stream)
+                       : launch<kRows16, false, 1>(ma, mb, p, tiles, stream);
 }
 
 extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* grad, int64_t ld_grad,
@@ -797,9 +798,9 @@ extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* 
         return BSP_ERR_INVALID_ARG;
     const int64_t tiles = groups * ceil_div(depth, kTile) * ceil_div(cols, kTile);
     if (tiles > 0x7fffffffLL - 65536) return BSP_ERR_UNSUPPORTED;
-    CUtensorMap ma, mb;
+    CUtensorMap ma, mb[3] = {};
     if ((st = rows_map(&ma, grad, dtype, rows, cols, ld_grad, 64)) != BSP_OK) return st;
-    if ((st = rows_map(&mb, x, dtype, rows, depth, ld_x, 64)) != BSP_OK) return st;
+    if ((st = rows_map(&mb[0], x, dtype, rows, depth, ld_x, 64)) != BSP_OK) return st;
     Params p = {};
     p.offsets = offsets;
     p.offsets_i64 = offsets_i64;
@@ -813,8 +814,8 @@ extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* 
     p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(kTile >> 4) << 24);
     p.status = status_word;
     const bool two = tile_halves(groups * ceil_div(depth, 2 * kTile) * ceil_div(cols, kTile), rows, groups) == 2;
-    return two ? launch<kGrad16, true, 2>(ma, mb, mb, p, tiles, (cudaStream_t)stream_)
-               : launch<kGrad16, true, 1>(ma, mb, mb, p, tiles, (cudaStream_t)stream_);
+    return two ? launch<kGrad16, true, 2>(ma, mb, p, tiles, (cudaStream_t)stream_)
+               : launch<kGrad16, true, 1>(ma, mb, p, tiles, (cudaStream_t)stream_);
 }
 
 extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x, const float* scale_x,
@@ -833,13 +834,14 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
     if ((depth & 15) || (cols & 7) || (ld_x & 15) || (ld_w & 15) || (group_stride_w & 15) || ld_x < depth ||
         ld_w < depth || group_stride_w < 0 || (groups > 1 && group_stride_w < 16))
         return BSP_ERR_INVALID_ARG;
-    CUtensorMap ma, mb, mbs;
+    CUtensorMap ma, mb[3];
     const int64_t dims[3] = {depth, cols, groups};
     const int64_t strides[2] = {ld_w, groups > 1 ? group_stride_w : cols * ld_w};
-    const int box[3] = {128, kN / 2, 1}, box_small[3] = {128, 32, 1};
-    if ((st = make_map(&mb, w, type_w, 3, dims, strides, box)) != BSP_OK) return st;
     const bool few = few_applies(rows, groups, cols);
-    if (!few && (st = make_map(&mbs, w, type_w, 3, dims, strides, box_small)) != BSP_OK) return st;
+    for (int i = 0; i < (few ? 1 : 3); ++i) {
+        const int box[3] = {128, 128 >> i, 1};
+        if ((st = make_map(&mb[i], w, type_w, 3, dims, strides, box)) != BSP_OK) return st;
+    }
     if ((st = rows_map(&ma, x, type_x, rows, depth, ld_x, few ? 32 : kHalf)) != BSP_OK) return st;
     Params p = {};
     p.offsets = offsets;
@@ -864,8 +866,8 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
         // the weights are A there
         p.idesc = (1u << 4) | ((type_w == BSP_E5M2 ? 1u : 0u) << 7) | ((type_x == BSP_E5M2 ? 1u : 0u) << 10) |
                   (128u >> 4 << 24);
-        return launch_few(true, false, mb, ma, p, (cudaStream_t)stream_);
+        return launch_few(true, false, mb[0], ma, p, (cudaStream_t)stream_);
     }
     const int64_t tiles = most_row_tiles(rows, groups, kTile) * ceil_div(cols, kN);
-    return launch<kRows8, false, 1>(ma, mb, mbs, p, tiles, (cudaStream_t)stream_);
+    return launch<kRows8, false, 1>(ma, mb, p, tiles, (cudaStream_t)stream_);
 }
