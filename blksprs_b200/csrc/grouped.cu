@@ -756,8 +756,8 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
     const int64_t strides[2] = {ld_w * 2, (groups > 1 ? group_stride_w : outer * ld_w) * 2};
     const int box[3] = {64, w_cols_inner ? 64 : kHalf, 1};
     if ((st = make_map(&ma, w, dtype, 3, dims, strides, box)) != BSP_OK) return st;
-    const bool few = few_applies(rows, groups, cols);
-    for (int i = few ? 2 : 0; i < 3; ++i)
+    const bool few = few_applies(rows, groups, cols, false);
+    for (int i = few ? 1 : 0; i < 3; ++i)
         if ((st = rows_map(&mb[i], x, dtype, rows, depth, ld_x, 128 >> i)) != BSP_OK) return st;
     Params p = {};
     p.offsets = offsets;
@@ -774,7 +774,7 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
     cudaStream_t stream = (cudaStream_t)stream_;
     if (few) {
         p.idesc = (p.idesc & 0x00ffffffu) | (128u >> 4 << 24);
-        return launch_few(false, w_cols_inner != 0, ma, mb[2], p, stream);
+        return launch_few(false, w_cols_inner != 0, ma, mb[1], mb[2], p, stream);
     }
     const int halves = tile_halves(most_row_tiles(rows, groups, 2 * kTile) * ceil_div(cols, kTile), rows, groups);
     const int64_t tiles = most_row_tiles(rows, groups, halves * kTile) * ceil_div(cols, kTile);
@@ -834,15 +834,16 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
     if ((depth & 15) || (cols & 7) || (ld_x & 15) || (ld_w & 15) || (group_stride_w & 15) || ld_x < depth ||
         ld_w < depth || group_stride_w < 0 || (groups > 1 && group_stride_w < 16))
         return BSP_ERR_INVALID_ARG;
-    CUtensorMap ma, mb[3];
+    CUtensorMap ma, ma_32, mb[3];
     const int64_t dims[3] = {depth, cols, groups};
     const int64_t strides[2] = {ld_w, groups > 1 ? group_stride_w : cols * ld_w};
-    const bool few = few_applies(rows, groups, cols);
+    const bool few = few_applies(rows, groups, cols, true);
     for (int i = 0; i < (few ? 1 : 3); ++i) {
         const int box[3] = {128, 128 >> i, 1};
         if ((st = make_map(&mb[i], w, type_w, 3, dims, strides, box)) != BSP_OK) return st;
     }
-    if ((st = rows_map(&ma, x, type_x, rows, depth, ld_x, few ? 32 : kHalf)) != BSP_OK) return st;
+    if ((st = rows_map(&ma, x, type_x, rows, depth, ld_x, few ? 64 : kHalf)) != BSP_OK) return st;
+    if (few && (st = rows_map(&ma_32, x, type_x, rows, depth, ld_x, 32)) != BSP_OK) return st;
     Params p = {};
     p.offsets = offsets;
     p.offsets_i64 = offsets_i64;
@@ -866,7 +867,7 @@ extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x
         // the weights are A there
         p.idesc = (1u << 4) | ((type_w == BSP_E5M2 ? 1u : 0u) << 7) | ((type_x == BSP_E5M2 ? 1u : 0u) << 10) |
                   (128u >> 4 << 24);
-        return launch_few(true, false, mb[0], ma, p, (cudaStream_t)stream_);
+        return launch_few(true, false, mb[0], ma, ma_32, p, (cudaStream_t)stream_);
     }
     const int64_t tiles = most_row_tiles(rows, groups, kTile) * ceil_div(cols, kN);
     return launch<kRows8, false, 1>(ma, mb, p, tiles, (cudaStream_t)stream_);

@@ -242,10 +242,11 @@ inline int rows_map(CUtensorMap* map, const void* base, int elem, int64_t rows, 
     return make_map(map, base, elem, 2, dims, strides, box);
 }
 
-// Product of few rows per group (grouped_few.cu); same operands as the products it stands in for.
-int launch_few(bool f8, bool a_mn, const CUtensorMap& weights, const CUtensorMap& rows_small, const Params& p,
-               cudaStream_t stream);
-bool few_applies(int64_t rows, int64_t groups, int64_t cols);
+// Product of few rows per group (grouped_few.cu); same operands as the products it stands in for: the weights in boxes
+// of 128 features, the rows in boxes of 64 and of 32.
+int launch_few(bool f8, bool a_mn, const CUtensorMap& weights, const CUtensorMap& rows_64, const CUtensorMap& rows_32,
+               const Params& p, cudaStream_t stream);
+bool few_applies(int64_t rows, int64_t groups, int64_t cols, bool f8);
 
 }  // namespace grouped
 }  // namespace bsp

@@ -60,9 +60,6 @@ __device__ __forceinline__ void few_mma(uint32_t d_tmem, uint64_t adesc, uint64_
         tc_mma_f16_elect(d_tmem, adesc, bdesc, idesc, accumulate);
 }
 
-__device__ __forceinline__ void few_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    tma_load_2d(dst, map, x, y, bar);
-}
 __device__ __forceinline__ void few_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -77,8 +74,8 @@ __device__ __forceinline__ float2 cluster_float2(uint32_t addr) {
 // grid: x = cluster rank (split of the contraction) + split * column tile, y = row tile.
 template <bool F8, bool A_MN>
 __global__ void __launch_bounds__(kFewThreads, 2)
-grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p,
-                   const int split) {
+grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x_64,
+                   const __grid_constant__ CUtensorMap map_x_32, const Params p, const int split) {
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
     const uint32_t data = (raw + 1023u) & ~1023u;
@@ -186,7 +183,7 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (warp == 0) {
         // ---------------- copies ----------------
         if (lane == 0) {
-            const int b_bytes = (n + 31) / 32 * 4096;
+            const int b_bytes = n > 32 ? 8192 : 4096;
             for (int k = 0; k < steps; ++k) {
                 const int s = k % kFewStages;
                 if (k >= kFewStages && !bounded_wait(empty_bar + 8 * s, (k / kFewStages - 1) & 1, abort_flag, p.status)) break;
@@ -200,7 +197,7 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 } else {
                     few_load_3d(a, &map_w, x0, c0, group, bar);
                 }
-                for (int r = 0; r < n; r += 32) few_load_2d(b + r * 128, &map_x, x0, r0 + r, bar);
+                tma_load_2d(b, n > 32 ? &map_x_64 : &map_x_32, x0, r0, bar);
             }
         }
         __syncwarp();
@@ -414,7 +411,8 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 }
 
 template <bool F8, bool A_MN>
-int launch_kernel(const CUtensorMap& weights, const CUtensorMap& rows_small, const Params& p, cudaStream_t stream) {
+int launch_kernel(const CUtensorMap& weights, const CUtensorMap& rows_64, const CUtensorMap& rows_32, const Params& p,
+                  cudaStream_t stream) {
     auto kern = grouped_few_kernel<F8, A_MN>;
     static std::atomic<uint64_t> opted_in{0};
     int dev = 0;
@@ -435,27 +433,32 @@ int launch_kernel(const CUtensorMap& weights, const CUtensorMap& rows_small, con
     int split = 1;
     while (split < 8 && c_tiles * hit * split * 2 <= 2 * sms && steps >= 8 * split) split *= 2;
     return launch_overlapped(kern, dim3((unsigned)(c_tiles * split), (unsigned)row_tiles), kFewThreads, FewSmem::kTotal,
-                             split, stream, weights, rows_small, p, split);
+                             split, stream, weights, rows_64, rows_32, p, split);
 }
 
 }  // namespace
 
-// Which of the two: by the mean rows of the groups that can have rows.  Measured (us, few / pairs; 2048 x 1024 bf16, 64
-// groups): 48 rows 52 / 61, 64 rows 57 / 65, 96 rows 68 / 66; 32 groups of 1024 x 2048: 48 rows 33 / 35, 64 rows 35 / 36, 96
-// rows 42 / 37; 8 groups of 2048 x 2048: 32 rows 19 / 20, 48 rows 23 / 20.  Where the pairs would have less than half a
-// tile each, splitting the depth pays longer: one group of 4096 x 4096: 64 rows 15 / 29, 96 rows 22 / 34 (8 bits 20 / 20).
-bool few_applies(int64_t rows, int64_t groups, int64_t cols) {
+// Which of the two: by the mean rows of the groups that can have rows, and by whether either kernel's tiles fill the GPU.
+// Measured (us, few / pairs; groups, depth x columns, rows per group):
+//   16 bits   64, 2048 x 1024: 32: 48 / 49, 48: 51 / 50, 128: 80 / 56     16, 4096 x 4096: 4: 77 / 87, 48: 89 / 90
+//             8, 2048 x 2048: 8: 14.9 / 14.6, 16: 15.5 / 14.7, 48: 23 / 15
+//             4, 1024 x 1024: 4: 5.7 / 8.8, 64: 8.4 / 9.4, 128: 13 / 10   1, 4096 x 4096: 64: 15 / 22, 96: 21 / 22
+//   8 bits    64, 2048 x 1024: 48: 35 / 42, 64: 44 / 43                   16, 4096 x 4096: 4: 45 / 64, 64: 68 / 75
+//             8, 2048 x 2048: 32: 14 / 15, 48: 18 / 15                    1, 4096 x 4096: 64: 14 / 18, 96: 19 / 19
+bool few_applies(int64_t rows, int64_t groups, int64_t cols, bool f8) {
     const int64_t hit = groups < rows ? groups : rows;
     if (rows / kFewN + hit > 65535) return false;
-    if (rows <= 72 * hit && hit * ceil_div(cols, kFewM) >= 512) return true;
-    return rows <= 40 * hit || (rows <= 96 * hit && 4 * hit * ceil_div(cols, 256) <= num_sms());
+    const bool fills = hit * ceil_div(cols, kFewM) >= 512;                   // a tile per group and 128 columns
+    const bool pairs_idle = 4 * hit * ceil_div(cols, 256) <= num_sms();      // less than half of the pairs have a tile
+    const int64_t most = pairs_idle ? (f8 ? 96 : 72) : fills ? (f8 ? 64 : 40) : (f8 ? 40 : 12);
+    return rows <= most * hit;
 }
 
-int launch_few(bool f8, bool a_mn, const CUtensorMap& weights, const CUtensorMap& rows_small, const Params& p,
-               cudaStream_t stream) {
-    if (f8) return launch_kernel<true, false>(weights, rows_small, p, stream);
-    return a_mn ? launch_kernel<false, true>(weights, rows_small, p, stream)
-                : launch_kernel<false, false>(weights, rows_small, p, stream);
+int launch_few(bool f8, bool a_mn, const CUtensorMap& weights, const CUtensorMap& rows_64, const CUtensorMap& rows_32,
+               const Params& p, cudaStream_t stream) {
+    if (f8) return launch_kernel<true, false>(weights, rows_64, rows_32, p, stream);
+    return a_mn ? launch_kernel<false, true>(weights, rows_64, rows_32, p, stream)
+                : launch_kernel<false, false>(weights, rows_64, rows_32, p, stream);
 }
 
 }  // namespace grouped
