@@ -20,12 +20,12 @@
 //   (one for each row and each 128 features) is one register per thread.
 //
 // What it measured on a B200 (time, rate; bf16): forward, dX and dW of 8 groups of 2048 rows, 4096 x 4096:
-// 385, 379 and 400 us, 1430, 1450 and 1375 TFLOP/s, the tensor pipe 79-80 % busy at the 1.54 GHz that the
-// power cap leaves (a plain library product of 8192^3: 1404 TFLOP/s sustained, 1687 in a burst).  16 groups
-// of 1024 rows, 2048 x 4096: 219 us, 1253 TFLOP/s; the same in 8 bits, 4096 x 4096: 298 us, 1844 TFLOP/s,
-// tensor pipe 56 %: there the epilogue bounds, 128 multiply-adds per thread and 512 cycles of MMAs, with the
-// waits around them (timed inside the kernel: 700 cycles per step).  64 groups of 64 rows, 2048 x 1024: 61 us, HBM
-// 59 % busy.
+// 370, 375 and 376-415 us, 1486, 1466 and 1325-1462 TFLOP/s, the tensor pipe 79-83 % busy at the 1.52-1.56 GHz
+// that the power cap leaves (a plain library product of 8192^3: 1404 TFLOP/s sustained, 1687 in a burst).  16
+// groups of 1024 rows, 2048 x 4096: 206 us, 1335 TFLOP/s; the same in 8 bits, 4096 x 4096: 293 us, 1876
+// TFLOP/s, tensor pipe 56 %: there the epilogue bounds, 128 multiply-adds per thread and 512 cycles of MMAs, with
+// the waits around them (timed inside the kernel: 700 cycles per step).  64 groups of 64 rows, 2048 x 1024: 52
+// us, HBM 65 % busy; 64 groups of 128 rows: 55 us, 318 MB at 5.8 TB/s.
 //
 // Persistent CTA pairs, 12 warps per CTA: warp 0 copies tiles with TMA into a ring in shared memory,
 // warp 1 of the first CTA issues the MMAs, warp 2 owns tensor memory, warps 4-11 are the epilogue.
@@ -717,7 +717,7 @@ int64_t most_row_tiles(int64_t rows, int64_t groups, int64_t height) {
 
 // Accumulators of a 16-bit tile.  Two: A is staged once for both, 24 KiB per CTA and 512 cycles of MMAs instead of
 // 32 (what L2 delivers, about 55 bytes per cycle and SM, is what bounds the ring); one where two would leave the
-// pairs fewer than four tiles each, or where the mean group would not fill them (192 rows: 71 / 81 us).  Measured, one / two: 16 groups of 1024 rows, 2048 x 4096: 248 / 239 us; weight
+// pairs fewer than four tiles each, or where the mean group would not fill them (192 rows: 71 / 81 us).  Measured, one / two: 16 groups of 1024 rows, 2048 x 4096: 248 / 239 us (three copies per half then); weight
 // gradient of 8 groups of 2048 rows, 4096 x 4096: 534 / 415 us; 33 groups of 60 rows, 1032 x 1496: 39 / 43 us.
 int tile_halves(int64_t tiles_of_two, int64_t rows, int64_t groups) {
     return tiles_of_two >= 4 * (num_sms() / 2) && rows >= 384 * (groups < rows ? groups : rows) ? 2 : 1;
