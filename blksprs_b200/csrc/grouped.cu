@@ -619,7 +619,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     const int n = half_n(o.n, h), above = h ? half_n(o.n, 0) : 0;
                     if (n == 0) break;
                     // first everything out of tensor memory, as packed words, so that the accumulator is free again
-                    // (the next tile's MMAs wait for it); then through the staging area into rows
+                    // (the next tile's MMAs wait for it); then through the staging area into rows.  The sums are fp32 until
+                    // here and rounded once, to the type of the operands: what a dense layer of that type returns
                     uint32_t words[4][16];
                     if (computed) {
                         alive = wait_all(tfull_bar + 8 * (acc % kAccs), (acc / kAccs) & 1, abort_flag, p.status);
@@ -717,8 +718,9 @@ int64_t most_row_tiles(int64_t rows, int64_t groups, int64_t height) {
 
 // Accumulators of a 16-bit tile.  Two: A is staged once for both, 24 KiB per CTA and 512 cycles of MMAs instead of
 // 32 (what L2 delivers, about 55 bytes per cycle and SM, is what bounds the ring); one where two would leave the
-// pairs fewer than four tiles each, or where the mean group would not fill them (192 rows: 71 / 81 us).  Measured, one / two: 16 groups of 1024 rows, 2048 x 4096: 248 / 239 us (three copies per half then); weight
-// gradient of 8 groups of 2048 rows, 4096 x 4096: 534 / 415 us; 33 groups of 60 rows, 1032 x 1496: 39 / 43 us.
+// pairs fewer than four tiles each, or where the mean group would not fill them (192 rows: 71 / 81 us; 64 groups of
+// 64 rows: 53 / 60 us; 33 groups of 60 rows, 1032 x 1496: 34 / 42 us).  Measured, one / two: 16 groups of 1024 rows,
+// 2048 x 4096: 215 / 213 us; weight gradient of 8 groups of 2048 rows, 4096 x 4096: 559 / 380 us.
 int tile_halves(int64_t tiles_of_two, int64_t rows, int64_t groups) {
     return tiles_of_two >= 4 * (num_sms() / 2) && rows >= 384 * (groups < rows ? groups : rows) ? 2 : 1;
 }

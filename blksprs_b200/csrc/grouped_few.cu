@@ -376,7 +376,8 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
     __syncthreads();
     if (split > 1) {
-        // partial sums [row][column] over the ring, which every copy and MMA is through with
+        // partial sums [row][column] over the ring, which every copy and MMA is through with; fp32, joined in fp32 and
+        // rounded once at the end
         if (warp >= 2 && warp < 6) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
