@@ -361,9 +361,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         // zeroed the second CTA's half reports to the stage's barrier there, which has no other use
                         const bool split = MODE == kGrad16 && ((o.depth - k * KE) & (KSTEP - 1)) && k == steps - 1;
                         uint32_t bar = map_to_rank(full_bar + 8 * s, 0);
+                        issued_stages = (int)it + 1;
                         if (rank == 0) {
                             mbar_arrive_expect_tx(full_bar + 8 * s, (kABytes + b_bytes) * (split ? 1 : 2));
-                            issued_stages = (int)it + 1;
                         } else if (split) {
                             bar = map_to_rank(full_bar + 8 * s, 1);
                             mbar_arrive_expect_tx(full_bar + 8 * s, kABytes + b_bytes);
@@ -418,7 +418,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     if (rank == 0) {
                         alive = wait_all(full_bar + 8 * s, (it / kStages) & 1, abort_flag, p.status);
                     } else if (zero_rows) {
-                        alive = wait_all(full_bar + 8 * s, (tail_parity >> s) & 1, abort_flag, p.status);
+                        alive = wait_all(full_bar + 8 * s, (tail_parity >> s) & 1, abort_flag, p.status, &issued_stages);
                     }
                     if (!alive) break;
                     if (zero_rows) {
@@ -623,7 +623,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     // here and rounded once, to the type of the operands: what a dense layer of that type returns
                     uint32_t words[4][16];
                     if (computed) {
-                        alive = wait_all(tfull_bar + 8 * (acc % kAccs), (acc / kAccs) & 1, abort_flag, p.status);
+                        alive = wait_all(tfull_bar + 8 * (acc % kAccs), (acc / kAccs) & 1, abort_flag, p.status, &issued_stages);
                         if (!alive) break;
                         tc_fence_after();
                     }

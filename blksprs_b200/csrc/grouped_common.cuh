@@ -86,14 +86,23 @@ __device__ __forceinline__ float4 shared_float4(uint32_t at) {
 }
 // A bounded wait of a whole warp: true only if it succeeded for every lane, so that the lanes go on or leave
 // together.  The first try is a straight line: 27 cycles on a barrier that is through, against 76 for the loop.
-__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+// progress: for waits that last as long as a whole contraction (the sums of 2^28 rows and more take a second): entries
+// of the ring asked for so far.  The time then counts from when that number last changed; a ring that stands still is
+// found by the roles that wait for its entries.
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
+                                         const volatile int* progress = nullptr) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     unsigned long long t0 = 0;
+    int seen = 0;
     for (uint32_t it = 1;; ++it) {
         if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
         if ((it & 0xff) == 0) {
             const unsigned long long now = global_timer();
             if (t0 == 0) t0 = now;
+            if (progress && *progress != seen) {
+                seen = *progress;
+                t0 = now;
+            }
             const bool late = now - t0 > kWaitLimitNs && now > t0;
             if (late) {
                 *abort_flag = 1;

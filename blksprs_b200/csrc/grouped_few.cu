@@ -311,7 +311,7 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 }
             }
         } else if (steps > 0) {
-            complete = wait_all(tfull_bar, 0, abort_flag, p.status);
+            complete = wait_all(tfull_bar, 0, abort_flag, p.status, &issued_stages);
             if (complete) {
                 tc_fence_after();
 #pragma unroll

@@ -355,6 +355,37 @@ def test_output_beyond_32_bit_offsets():
     assert not out[0].any() and not out[70000].any()
 
 
+def test_weight_gradient_of_very_many_rows():
+    """A wait for a whole contraction may last longer than the second after which one that makes no progress ends.
+    One group of 2^29 rows and 13 more: its weight gradient is one tile, 8.4 million steps and 2.7 seconds long.
+    Values are 1 or -1, repeated from 2^20 rows, so that every partial sum is an integer below 2^24 and the sums are
+    exact; one rounding."""
+    import blksprs_b200 as bs
+    from blksprs_b200.plan import check_device_status
+    part, times, rest = 2 ** 20, 512, 13
+    gen = torch.Generator().manual_seed(5)
+    x, grad, w = ((torch.randint(0, 2, shape, generator=gen) * 2 - 1).to(BF16).to(DEV)
+                  for shape in ((part, 8), (part, 8), (1, 8, 8)))
+    w.requires_grad_()
+    products = x.double()[:, :, None] * grad.double()[:, None, :]
+    assert products.cumsum(0).abs().max() * times < 2 ** 24
+    want = products.sum(0) * times + products[:rest].sum(0)
+    forward = (x.double() @ w[0].detach().double()).to(BF16)
+    del products
+    long = torch.cat([x.repeat(times, 1), x[:rest]]).requires_grad_()
+    offsets = torch.tensor([0, long.shape[0]], device=DEV)
+    out = bs.ops.grouped_matmul(long, w, offsets)
+    for i in (0, 1, times // 2, times - 1):
+        assert torch.equal(out[i * part:(i + 1) * part], forward)
+    assert torch.equal(out[times * part:], forward[:rest])
+    out.backward(torch.cat([grad.repeat(times, 1), grad[:rest]]))
+    check_device_status()
+    assert torch.equal(w.grad[0], want.to(BF16))
+    last = (grad.double() @ w[0].detach().double().T).to(BF16)
+    assert torch.equal(long.grad[(times - 1) * part:times * part], last)
+    assert torch.equal(long.grad[times * part:], last[:rest])
+
+
 def test_layer_of_experts_with_its_gradients():
     """Two products with an activation between, forward and backward, on whole numbers small enough that fp16 holds
     every product, sum and gradient exactly: all of them have to be equal."""
