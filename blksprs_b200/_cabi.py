@@ -81,7 +81,8 @@ SIGNATURES = {
     "bsp_grouped_matmul": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_int64,
                                    c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p]),
     "bsp_grouped_weight_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64,
-                                        c_int64, c_void_p, c_int, c_void_p, c_void_p]),
+                                        c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "bsp_grouped_weight_grad_workspace": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
     "bsp_grouped_matmul_scaled": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                           c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64,
                                           c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p]),

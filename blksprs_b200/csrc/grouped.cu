@@ -81,7 +81,7 @@ struct Smem {
 };
 
 struct Tile {
-    int group;
+    int group;       // weight gradient in parts: part * groups + group
     int r0, rows;    // first output row (of the whole output, or of the group's output), rows to store
     int c0, cols;    // first output column, columns to store
     int n;           // accumulator columns, in two halves if more than kTile
@@ -285,7 +285,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     cluster_sync();      // the other CTA's barriers and tensor memory are ready
 
     const int r_tiles_all = (p.out_rows + tile_rows - 1) / tile_rows;
-    const int n_tiles = uniform(MODE != kGrad16 ? tile_start[p.groups] : p.groups * c_tiles * r_tiles_all);
+    const int n_tiles = uniform(MODE != kGrad16 ? tile_start[p.groups] : p.groups * p.parts * c_tiles * r_tiles_all);
     const int first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
 
     auto tile_at = [&](int t) -> Tile {
@@ -311,13 +311,17 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const int c = rest / in_band, r = band * kBand + rest - c * in_band;
         o.c0 = c * kTileCols;
         o.cols = min(kTileCols, p.cols - o.c0);
-        const int first = row_start[o.group], m = row_start[o.group + 1] - first;
+        const int g = MODE == kGrad16 ? o.group % p.groups : o.group;
+        const int first = row_start[g], m = row_start[g + 1] - first;
         if (MODE == kGrad16) {
             const int h = tile_height(p.out_rows, tile_rows);
             o.r0 = r * h;
             o.rows = min(h, p.out_rows - o.r0);
-            o.t0 = first;
-            o.depth = m;
+            // whole ring entries per part, so that only a group's last part may have rows to zero
+            const int share = round_up((m + p.parts - 1) / p.parts, KE);
+            const int skipped = (int)min((int64_t)(o.group / p.groups) * share, (int64_t)m);
+            o.t0 = first + skipped;
+            o.depth = min(share, m - skipped);
         } else {
             const int h = MODE == kRows16 ? tile_height(m, tile_rows) : kTile;
             o.r0 = first + r * h;
@@ -611,7 +615,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 // lane = output column
                 const int c = o.c0 + (int)rank * kHalf + quarter * 32;
                 const int64_t first = MODE == kRows16 ? o.r0 : (int64_t)o.group * p.out_rows + o.r0;
-                char* out = (char*)p.out + first * row_bytes + (int64_t)c * 2;
+                char* out = (char*)p.out + first * row_bytes + (int64_t)c * esize;
                 const int bytes = (p.cols - c) * 2;
                 const bool computed = steps > 0;    // a group without rows has a gradient of zero
 #pragma unroll 1
@@ -621,6 +625,36 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     // first everything out of tensor memory, as packed words, so that the accumulator is free again
                     // (the next tile's MMAs wait for it); then through the staging area into rows.  The sums are fp32 until
                     // here and rounded once, to the type of the operands: what a dense layer of that type returns
+                    if (MODE == kGrad16 && HALVES == 1 && p.out_dtype == BSP_F32) {
+                        // a part's sums, as they are; a column per lane, 128 bytes of a row per store
+                        if (computed) {
+                            alive = wait_all(tfull_bar + 8 * (acc % kAccs), (acc / kAccs) & 1, abort_flag, p.status, &issued_stages);
+                            if (!alive) break;
+                            tc_fence_after();
+                        }
+#pragma unroll 1
+                        for (int c32 = part * 32; c32 < n; c32 += 64) {
+                            uint32_t v[32];
+                            if (computed) {
+                                tc_ld32(lanes + acc % kAccs * kN + c32, v);
+                                tc_wait_ld();
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) v[j] = 0;
+                            }
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (c32 + j < o.rows && c + lane < p.cols)
+                                    *reinterpret_cast<uint32_t*>(out + (c32 + j) * row_bytes + lane * 4) = v[j];
+                        }
+                        if (computed) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive_pair(tempty_first + 8 * (acc % kAccs));
+                            ++acc;
+                        }
+                        continue;
+                    }
                     uint32_t words[4][16];
                     if (computed) {
                         alive = wait_all(tfull_bar + 8 * (acc % kAccs), (acc / kAccs) & 1, abort_flag, p.status, &issued_stages);
@@ -690,6 +724,31 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
 }
 
+// Sums of the parts, added up in their order and rounded once.  Four values per thread.
+constexpr int kJoinThreads = 128;
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads)
+join_parts_kernel(const float4* __restrict__ sums, int64_t quads, int parts, uint2* __restrict__ out) {
+    let_next_launch();
+    wait_for_previous_launch();
+    const int64_t i = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x;
+    if (i >= quads) return;
+    float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int first = 0; first < parts; first += 8) {
+        float4 v[8];         // eight loads under way, the last ones too
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = first + k < parts ? sums[(first + k) * quads + i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            total.x += v[k].x;
+            total.y += v[k].y;
+            total.z += v[k].z;
+            total.w += v[k].w;
+        }
+    }
+    out[i] = make_uint2(pack2<T>(total.x, total.y), pack2<T>(total.z, total.w));
+}
+
 // ---- host side ---------------------------------------------------------------------
 
 template <int MODE, bool A_MN, int HALVES>
@@ -723,6 +782,23 @@ int64_t most_row_tiles(int64_t rows, int64_t groups, int64_t height) {
 // 2048 x 4096: 215 / 213 us; weight gradient of 8 groups of 2048 rows, 4096 x 4096: 559 / 380 us.
 int tile_halves(int64_t tiles_of_two, int64_t rows, int64_t groups) {
     return tiles_of_two >= 4 * (num_sms() / 2) && rows >= 384 * (groups < rows ? groups : rows) ? 2 : 1;
+}
+
+// Parts that the rows of every group are split into for the weight gradient, where its tiles leave pairs idle: each
+// part of a tile has a pair of its own, leaves its sums in the workspace, and a second launch adds them up.  A step of
+// 64 rows takes a pair 0.39 us; a part more costs about 0.08 us per tile (its 256 KiB written and read), so the time
+// is least near parts^2 = rows * 0.39 / 64 / (tiles * 0.08).  Measured, one part / parts, us: one group of 256 x 256,
+// 1024 rows 12.1 / 9.2, 16384 rows 106 / 15.8; 8 groups, 256 x 256, 1024 rows each 12.5 / 11.4, 4096 rows 31.8 / 15.2;
+// 4 groups, 512 x 520, 16384 rows 108 / 47.7.  Below 1024 rows the second launch costs what it saves (8 groups of 512
+// rows: 9.3 / 10.4), as it does for parts of fewer than 256.
+constexpr int64_t kRowsToSplit = 1024, kPartRows = 256, kPartCost = 13;
+int64_t gradient_parts(int64_t rows, int64_t groups, int64_t depth, int64_t cols) {
+    const int64_t tiles = groups * ceil_div(depth, kTile) * ceil_div(cols, kTile), fit = num_sms() / 2 / tiles;
+    const int64_t mean = rows / (groups < rows ? groups : rows);
+    if (mean < kRowsToSplit) return 1;
+    int64_t parts = 1;
+    while (parts < fit && (parts + 1) * kPartRows <= mean && (parts + 1) * (parts + 1) * tiles * kPartCost <= mean) ++parts;
+    return parts;
 }
 
 int check_sizes(int64_t rows, int64_t groups, int64_t depth, int64_t cols, const void* offsets) {
@@ -787,10 +863,17 @@ extern "C" int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, in
                        : launch<kRows16, false, 1>(ma, mb, p, tiles, stream);
 }
 
+extern "C" int64_t bsp_grouped_weight_grad_workspace(int64_t rows, int64_t groups, int64_t depth, int64_t cols) {
+    if (rows < 1 || groups < 1 || depth < 1 || cols < 1 || groups > kMaxGroups || depth > 0x7fffffffLL || cols > 0x7fffffffLL)
+        return 0;
+    const int64_t parts = gradient_parts(rows, groups, depth, cols);
+    return parts > 1 ? parts * groups * depth * cols * 4 : 0;
+}
+
 extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* grad, int64_t ld_grad,
                                        const void* offsets, int offsets_i64, int64_t rows, int64_t groups,
-                                       int64_t depth, int64_t cols, void* out, int dtype, int32_t* status_word,
-                                       void* stream_) {
+                                       int64_t depth, int64_t cols, void* out, int dtype, void* workspace,
+                                       int64_t workspace_bytes, int32_t* status_word, void* stream_) {
     int st = check_sizes(rows, groups, depth, cols, offsets);
     if (st != BSP_OK) return st;
     if (rows < 1) return BSP_ERR_INVALID_ARG;
@@ -800,6 +883,9 @@ extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* 
         return BSP_ERR_INVALID_ARG;
     const int64_t tiles = groups * ceil_div(depth, kTile) * ceil_div(cols, kTile);
     if (tiles > 0x7fffffffLL - 65536) return BSP_ERR_UNSUPPORTED;
+    const int parts = (int)gradient_parts(rows, groups, depth, cols);
+    if (parts > 1 && (!workspace || !aligned16(workspace) || workspace_bytes < parts * groups * depth * cols * 4))
+        return BSP_ERR_INVALID_ARG;
     CUtensorMap ma, mb[3] = {};
     if ((st = rows_map(&ma, grad, dtype, rows, cols, ld_grad, 64)) != BSP_OK) return st;
     if ((st = rows_map(&mb[0], x, dtype, rows, depth, ld_x, 64)) != BSP_OK) return st;
@@ -810,14 +896,23 @@ extern "C" int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* 
     p.rows = (int)rows;
     p.cols = (int)cols;
     p.out_rows = (int)depth;
-    p.out = out;
-    p.out_dtype = dtype;
+    p.parts = parts;
+    p.out = parts > 1 ? workspace : out;
+    p.out_dtype = parts > 1 ? BSP_F32 : dtype;
     const uint32_t fmt = dtype == BSP_BF16 ? 1u : 0u;
     p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(kTile >> 4) << 24);
     p.status = status_word;
+    cudaStream_t stream = (cudaStream_t)stream_;
+    if (parts > 1) {
+        if ((st = launch<kGrad16, true, 1>(ma, mb, p, tiles * parts, stream)) != BSP_OK) return st;
+        const int64_t quads = groups * depth * cols / 4;
+        auto join = dtype == BSP_F16 ? join_parts_kernel<__half> : join_parts_kernel<__nv_bfloat16>;
+        return launch_overlapped(join, dim3((unsigned)ceil_div(quads, kJoinThreads)), kJoinThreads, 0, 1, stream,
+                                 (const float4*)workspace, quads, parts, (uint2*)out);
+    }
     const bool two = tile_halves(groups * ceil_div(depth, 2 * kTile) * ceil_div(cols, kTile), rows, groups) == 2;
-    return two ? launch<kGrad16, true, 2>(ma, mb, p, tiles, (cudaStream_t)stream_)
-               : launch<kGrad16, true, 1>(ma, mb, p, tiles, (cudaStream_t)stream_);
+    return two ? launch<kGrad16, true, 2>(ma, mb, p, tiles, stream)
+               : launch<kGrad16, true, 1>(ma, mb, p, tiles, stream);
 }
 
 extern "C" int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x, const float* scale_x,

@@ -21,6 +21,7 @@ struct Params {
     int rows;        // T
     int cols;        // extent of the output's contiguous dimension
     int out_rows;    // weight gradient: rows of one group's output
+    int parts;       // weight gradient: parts that a group's rows are split into (more than one: fp32 sums to be joined)
     int depth;       // rows product: contraction length
     void* out;
     int out_dtype;

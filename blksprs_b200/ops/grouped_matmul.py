@@ -156,10 +156,13 @@ def _weight_gradient(x: Tensor, grad: Tensor, group_offsets: Tensor, groups: int
     if not ld_grad:
         grad, ld_grad = _copied(grad, True), cols
     out = x.new_empty((groups, depth, cols))
-    status = _cabi.lib().bsp_grouped_weight_grad(
+    lib = _cabi.lib()
+    size = lib.bsp_grouped_weight_grad_workspace(rows, groups, depth, cols)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    status = lib.bsp_grouped_weight_grad(
         x.data_ptr(), ld_x, grad.data_ptr(), ld_grad, group_offsets.data_ptr(), group_offsets.dtype is torch.int64,
-        rows, groups, depth, cols, out.data_ptr(), _16_BIT[x.dtype], status_word(device).data_ptr(),
-        _cabi.stream_handle(device))
+        rows, groups, depth, cols, out.data_ptr(), _16_BIT[x.dtype], workspace.data_ptr() if size else None, size,
+        status_word(device).data_ptr(), _cabi.stream_handle(device))
     if status:
         _cabi.check(status, "bsp_grouped_weight_grad")
     return out

@@ -435,10 +435,15 @@ int bsp_grouped_matmul(const void* x, int64_t ld_x, const void* w, int64_t group
 
 /* out[e] = sum over the rows t of group e of x[t, :]^T * grad[t, :]; zero for
  * a group without rows.  x: (rows, depth), grad: (rows, cols), out: contiguous
- * (groups, depth, cols); types and sizes as above, rows >= 1. */
+ * (groups, depth, cols); types and sizes as above, rows >= 1.
+ * workspace: 16-byte aligned, of at least
+ * bsp_grouped_weight_grad_workspace bytes, written by the call (fp32 sums of
+ * parts of the rows, where there are few tiles and many rows); NULL where that
+ * is 0. */
+int64_t bsp_grouped_weight_grad_workspace(int64_t rows, int64_t groups, int64_t depth, int64_t cols);
 int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* grad, int64_t ld_grad, const void* offsets,
                             int offsets_i64, int64_t rows, int64_t groups, int64_t depth, int64_t cols, void* out,
-                            int dtype, int32_t* status_word, void* stream);
+                            int dtype, void* workspace, int64_t workspace_bytes, int32_t* status_word, void* stream);
 
 /* out[t, n] = sum over the blocks b of 128 contraction values of
  * scale_x[t, b] * scale_w[e, b, n / 128] * (x[t, b] . w[e, b, n]) for the rows

@@ -355,9 +355,45 @@ def test_output_beyond_32_bit_offsets():
     assert not out[0].any() and not out[70000].any()
 
 
-def test_weight_gradient_of_very_many_rows():
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("stored", ["kn", "nk"])
+@pytest.mark.parametrize("sizes,depth,cols", [
+    ([1024], 8, 8), ([4100], 264, 136), ([1, 0, 12345, 70, 3], 72, 264), ([0, 9000, 0], 520, 40), ([5000, 5001], 256, 512),
+    ([40000], 128, 1032)], ids=str)
+def test_weight_gradient_in_parts(sizes, depth, cols, stored, dtype):
+    """Few tiles, many rows: parts without rows, parts that end inside a step, rows before and behind the groups."""
+    from blksprs_b200 import _cabi
+    x, w, grad, offsets = make(sizes, depth, cols, dtype, seed=depth, stored=stored, before=9, behind=21)
+    assert _cabi.lib().bsp_grouped_weight_grad_workspace(x.shape[0], len(sizes), depth, cols) > 0
+    x[:9] = grad[-21:] = float("nan")
+    check_training(torch.nan_to_num(x), w, torch.nan_to_num(grad), offsets)
+    import blksprs_b200 as bs
+    x, w = x.requires_grad_(), w.requires_grad_()
+    first = torch.autograd.grad(bs.ops.grouped_matmul(x, w, offsets), w, grad)[0]
+    clean = torch.autograd.grad(bs.ops.grouped_matmul(torch.nan_to_num(x.detach()), w, offsets), w, torch.nan_to_num(grad))[0]
+    assert torch.equal(first, clean)
+
+
+def test_weight_gradient_needs_its_workspace():
+    """Refused before anything is launched: no workspace, one that is too small, one that is not aligned."""
+    from blksprs_b200 import _cabi
+    x, w, grad, offsets = make([5000], 64, 72, BF16)
+    lib, out = _cabi.lib(), torch.full((1, 64, 72), 3.0, dtype=BF16, device=DEV)
+    size = lib.bsp_grouped_weight_grad_workspace(5000, 1, 64, 72)
+    workspace = torch.empty(size + 16, dtype=torch.uint8, device=DEV)
+    for at, given in ((None, size), (workspace.data_ptr(), size - 1), (workspace.data_ptr() + 4, size)):
+        assert lib.bsp_grouped_weight_grad(x.data_ptr(), 64, grad.data_ptr(), 72, offsets.data_ptr(), 0, 5000, 1, 64, 72,
+                                           out.data_ptr(), 1, at, given, None,
+                                           _cabi.stream_handle(x.device)) == _cabi.ERR_INVALID_ARG
+    torch.cuda.synchronize()
+    assert bool((out == 3.0).all())
+
+
+@pytest.mark.parametrize("groups", [1, 64])
+def test_weight_gradient_of_very_many_rows(groups):
     """A wait for a whole contraction may last longer than the second after which one that makes no progress ends.
-    One group of 2^29 rows and 13 more: its weight gradient is one tile, 8.4 million steps and 2.7 seconds long.
+    One group of 2^29 rows and 13 more: its weight gradient is one tile, 8.4 million steps and 2.7 seconds long where
+    63 other groups (without rows) leave too few pairs for parts, and in 74 parts where there is no other group.
     Values are 1 or -1, repeated from 2^20 rows, so that every partial sum is an integer below 2^24 and the sums are
     exact; one rounding."""
     import blksprs_b200 as bs
@@ -365,7 +401,7 @@ def test_weight_gradient_of_very_many_rows():
     part, times, rest = 2 ** 20, 512, 13
     gen = torch.Generator().manual_seed(5)
     x, grad, w = ((torch.randint(0, 2, shape, generator=gen) * 2 - 1).to(BF16).to(DEV)
-                  for shape in ((part, 8), (part, 8), (1, 8, 8)))
+                  for shape in ((part, 8), (part, 8), (groups, 8, 8)))
     w.requires_grad_()
     products = x.double()[:, :, None] * grad.double()[:, None, :]
     assert products.cumsum(0).abs().max() * times < 2 ** 24
@@ -373,14 +409,14 @@ def test_weight_gradient_of_very_many_rows():
     forward = (x.double() @ w[0].detach().double()).to(BF16)
     del products
     long = torch.cat([x.repeat(times, 1), x[:rest]]).requires_grad_()
-    offsets = torch.tensor([0, long.shape[0]], device=DEV)
+    offsets = torch.tensor([0] + [long.shape[0]] * groups, device=DEV)
     out = bs.ops.grouped_matmul(long, w, offsets)
     for i in (0, 1, times // 2, times - 1):
         assert torch.equal(out[i * part:(i + 1) * part], forward)
     assert torch.equal(out[times * part:], forward[:rest])
     out.backward(torch.cat([grad.repeat(times, 1), grad[:rest]]))
     check_device_status()
-    assert torch.equal(w.grad[0], want.to(BF16))
+    assert torch.equal(w.grad[0], want.to(BF16)) and not w.grad[1:].any()
     last = (grad.double() @ w[0].detach().double().T).to(BF16)
     assert torch.equal(long.grad[(times - 1) * part:times * part], last)
     assert torch.equal(long.grad[times * part:], last[:rest])

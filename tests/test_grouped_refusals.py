@@ -116,11 +116,13 @@ def test_c_entries_refuse_without_a_device():
         assert rows(**change) == unsupported, change
 
     def grad(x=p, ld_x=64, g=p, ld_g=64, offsets=p, T=4, E=2, K=64, N=64, out=p, dtype=1):
-        return lib.bsp_grouped_weight_grad(x, ld_x, g, ld_g, offsets, 0, T, E, K, N, out, dtype, None, None)
+        return lib.bsp_grouped_weight_grad(x, ld_x, g, ld_g, offsets, 0, T, E, K, N, out, dtype, None, 0, None, None)
 
     for change in (dict(T=0), dict(x=None), dict(g=p + 4), dict(K=4), dict(N=4), dict(ld_g=32), dict(offsets=None)):
         assert grad(**change) == bad, change
     assert grad(dtype=2) == unsupported
+    for sizes in ((0, 1, 64, 64), (64, 0, 64, 64), (64, 1, 0, 64), (64, 1, 64, 0), (64, 5000, 64, 64)):
+        assert lib.bsp_grouped_weight_grad_workspace(*sizes) == 0
 
     def scaled(x=p, ld_x=64, tx=3, sx=p, w=p, sg=64 * 64, ld_w=64, tw=4, sw=p, T=4, E=2, K=64, N=64, out=p, dtype=1):
         return lib.bsp_grouped_matmul_scaled(x, ld_x, tx, sx, 1, 1, w, sg, ld_w, tw, sw, 1, 1, 1, p, 0, T, E, K, N,
