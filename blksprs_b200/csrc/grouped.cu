@@ -435,14 +435,15 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                             for (int i = lane; i < pieces; i += 32)
                                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + i * 16), "r"(0) : "memory");
                         }
-                        // what is zeroed here is read by this SM's tensor core only: visible to it after the proxy fence,
-                        // and the first CTA issues the MMA after this CTA's arrival
+                        // what is zeroed here is read by this SM's tensor core, in an MMA that the first CTA issues: the
+                        // second CTA's zeros pass to the async proxy here and to the first CTA with the arrival (release
+                        // at cluster scope; one per group and tile, so its cost does not count)
                         asm volatile("fence.proxy.async;" ::: "memory");
                         __syncwarp();
                         if (rank == 1) {
-                            if (lane == 0) mbar_arrive_pair(map_to_rank(zeroed_bar + 8 * s, 0));
+                            if (lane == 0) mbar_publish_pair(map_to_rank(zeroed_bar + 8 * s, 0));
                         } else {
-                            alive = wait_all(zeroed_bar + 8 * s, (tail_parity >> s) & 1, abort_flag, p.status);
+                            alive = wait_all<true>(zeroed_bar + 8 * s, (tail_parity >> s) & 1, abort_flag, p.status);
                             if (!alive) break;
                         }
                         tail_parity ^= 1u << s;

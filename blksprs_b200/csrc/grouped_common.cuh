@@ -53,6 +53,19 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The forms that do: writes of this warp before the arrival are visible behind a wait that saw it in the other CTA.
+__device__ __forceinline__ void mbar_publish_pair(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+}
 // mbar_wait without a call: a call would have the epilogue's sums saved around it.
 __device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
                                              bool honor_abort = true) {
@@ -90,13 +103,16 @@ __device__ __forceinline__ float4 shared_float4(uint32_t at) {
 // progress: for waits that last as long as a whole contraction (the sums of 2^28 rows and more take a second): entries
 // of the ring asked for so far.  The time then counts from when that number last changed; a ring that stands still is
 // found by the roles that wait for its entries.
+// CLUSTER: acquires what the other CTA published with its arrival.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
                                          const volatile int* progress = nullptr) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    auto through = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+    if (__all_sync(0xffffffffu, through())) return true;
     unsigned long long t0 = 0;
     int seen = 0;
     for (uint32_t it = 1;; ++it) {
-        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if (__all_sync(0xffffffffu, through())) return true;
         if ((it & 0xff) == 0) {
             const unsigned long long now = global_timer();
             if (t0 == 0) t0 = now;

@@ -1,0 +1,51 @@
+"""Grouped products and 8-bit rounding where they can go wrong at their edges: both kernels of each product, values that
+are not finite next to a group, very wide outputs, scales far from one, recorded and forward-mode calls.
+
+Most operands are small whole numbers, so that every product and sum is exact in the output type and results have to be
+equal; the other tolerances are those of the grouped products' own tests.
+"""
+import pytest
+import torch
+
+from gpu_util import DEV
+from test_gpu_p_grouped_matmul import BF16, FP16, FP32, bounds_of, plain_weight_gradient
+
+pytestmark = pytest.mark.gpu
+
+
+def whole(*shape, gen, dtype=FP16, high=1):
+    return torch.randint(-high, high + 1, shape, generator=gen).to(dtype).to(DEV)
+
+
+def weight_gradient(x, grad, offsets):
+    import blksprs_b200 as bs
+    w = torch.zeros((offsets.numel() - 1, x.shape[1], grad.shape[1]), dtype=x.dtype, device=DEV).requires_grad_(True)
+    return torch.autograd.grad(bs.ops.grouped_matmul(x, w, offsets), w, grad)[0]
+
+
+# sizes of groups, depth, columns: tiles of 256 rows, of 512 rows (a few hundred tiles, long groups), rows in parts
+GRADIENT_FORMS = [([17, 1, 31, 63, 79, 95, 15, 130], 264, 392), ([33] * 40, 136, 520),
+                  ([385 + 13 * i for i in range(8)], 2048, 2568), ([4101], 264, 136), ([3, 9000, 2], 72, 264)]
+
+
+@pytest.mark.parametrize("sizes,depth,cols", GRADIENT_FORMS, ids=["short", "equal", "tall", "parts", "parts-of-one"])
+def test_weight_gradient_keeps_out_the_rows_of_other_groups(sizes, depth, cols):
+    """The last rows of a group share sixteen rows of a tile with the next group's, which are NaN and infinity here in
+    every second group and behind the last; both blocks of a pair clear theirs before one of them multiplies."""
+    gen = torch.Generator().manual_seed(depth)
+    before, behind = 5, 40
+    rows = before + sum(sizes) + behind
+    x, grad, offsets = whole(rows, depth, gen=gen), whole(rows, cols, gen=gen), bounds_of(sizes, before).to(DEV)
+    want = plain_weight_gradient(x, grad, offsets)
+    assert want.abs().max() <= 2048        # whole numbers that fp16 holds
+    bounds = offsets.tolist()
+    for clean in (0, 1):
+        spoilt, spoilt_grad = x.clone(), grad.clone()
+        for e, (a, b) in enumerate(zip([0, *bounds], [*bounds, rows])):      # part e is group e - 1
+            if e % 2 != clean or e in (0, len(bounds)):
+                spoilt[a:b], spoilt_grad[a:b] = float("nan"), float("inf")
+        for _ in range(3):
+            got = weight_gradient(spoilt, spoilt_grad, offsets)
+            for e in range(len(sizes)):
+                if (e + 1) % 2 == clean:
+                    assert torch.equal(got[e].double(), want[e]), (clean, e)
