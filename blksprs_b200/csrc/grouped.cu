@@ -726,10 +726,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 }
 
 // Sums of the parts, added up in their order and rounded once.  Four values per thread.
+// The launch before writes `sums` while this one may already have started, so they are not declared unchanging
+// (__restrict__ would let their loads go ahead of the wait for that launch).
 constexpr int kJoinThreads = 128;
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads)
-join_parts_kernel(const float4* __restrict__ sums, int64_t quads, int parts, uint2* __restrict__ out) {
+join_parts_kernel(const float4* sums, int64_t quads, int parts, uint2* out) {
     let_next_launch();
     wait_for_previous_launch();
     const int64_t i = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x;

@@ -49,3 +49,14 @@ def test_weight_gradient_keeps_out_the_rows_of_other_groups(sizes, depth, cols):
             for e in range(len(sizes)):
                 if (e + 1) % 2 == clean:
                     assert torch.equal(got[e].double(), want[e]), (clean, e)
+
+
+def test_parts_are_joined_after_they_are_written():
+    """Many split weight gradients one behind the other, every one on other rows and in the workspace of the one before."""
+    gen = torch.Generator().manual_seed(31)
+    offsets = bounds_of([8200]).to(DEV)
+    x, grad = whole(8200, 64, gen=gen), whole(8200, 136, gen=gen)
+    got = [weight_gradient(x.roll(i, 0), grad, offsets) for i in range(60)]
+    for i, g in enumerate(got):
+        want = plain_weight_gradient(x.roll(i, 0), grad, offsets)
+        assert want.abs().max() <= 2048 and torch.equal(g.double(), want), i
