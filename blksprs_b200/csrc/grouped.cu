@@ -617,7 +617,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 const int c = o.c0 + (int)rank * kHalf + quarter * 32;
                 const int64_t first = MODE == kRows16 ? o.r0 : (int64_t)o.group * p.out_rows + o.r0;
                 char* out = (char*)p.out + first * row_bytes + (int64_t)c * esize;
-                const int bytes = (p.cols - c) * 2;
+                const int bytes = min(p.cols - c, 32) * 2;
                 const bool computed = steps > 0;    // a group without rows has a gradient of zero
 #pragma unroll 1
                 for (int h = 0; h < kHalves; ++h) {

@@ -358,7 +358,7 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                             words[j] = p.out_dtype == BSP_F16 ? pack2<__half>(sum[h][2 * j], sum[h][2 * j + 1])
                                                               : pack2<__nv_bfloat16>(sum[h][2 * j], sum[h][2 * j + 1]);
                         stage_transposed(staging, words);
-                        store_staged(staging, out + h * 32 * row_bytes, row_bytes, rows - h * 32, (p.cols - c) * 2);
+                        store_staged(staging, out + h * 32 * row_bytes, row_bytes, rows - h * 32, min(p.cols - c, 32) * 2);
                     }
                 }
             }

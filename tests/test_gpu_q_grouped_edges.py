@@ -60,3 +60,38 @@ def test_parts_are_joined_after_they_are_written():
     for i, g in enumerate(got):
         want = plain_weight_gradient(x.roll(i, 0), grad, offsets)
         assert want.abs().max() <= 2048 and torch.equal(g.double(), want), i
+
+
+def spoil_free_memory(*shape):
+    """What the next allocation of this size holds before it is written."""
+    torch.empty(shape, dtype=torch.int16, device=DEV).fill_(-1)
+
+
+def test_more_than_2_to_30_columns():
+    """Byte counts behind a column pass 31 bits: the forward product of one row and the weight gradient of two."""
+    import blksprs_b200 as bs
+    cols = 2 ** 30 + 8
+    gen = torch.Generator().manual_seed(7)
+    x = torch.zeros((1, 8), dtype=BF16, device=DEV)
+    x[0, 3] = 2.0
+    w = torch.empty((1, 8, cols), dtype=BF16, device=DEV)
+    line = whole(2 ** 20, gen=gen, dtype=BF16, high=9)
+    for k in range(8):
+        w[0, k, :2 ** 30].view(-1, 2 ** 20).copy_(line.roll(k))
+        w[0, k, 2 ** 30:] = k + 1
+    offsets = bounds_of([1]).to(DEV)
+    spoil_free_memory(1, cols)
+    out = bs.ops.grouped_matmul(x, w, offsets)
+    assert torch.equal(out, 2 * w[0, 3:4])
+    grad = w[0, 2:4].clone()
+    del out, w
+    torch.cuda.empty_cache()
+    x = whole(2, 8, gen=gen, dtype=BF16, high=3)
+    w = torch.empty((1, 8, cols), dtype=BF16, device=DEV).requires_grad_(True)
+    product = bs.ops.grouped_matmul(x, w, bounds_of([2]).to(DEV))
+    spoil_free_memory(1, 8, cols)
+    got, = torch.autograd.grad(product, w, grad)
+    for k in range(8):
+        assert torch.equal(got[0, k], x[0, k] * grad[0] + x[1, k] * grad[1]), k
+    del got, w, grad, product
+    torch.cuda.empty_cache()
