@@ -161,9 +161,10 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
 }
 
 // 16 bits: the rows of a group are cut into the fewest tiles of at most `most` rows, all of about the same height.
+// (The largest m are close to 2^31: m + n - 1 would pass it.)
 __device__ __forceinline__ int tile_height(int m, int most) {
     const int n = (m + most - 1) / most;
-    return n == 0 ? 0 : round_up((m + n - 1) / n, 32);
+    return n == 0 ? 0 : round_up((m - 1) / n + 1, 32);
 }
 // N of either half's MMAs.
 __device__ __forceinline__ int half_n(int n, int half) {

@@ -95,3 +95,35 @@ def test_more_than_2_to_30_columns():
         assert torch.equal(got[0, k], x[0, k] * grad[0] + x[1, k] * grad[1]), k
     del got, w, grad, product
     torch.cuda.empty_cache()
+
+
+def test_nearly_2_to_31_rows():
+    """Heights of tiles are found without leaving 31 bits: one group of 2^31 - 520 rows, and a weight gradient of as many."""
+    import sys
+    import blksprs_b200 as bs
+    rows, part = 2 ** 31 - 520, 2 ** 20
+    gen = torch.Generator().manual_seed(8)
+    line, w = whole(part, 8, gen=gen, dtype=BF16, high=3), whole(1, 8, 8, gen=gen, dtype=BF16, high=3)
+    times, rest = divmod(rows, part)
+    x = torch.empty((rows, 8), dtype=BF16, device=DEV)
+    x[:times * part].view(times, part, 8).copy_(line)
+    x[times * part:] = line[:rest]
+    spoil_free_memory(rows, 8)
+    out = bs.ops.grouped_matmul(x, w, torch.tensor([0, rows], device=DEV))
+    want = (line.double() @ w[0].double()).to(BF16)
+    for i in range(0, times, 64):
+        assert bool((out[i * part:min(i + 64, times) * part].view(-1, part, 8) == want).all()), i
+    assert torch.equal(out[times * part:], want[:rest])
+    del out, x
+    torch.cuda.empty_cache()
+    x = torch.empty((2, rows), dtype=BF16, device=DEV)
+    for r in range(2):
+        x[r, :times * part].view(times, part).copy_(line[:, r])
+        x[r, times * part:] = r + 1
+    grad = whole(2, 8, gen=gen, dtype=BF16, high=3)
+    spoil_free_memory(1, rows, 8)
+    got = sys.modules["blksprs_b200.ops.grouped_matmul"]._weight_gradient(x, grad, bounds_of([2]).to(DEV), 1)
+    for c in range(8):
+        assert torch.equal(got[0, :, c], x[0] * grad[0, c] + x[1] * grad[1, c]), c
+    del got, x, grad
+    torch.cuda.empty_cache()
