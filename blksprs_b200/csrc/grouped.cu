@@ -56,7 +56,8 @@ constexpr int kEpiWarps = 8;
 constexpr int kTile = 256;            // M of a pair's tile, and most of an MMA's N
 constexpr int kHalf = 128;            // M in either CTA
 constexpr int kScaleSlots = 4;        // groups of four steps whose scales are staged ahead
-constexpr int kScaleSlot = 4 * kHalf + 8;   // floats of a slot: four per row of the CTA's half, four of either block of w
+constexpr int kScaleSlot = 4 * kHalf + 12;  // words of a slot: four scales per row of the CTA's half, four of either block of
+constexpr int kScaleFlag = (4 * kHalf + 8) * 4;     // w, whether these steps are multiplied by both, and three unused
 constexpr int kBand = 8;              // row tiles that are walked together for every column tile
 
 enum Mode { kRows16, kGrad16, kRows8 };
@@ -488,8 +489,30 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             __syncwarp();
         } else if (F8 && warp == 3) {
             // ---------------- scales: this CTA's rows' and the tile's two blocks of w's, steps ahead ----------------
+            // Four steps' scales are on their way while those of the four before are looked at: whether a product of theirs may
+            // leave fp32's range.  The least and the greatest of either operand's tell (a finer answer for 32 rows and one
+            // block of w cost 25 us of 300, and asking in the epilogue 10), and fewer than four steps count as one that may.
             uint32_t at = 0;
             bool alive = true;
+            int rows_before = 0, cols_before = 0, steps_before = 0;       // of what is on its way
+            auto publish = [&](uint32_t slot) {
+                __syncwarp();
+                const uint32_t from = scales + slot * kScaleSlot * 4;
+                float x_low = 1.0f, x_high = 1.0f, w_low = 1.0f, w_high = 1.0f;
+                auto bound = [](float& low, float& high, const float4& v) {
+                    low = fminf(fminf(low, fminf(fabsf(v.x), fabsf(v.y))), fminf(fabsf(v.z), fabsf(v.w)));
+                    high = fmaxf(fmaxf(high, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                };
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i * 32 + lane < rows_before) bound(x_low, x_high, shared_float4(from + (i * 32 + lane) * 16));
+                bound(w_low, w_high, shared_float4(from + kHalf * 16));
+                if (cols_before > 128) bound(w_low, w_high, shared_float4(from + kHalf * 16 + 16));
+                const bool twice = steps_before < 4 || __any_sync(0xffffffffu, !in_range(x_low * w_low) || !in_range(x_high * w_high));
+                if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(from + kScaleFlag), "r"((int)twice) : "memory");
+                __syncwarp();
+                mbar_arrive(sfull_bar + 8 * slot);
+            };
             for (int t = first_tile; t < n_tiles && alive; t += tile_step) {
                 const Tile o = tile_at(t);
                 const int steps = (o.depth + KE - 1) / KE;
@@ -510,10 +533,18 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                                     copy_async_4(to + (i * 32 + lane) * 16 + j * 4, sx + i * 32 * p.sx_row + (k + j) * p.sx_block);
                     if (lane < 8 && k + (lane & 3) < steps && (lane >> 2) * 128 < o.cols)
                         copy_async_4(to + kHalf * 16 + lane * 4, sw + (k + (lane & 3)) * p.sw_k);
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sfull_bar + 8 * slot) : "memory");
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (at > 0) {
+                        asm volatile("cp.async.wait_group 1;" ::: "memory");
+                        publish((at - 1) % kScaleSlots);
+                    }
+                    rows_before = o.rows - first;
+                    cols_before = o.cols;
+                    steps_before = steps - k;
                 }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
+            if (at > 0 && alive) publish((at - 1) % kScaleSlots);
             __syncwarp();
         }
     } else {
@@ -546,15 +577,43 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 float sum[128];
 #pragma unroll
                 for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
-                // the scales of four steps (this row's times the one of these 128 columns)
+                // one step's sums, 32 columns at a time; columns behind n, and rows behind the tile's, hold what came
+                // before: they are not stored
+                auto each_32_of_step = [&](auto add) {
+                    if (!wait_all(tfull_bar + 8 * (acc % kAccs), (acc / kAccs) & 1, abort_flag, p.status)) return false;
+                    tc_fence_after();
+                    const uint32_t from = lanes + acc % kAccs * kN + part * 128;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t v[32];
+                        tc_ld32(from + i * 32, v);
+                        tc_wait_ld();
+                        if (i == 3) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive_pair(tempty_first + 8 * (acc % kAccs));
+                        }
+                        add(i, v);
+                    }
+                    ++acc;
+                    return true;
+                };
+                // the scales of four steps (this row's times the one of these 128 columns), or `twice`: a product may leave
+                // fp32's range, and both scales stay where they are for these steps
                 float scale[4];
+                bool twice = false;
+                auto release = [&]() {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sempty_bar + 8 * (scale_group % kScaleSlots));
+                    ++scale_group;
+                };
+                auto scales_at = [&]() { return scales + scale_group % kScaleSlots * kScaleSlot * 4; };
                 auto fetch = [&]() {
-                    const uint32_t slot = scale_group % kScaleSlots, from = scales + slot * kScaleSlot * 4;
+                    const uint32_t slot = scale_group % kScaleSlots, from = scales_at();
                     if (!wait_all(sfull_bar + 8 * slot, (scale_group / kScaleSlots) & 1, abort_flag, p.status)) return false;
                     const float4 x = shared_float4(from + (quarter * 32 + lane) * 16), w = shared_float4(from + kHalf * 16 + part * 16);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(sempty_bar + 8 * slot);
-                    ++scale_group;
+                    twice = __float_as_int(shared_float(from + kScaleFlag)) != 0;
+                    if (!twice) release();
                     scale[0] = x.x * w.x;
                     scale[1] = x.y * w.y;
                     scale[2] = x.z * w.z;
@@ -564,27 +623,27 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 for (int k0 = 0; k0 < steps && alive; k0 += 4) {
                     alive = fetch();
                     if (!alive) break;
+                    if (twice) {
+                        // (with every step so: 341-371 instead of 304 us)
 #pragma unroll 1
-                    for (int kk = 0; kk < 4 && k0 + kk < steps; ++kk, ++acc) {
-                        alive = wait_all(tfull_bar + 8 * (acc % kAccs), (acc / kAccs) & 1, abort_flag, p.status);
-                        if (!alive) break;
-                        tc_fence_after();
-                        const float f = kk == 0 ? scale[0] : kk == 1 ? scale[1] : kk == 2 ? scale[2] : scale[3];
-                        // columns behind n, and rows behind the tile's, hold what came before: they are not stored
-                        const uint32_t from = lanes + acc % kAccs * kN + part * 128;
+                        for (int kk = 0; kk < 4 && k0 + kk < steps && alive; ++kk) {
+                            const float2 factors = in_order(shared_float(scales_at() + (quarter * 32 + lane) * 16 + kk * 4),
+                                                            shared_float(scales_at() + kHalf * 16 + part * 16 + kk * 4));
+                            alive = each_32_of_step([&](int i, const uint32_t* v) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t v[32];
-                            tc_ld32(from + i * 32, v);
-                            tc_wait_ld();
-                            if (i == 3) {
-                                tc_fence_before();
-                                __syncwarp();
-                                if (lane == 0) mbar_arrive_pair(tempty_first + 8 * (acc % kAccs));
-                            }
+                                for (int j = 0; j < 32; j += 2) add_pair(sum[32 * i + j], sum[32 * i + j + 1], v[j], v[j + 1], factors);
+                            });
+                        }
+                        release();
+                        continue;
+                    }
+#pragma unroll 1
+                    for (int kk = 0; kk < 4 && k0 + kk < steps && alive; ++kk) {
+                        const float f = kk == 0 ? scale[0] : kk == 1 ? scale[1] : kk == 2 ? scale[2] : scale[3];
+                        alive = each_32_of_step([&](int i, const uint32_t* v) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) sum[32 * i + j] = fmaf(__uint_as_float(v[j]), f, sum[32 * i + j]);
-                        }
+                        });
                     }
                 }
                 if (!alive) break;

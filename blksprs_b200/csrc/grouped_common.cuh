@@ -98,6 +98,28 @@ __device__ __forceinline__ float4 shared_float4(uint32_t at) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
 }
+// ---- scales of 8-bit steps -----------------------------------------------------------
+// A step's sums are multiplied by two scales.  Their product is one factor, unless it leaves fp32's normal numbers: then
+// it would be infinite (and infinity times a sum of 0 is NaN), have lost bits, or be 0, where the sum times both need not
+// be.  Such a step multiplies twice: by the larger first where the product is small, by the smaller first where it is
+// large, so that what lies between overflows or vanishes only if the result does (sums are 0 or 2^-32 .. 2^39).
+__device__ __forceinline__ bool in_range(float product) {
+    return fabsf(product) >= 1.17549435e-38f && fabsf(product) <= 3.40282347e38f;
+}
+// The two factors, in order; {1, product} where that is in range, or a scale is 0.
+__device__ __forceinline__ float2 in_order(float a, float b) {
+    const float product = a * b;
+    if (in_range(product) || a == 0.0f || b == 0.0f) return make_float2(1.0f, product);
+    const bool smaller_first = fabsf(product) > 1.0f;
+    return (fabsf(a) > fabsf(b)) == smaller_first ? make_float2(b, a) : make_float2(a, b);
+}
+// sums += values * first * second, two neighbouring ones at a time.
+__device__ __forceinline__ void add_pair(float& x, float& y, uint32_t v, uint32_t w, float2 factors) {
+    asm("{\n\t.reg .b64 s, v, f;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 f, {%4, %4};\n\tmul.rn.f32x2 v, v, f;\n\t"
+        "mov.b64 f, {%5, %5};\n\tfma.rn.f32x2 s, v, f, s;\n\tmov.b64 {%0, %1}, s;\n\t}"
+        : "+f"(x), "+f"(y) : "r"(v), "r"(w), "f"(factors.x), "f"(factors.y));
+}
+
 // A bounded wait of a whole warp: true only if it succeeded for every lane, so that the lanes go on or leave
 // together.  The first try is a straight line: 27 cycles on a barrier that is through, against 76 for the loop.
 // progress: for waits that last as long as a whole contraction (the sums of 2^28 rows and more take a second): entries

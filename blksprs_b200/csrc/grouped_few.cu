@@ -9,7 +9,8 @@
 // the same bits on every run.
 //
 // A = weights (M = 128 features, accumulator lanes), B = rows (N = their number rounded up to 16).  8 bits: the
-// scale of a step belongs to the accumulator's columns; 32 of them are read from shared memory as vectors.
+// scale of a step belongs to the accumulator's columns; two factors for each are read from shared memory as vectors.
+// (A second multiplication costs nothing here; whether one is needed, decided in the epilogue, cost 1-3 of 45 us.)
 //
 // What it measured on a B200: 128 rows over 32 groups, 4096 x 2048 bf16: 77 us, 521 MB
 // of weights at 6.8 TB/s (a plain copy moves 6.5); in 8 bits 45 us, 5.8 TB/s.  Two rows of two groups, 2048 x 4096 bf16
@@ -33,8 +34,8 @@ constexpr int kFewN = 64;
 constexpr int kFewStages = 4;
 constexpr int kFewStageBytes = kFewM * 128 + kFewN * 128;
 constexpr int kFewAccs = 2;                    // 8 bits: one per step, 16 bits: the first one
-constexpr int kFewScaleSlots = 4;              // steps in groups of four
-constexpr int kFewScaleSlot = 4 * kFewN + 4;   // floats: one per step and row, one per step
+constexpr int kFewScaleSlots = 3;              // steps in groups of four
+constexpr int kFewScaleSlot = 4 * kFewN * 2;   // floats: two factors per step and row
 
 struct FewSmem {
     static constexpr int kData = kFewStages * kFewStageBytes;   // afterwards the partial sums, 64 x 128 floats
@@ -234,8 +235,21 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     } else if (warp == 6) {
         // ---------------- scales of four steps at a time (8 bits) ----------------
         if (F8) {
-            const float* sx = p.scale_x + (int64_t)r0 * p.sx_row;
+            // two factors for every step and row: what its two scales come to (one lane has two rows)
+            const float* sx = p.scale_x + (int64_t)(r0 + lane) * p.sx_row;
             const float* sw = p.scale_w + (int64_t)group * p.sw_group + (int64_t)(c0 / 128) * p.sw_n;
+            float x[2][4], w[4];
+            auto load = [&](int k0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t k = first_step + k0 + j;
+                    w[j] = k0 + j < steps ? sw[k * p.sw_k] : 0.0f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        x[h][j] = k0 + j < steps && h * 32 + lane < rows ? sx[h * 32 * p.sx_row + k * p.sx_block] : 0.0f;
+                }
+            };
+            load(0);
             for (int k0 = 0, at = 0; k0 < steps; k0 += 4, ++at) {
                 const int slot = at % kFewScaleSlots;
                 if (at >= kFewScaleSlots &&
@@ -243,17 +257,16 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     break;
                 const uint32_t to = scales + slot * kFewScaleSlot * 4;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int64_t k = first_step + k0 + j;
-                    if (k0 + j < steps) {
-                        for (int r = lane; r < rows; r += 32)
-                            copy_async_4(to + (j * kFewN + r) * 4, sx + r * p.sx_row + k * p.sx_block);
-                        if (lane == j) copy_async_4(to + (4 * kFewN + j) * 4, sw + k * p.sw_k);
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 f = in_order(x[h][j], w[j]);
+                        asm volatile("st.shared.v2.f32 [%0], {%1, %2};"
+                                     ::"r"(to + (j * kFewN + h * 32 + lane) * 8), "f"(f.x), "f"(f.y) : "memory");
                     }
-                }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sfull_bar + 8 * slot) : "memory");
+                mbar_arrive(sfull_bar + 8 * slot);
+                load(k0 + 4);
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
         }
     }
@@ -280,26 +293,23 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         if (F8) {
             for (int k = 0; k < steps; ++k) {
                 const int slot = k / 4 % kFewScaleSlots;
-                const uint32_t from = scales + slot * kFewScaleSlot * 4 + (k & 3) * kFewN * 4;
+                const uint32_t from = scales + slot * kFewScaleSlot * 4 + (k & 3) * kFewN * 8;
                 complete = ((k & 3) != 0 || wait_all(sfull_bar + 8 * slot, (k / 4 / kFewScaleSlots) & 1, abort_flag, p.status)) &&
                            wait_all(tfull_bar + 8 * (k % kFewAccs), (k / kFewAccs) & 1, abort_flag, p.status);
                 if (!complete) break;
                 tc_fence_after();
-                const float w = shared_float(scales + slot * kFewScaleSlot * 4 + (4 * kFewN + (k & 3)) * 4);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (h * 32 < n) {
-                        // columns behind n, and scales behind the rows, hold anything: they are not stored
+                        // columns behind n hold anything: they are not stored
                         uint32_t v[32];
                         tc_ld32(lanes + k % kFewAccs * kFewN + h * 32, v);
                         tc_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 s = shared_float4(from + (h * 32 + j) * 4);
-                            sum[h][j] = fmaf(__uint_as_float(v[j]), s.x * w, sum[h][j]);
-                            sum[h][j + 1] = fmaf(__uint_as_float(v[j + 1]), s.y * w, sum[h][j + 1]);
-                            sum[h][j + 2] = fmaf(__uint_as_float(v[j + 2]), s.z * w, sum[h][j + 2]);
-                            sum[h][j + 3] = fmaf(__uint_as_float(v[j + 3]), s.w * w, sum[h][j + 3]);
+                        for (int j = 0; j < 32; j += 2) {
+                            const float4 f = shared_float4(from + (h * 32 + j) * 8);
+                            sum[h][j] = fmaf(__uint_as_float(v[j]) * f.x, f.y, sum[h][j]);
+                            sum[h][j + 1] = fmaf(__uint_as_float(v[j + 1]) * f.z, f.w, sum[h][j + 1]);
                         }
                     }
                 }

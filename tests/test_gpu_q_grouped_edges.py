@@ -127,3 +127,69 @@ def test_nearly_2_to_31_rows():
         assert torch.equal(got[0, :, c], x[0] * grad[0, c] + x[1] * grad[1, c]), c
     del got, x, grad
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("out_dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("side", ["small", "large"])
+@pytest.mark.parametrize("sizes,cols", [([1], 136), ([30, 0, 64, 1, 65], 136), ([5, 3], 4096), ([257, 1, 255, 0, 256], 392),
+                                        ([600], 2056)], ids=str)
+def test_scales_whose_product_leaves_fp32(sizes, cols, side, out_dtype):
+    """Scales are any fp32 numbers: products of two below 2^-126 or above 2^128 next to ordinary ones, with sums that
+    bring the result back into range, and sums of 0 where the product is infinite.  Both kernels of the product
+    (few rows with and without a split contraction, many rows).  Multiplying twice is one rounding more than the one
+    of the scales' product: the terms of a sum plus four, as for ordinary scales."""
+    import blksprs_b200 as bs
+    from test_gpu_p_grouped_matmul import assert_near, plain_scaled
+    gen = torch.Generator().manual_seed(sum(sizes) + cols)
+    rows, depth = sum(sizes), 1168
+    blocks = -(-depth // 128)
+    sign = -1.0 if side == "small" else 1.0
+    # which rows have ordinary products, ones on either side of the border, and ones outside
+    far = torch.tensor([0.0, 130.0, 142.0] if side == "small" else [0.0, 125.0, 130.0])
+    far = far[torch.randint(0, 3, (rows, 1), generator=gen)]
+    power = 70.0 + 5.0 * torch.randint(0, 3, (len(sizes), blocks, -(-cols // 128)), generator=gen)
+    group = torch.repeat_interleave(torch.arange(len(sizes)), torch.tensor(sizes))
+
+    def mantissa(*shape):
+        return (1.0 + torch.rand(shape, generator=gen)) * (1 - 2 * torch.randint(0, 2, shape, generator=gen))
+    # one exponent for a block of the rows whatever the columns: what a block of the weights has is taken off again
+    sw = mantissa(*power.shape) * 2.0 ** (sign * power)
+    sx = mantissa(rows, blocks) * 2.0 ** (sign * (far - 75.0))
+    # values whose sums are large where the scales are small, and small where they are large
+    magnitude = 2.0 ** (13 if side == "small" else -12)
+    x = torch.randn((rows, depth), generator=gen) * magnitude
+    x[torch.rand((rows, blocks), generator=gen).repeat_interleave(128, 1)[:, :depth] < 0.2] = 0.0
+    w = torch.randn((len(sizes), cols, depth), generator=gen) * magnitude
+    x, w = x.to(torch.float8_e5m2).to(DEV), w.to(torch.float8_e5m2).to(DEV).transpose(1, 2)
+    sx, sw, offsets = sx.to(DEV), sw.to(DEV), bounds_of(sizes).to(DEV)
+    products = sx.double()[:, :, None] * sw.double()[group.to(DEV)]
+    outside = (products.abs() < 2.0 ** -126) | (products.abs() >= 2.0 ** 128)
+    assert sx.isfinite().all() and sw.isfinite().all() and (rows < 8 or outside.any())
+    want, magnitudes = plain_scaled(x, sx, w, sw, offsets)
+    # no result overflows; the tolerance of the sums (2^-12.8 of their magnitude) covers half of bf16's smallest step, 2^-134
+    assert magnitudes.max() < 2.0 ** 127 and magnitudes[magnitudes > 0].min() > 2.0 ** -121
+    got = bs.ops.grouped_matmul_scaled(x, sx, w, sw, offsets, out_dtype=out_dtype)
+    assert_near(got, want, magnitudes, depth + 4)
+
+
+def test_scales_of_any_kind():
+    """A scale of 0, infinity or NaN reaches its own rows and columns only, next to products out of range."""
+    import blksprs_b200 as bs
+    from test_gpu_p_grouped_matmul import make_scaled
+    for sizes in ([40, 30], [400, 300]):
+        x, sx, w, sw, offsets = make_scaled(sizes, 256, 264, seed=2)
+        sx.fill_(2.0 ** -10)
+        sw[:, :, 2] = 3e38
+        clean = bs.ops.grouped_matmul_scaled(x, sx, w, sw, offsets)
+        assert clean.isfinite().all()
+        sx[3], sx[5, 1], sx[7, 0], sx[9], sx[11] = 0.0, float("nan"), float("inf"), 1e38, -1e-42
+        out = bs.ops.grouped_matmul_scaled(x, sx, w, sw, offsets)
+        assert not out[3].any() and out[5].isnan().all() and not out[7].isfinite().any()
+        keep = torch.ones(x.shape[0], dtype=torch.bool, device=DEV)
+        keep[[3, 5, 7, 9, 11]] = False
+        assert torch.equal(out[keep], clean[keep])
+        sw[1, 0, 1] = float("inf")
+        other = bs.ops.grouped_matmul_scaled(x, sx, w, sw, offsets)
+        assert not other[sizes[0]:, 128:256].isfinite().any()
+        assert torch.equal(other[sizes[0]:, :128], clean[sizes[0]:, :128])
+        assert torch.equal(other[sizes[0]:, 256:], clean[sizes[0]:, 256:])
