@@ -36,7 +36,8 @@ struct Divider {
     __device__ __forceinline__ bool fast() const { return scale > 8.67e-19f && scale < 1.0e30f; }
     __device__ __forceinline__ float quick(float x) const {
         const float q = x * reciprocal;
-        return fmaf(fmaf(-q, scale, x), reciprocal, q);
+        // the residual's negative, so that what is exact leaves q as it is: -0 stays -0
+        return fmaf(-fmaf(q, scale, -x), reciprocal, q);
     }
 };
 __device__ __forceinline__ Divider divide_by(float scale) { return {scale, 1.0f / scale}; }

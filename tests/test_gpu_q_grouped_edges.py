@@ -193,3 +193,28 @@ def test_scales_of_any_kind():
         assert not other[sizes[0]:, 128:256].isfinite().any()
         assert torch.equal(other[sizes[0]:, :128], clean[sizes[0]:, :128])
         assert torch.equal(other[sizes[0]:, 256:], clean[sizes[0]:, 256:])
+
+
+@pytest.mark.parametrize("to", [torch.float8_e4m3fn, torch.float8_e5m2], ids=["e4m3", "e5m2"])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+def test_quantize_keeps_the_sign_of_zero(dtype, to):
+    """Zeros of either sign, and values so small that they round to one, next to ordinary values and in a block of zeros."""
+    import blksprs_b200 as bs
+    from test_gpu_p_grouped_matmul import LARGEST, blocked, plain_quantize, plain_scale
+    gen = torch.Generator().manual_seed(41)
+    x = torch.randn((128, 384), generator=gen)
+    x[torch.rand(x.shape, generator=gen) < 0.2] = 0.0
+    x[torch.rand(x.shape, generator=gen) < 0.2] *= 2.0 ** -14
+    x[:, 256:] = 0.0
+    x = torch.where(torch.rand(x.shape, generator=gen) < 0.5, -x.abs(), x.abs()).to(dtype).to(DEV)
+    q, scale = bs.ops.quantize_rows(x, to)
+    want = plain_scale(x.float().reshape(128, 3, 128).abs().amax(2), to)
+    assert torch.equal(scale, want)
+    codes = q.view(torch.uint8)
+    assert torch.equal(codes, plain_quantize(x, LARGEST[to], blocked(want, (1,)), to).view(torch.uint8))
+    assert int((codes == 0x80).sum()) > 1000 and int((codes == 0).sum()) > 1000
+    want = plain_scale(x.float().reshape(1, 128, 3, 128).abs().amax((1, 3)), to).reshape(1, 1, 3)
+    codes = plain_quantize(x[None], LARGEST[to], blocked(want, (1, 2)), to)
+    for w in (x[None], x.t().contiguous().t()[None]):
+        q, scale = bs.ops.quantize_blocks(w, to)
+        assert torch.equal(scale, want) and torch.equal(q.contiguous().view(torch.uint8), codes.view(torch.uint8))
