@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from .. import _cabi
 from ..plan import status_word
@@ -39,6 +40,17 @@ def check_device(*tensors: Tensor) -> None:
         raise ValueError("Tensors must be on GPU")
     if any(t.device != tensors[0].device for t in tensors[1:]):
         raise ValueError("Tensors must be on same device")
+
+
+def forward_mode() -> bool:
+    """Whether a forward-mode level is open (one attribute; a torch without it looks at the tensors every time)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
+def check_no_tangents(*tensors: Tensor) -> None:
+    """A tangent would be lost without a word: a dual tensor need not require a gradient."""
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("Forward-mode gradients are not supported")
 
 
 def _copied(t: Tensor, in_backward: bool = False) -> Tensor:
@@ -181,6 +193,8 @@ class _GroupedMatmul(torch.autograd.Function):
     @plain_dispatch
     def backward(ctx, grad_output: Tensor):
         x, w, group_offsets = ctx.saved_tensors
+        if forward_mode():
+            check_no_tangents(grad_output)
         if grad_output.dtype != x.dtype:
             grad_output = grad_output.to(x.dtype)
         grad_x = grad_w = None
@@ -198,6 +212,8 @@ class _GroupedMatmul(torch.autograd.Function):
 def _grouped_matmul_eager(x, w, group_offsets):
     if torch.is_autocast_enabled():
         x, w = cast_for_autocast(x, w)
+    if forward_mode():
+        check_no_tangents(x, w)
     _validate(x, w, group_offsets)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         return _GroupedMatmul.apply(x, w, group_offsets)
@@ -214,7 +230,7 @@ def grouped_matmul(x: Tensor, w: Tensor, group_offsets: Tensor) -> Tensor:
 
     ``out[t] = x[t] @ w[e]`` for ``group_offsets[e] <= t < group_offsets[e + 1]``; rows of no group (before the
     first offset, behind the last) are zero, and so are their gradients and the gradient of a group without rows.
-    Sums run in float32 and are rounded once.
+    Sums run in float32 and are rounded once. Forward-mode gradients are refused.
 
     Args:
         x (Tensor): The rows ``(T, K)``, sorted by group, float16 or bfloat16. ``K`` is a multiple of 8.
@@ -277,6 +293,8 @@ def _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype) -> None:
 
 
 def _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtype):
+    if forward_mode():
+        check_no_tangents(x, scale_x, w, scale_w)
     _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype)
     rows, depth = x.shape
     groups, _, cols = w.shape

@@ -12,7 +12,7 @@ from torch import Tensor
 from .. import _cabi
 from ..utils.tools import plain_dispatch
 from ..utils.validation import contiguous_enabled
-from .grouped_matmul import SCALE_BLOCK, check_device, check_dimensions
+from .grouped_matmul import SCALE_BLOCK, check_device, check_dimensions, check_no_tangents, forward_mode
 
 
 def _validate(t: Tensor, dtype: torch.dtype, dims: int) -> None:
@@ -23,6 +23,8 @@ def _validate(t: Tensor, dtype: torch.dtype, dims: int) -> None:
         raise ValueError("Tensor must have either float16, bfloat16, or float32 dtype")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("Rounding to 8 bits has no gradient")
+    if forward_mode():
+        check_no_tangents(t)
     check_device(t)
 
 

@@ -218,3 +218,17 @@ def test_quantize_keeps_the_sign_of_zero(dtype, to):
     for w in (x[None], x.t().contiguous().t()[None]):
         q, scale = bs.ops.quantize_blocks(w, to)
         assert torch.equal(scale, want) and torch.equal(q.contiguous().view(torch.uint8), codes.view(torch.uint8))
+
+
+def test_a_tangent_of_the_output_s_gradient_is_refused():
+    import blksprs_b200 as bs
+    from torch.autograd import forward_ad
+    gen = torch.Generator().manual_seed(3)
+    x, w, grad = whole(20, 32, gen=gen), whole(2, 32, 40, gen=gen), whole(20, 40, gen=gen)
+    offsets = bounds_of([11, 9]).to(DEV)
+    want = torch.autograd.grad(bs.ops.grouped_matmul(x.requires_grad_(True), w, offsets), x, grad)[0]
+    with forward_ad.dual_level():
+        assert torch.equal(torch.autograd.grad(bs.ops.grouped_matmul(x, w, offsets), x, grad)[0], want)
+        out = bs.ops.grouped_matmul(x, w, offsets)
+        with pytest.raises(ValueError, match="Forward-mode"):
+            torch.autograd.grad(out, x, forward_ad.make_dual(grad, torch.ones_like(grad)))
