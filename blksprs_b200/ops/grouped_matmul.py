@@ -220,6 +220,49 @@ def _grouped_matmul_eager(x, w, group_offsets):
     return _rows_product(x, w, group_offsets)
 
 
+# What a compiled caller calls: the same launches as registered ops, so that they stay inside its graph.  In the backward
+# pass the operands are copied where they have to be, whatever the switch for inputs says.
+
+@torch.library.custom_op("blksprs_b200::grouped_matmul", mutates_args=(), device_types="cuda")
+def _registered_product(x: Tensor, w: Tensor, group_offsets: Tensor, in_backward: bool = False) -> Tensor:
+    _validate(x, w, group_offsets)
+    return _rows_product(x, w, group_offsets, in_backward)
+
+
+@_registered_product.register_fake
+def _(x, w, group_offsets, in_backward=False):
+    return x.new_empty((x.size(0), w.size(2)))
+
+
+@torch.library.custom_op("blksprs_b200::grouped_weight_gradient", mutates_args=(), device_types="cuda")
+def _registered_weight_gradient(x: Tensor, grad: Tensor, group_offsets: Tensor) -> Tensor:
+    return _weight_gradient(x, grad, group_offsets, group_offsets.size(0) - 1)
+
+
+@_registered_weight_gradient.register_fake
+def _(x, grad, group_offsets):
+    return x.new_empty((group_offsets.size(0) - 1, x.size(1), grad.size(1)))
+
+
+def _registered_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:3])
+
+
+def _registered_backward(ctx, grad_output):
+    x, w, group_offsets = ctx.saved_tensors
+    grad_x = grad_w = None
+    if ctx.needs_input_grad[0]:
+        grad_x = _registered_product(grad_output, w.transpose(1, 2), group_offsets, True)
+    if ctx.needs_input_grad[1]:
+        if w.stride(1) == 1 and w.stride(2) != 1:
+            grad_w = _registered_weight_gradient(grad_output, x, group_offsets).transpose(1, 2)
+        else:
+            grad_w = _registered_weight_gradient(x, grad_output, group_offsets)
+    return grad_x, grad_w, None, None
+
+
+_registered_product.register_autograd(_registered_backward, setup_context=_registered_setup)
+
 _PLAIN = (Tensor, torch.nn.Parameter)
 _grouped_matmul_plain = plain_dispatch(_grouped_matmul_eager)
 _grouped_matmul_no_compile = torch.compiler.disable(_grouped_matmul_plain)
@@ -244,7 +287,11 @@ def grouped_matmul(x: Tensor, w: Tensor, group_offsets: Tensor) -> Tensor:
         Tensor: The products ``(T, N)``.
     """
     if torch.compiler.is_compiling():
-        return _grouped_matmul_no_compile(x, w, group_offsets)
+        if type(x) not in _PLAIN or type(w) not in _PLAIN:
+            return _grouped_matmul_no_compile(x, w, group_offsets)
+        if torch.is_autocast_enabled():
+            x, w = cast_for_autocast(x, w)
+        return _registered_product(x, w, group_offsets)
     # only other tensor subclasses need their dispatch switched off
     impl = _grouped_matmul_eager if type(x) in _PLAIN and type(w) in _PLAIN else _grouped_matmul_plain
     return impl(x, w, group_offsets)
@@ -296,6 +343,10 @@ def _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtyp
     if forward_mode():
         check_no_tangents(x, scale_x, w, scale_w)
     _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype)
+    return _scaled_product(x, scale_x, w, scale_w, group_offsets, out_dtype)
+
+
+def _scaled_product(x, scale_x, w, scale_w, group_offsets, out_dtype):
     rows, depth = x.shape
     groups, _, cols = w.shape
     device = x.device
@@ -303,7 +354,7 @@ def _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtyp
         return torch.zeros((rows, cols), dtype=out_dtype, device=device)
     if _cabi.current_device() != device.index:
         with torch.cuda.device(device):
-            return _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtype)
+            return _scaled_product(x, scale_x, w, scale_w, group_offsets, out_dtype)
     ld_x = _row_stride(x, 15)
     if not ld_x:
         x, ld_x = _copied(x), depth
@@ -319,6 +370,18 @@ def _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtyp
     if status:
         _cabi.check(status, "bsp_grouped_matmul_scaled")
     return out
+
+
+@torch.library.custom_op("blksprs_b200::grouped_matmul_scaled", mutates_args=(), device_types="cuda")
+def _registered_scaled(x: Tensor, scale_x: Tensor, w: Tensor, scale_w: Tensor, group_offsets: Tensor,
+                       out_dtype: torch.dtype) -> Tensor:
+    _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype)
+    return _scaled_product(x, scale_x, w, scale_w, group_offsets, out_dtype)
+
+
+@_registered_scaled.register_fake
+def _(x, scale_x, w, scale_w, group_offsets, out_dtype):
+    return x.new_empty((x.size(0), w.size(2)), dtype=out_dtype)
 
 
 _grouped_matmul_scaled_plain = plain_dispatch(_grouped_matmul_scaled_eager)
@@ -346,6 +409,10 @@ def grouped_matmul_scaled(x: Tensor, scale_x: Tensor, w: Tensor, scale_w: Tensor
         Tensor: The products ``(T, N)``; rows of no group are zero.
     """
     if torch.compiler.is_compiling():
-        return _grouped_matmul_scaled_no_compile(x, scale_x, w, scale_w, group_offsets, out_dtype)
+        if type(x) is not Tensor or type(w) not in _PLAIN or (
+                torch.is_grad_enabled() and (scale_x.requires_grad or scale_w.requires_grad or x.requires_grad
+                                             or w.requires_grad)):
+            return _grouped_matmul_scaled_no_compile(x, scale_x, w, scale_w, group_offsets, out_dtype)
+        return _registered_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype)
     impl = _grouped_matmul_scaled_eager if type(x) is Tensor and type(w) in _PLAIN else _grouped_matmul_scaled_plain
     return impl(x, scale_x, w, scale_w, group_offsets, out_dtype)

@@ -63,9 +63,42 @@ def _quantize_blocks_eager(w: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tenso
     return q, scale
 
 
-_quantize_rows_plain, _quantize_blocks_plain = plain_dispatch(_quantize_rows_eager), plain_dispatch(_quantize_blocks_eager)
+# What a compiled caller calls, so that the rounding stays inside its graph.
+
+@torch.library.custom_op("blksprs_b200::quantize_rows", mutates_args=(), device_types="cuda")
+def _registered_rows(x: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    return _quantize_rows_eager(x, dtype)
+
+
+@_registered_rows.register_fake
+def _(x, dtype):
+    return (x.new_empty((x.size(0), x.size(1)), dtype=dtype),
+            x.new_empty((x.size(0), (x.size(1) + SCALE_BLOCK - 1) // SCALE_BLOCK), dtype=torch.float32))
+
+
+@torch.library.custom_op("blksprs_b200::quantize_blocks", mutates_args=(), device_types="cuda")
+def _registered_blocks(w: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    """The matrices as they are stored: (groups, columns, depth)."""
+    q, scale = _quantize_blocks_eager(w, dtype)
+    return q.transpose(1, 2), scale
+
+
+@_registered_blocks.register_fake
+def _(w, dtype):
+    return (w.new_empty((w.size(0), w.size(2), w.size(1)), dtype=dtype),
+            w.new_empty((w.size(0), (w.size(1) + SCALE_BLOCK - 1) // SCALE_BLOCK,
+                         (w.size(2) + SCALE_BLOCK - 1) // SCALE_BLOCK), dtype=torch.float32))
+
+
+_quantize_rows_plain = plain_dispatch(_quantize_rows_eager)
+_quantize_blocks_plain = plain_dispatch(_quantize_blocks_eager)
 _quantize_rows_no_compile = torch.compiler.disable(_quantize_rows_plain)
 _quantize_blocks_no_compile = torch.compiler.disable(_quantize_blocks_plain)
+
+
+def _in_graph(t: Tensor) -> bool:
+    """Whether a compiled call becomes part of the caller's graph; others break it (and are refused where they have to be)."""
+    return type(t) in (Tensor, torch.nn.Parameter) and not (t.requires_grad and torch.is_grad_enabled())
 
 
 def quantize_rows(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[Tensor, Tensor]:
@@ -79,7 +112,7 @@ def quantize_rows(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[
         tuple[Tensor, Tensor]: The rounded rows ``(T, K)`` and the scales, float32 ``(T, ceil(K / 128))``.
     """
     if torch.compiler.is_compiling():
-        return _quantize_rows_no_compile(x, dtype)
+        return (_registered_rows if _in_graph(x) else _quantize_rows_no_compile)(x, dtype)
     return (_quantize_rows_eager if type(x) is Tensor else _quantize_rows_plain)(x, dtype)
 
 
@@ -96,5 +129,8 @@ def quantize_blocks(w: Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tupl
         ``grouped_matmul_scaled`` reads them, and the scales, float32 ``(E, ceil(K / 128), ceil(N / 128))``.
     """
     if torch.compiler.is_compiling():
-        return _quantize_blocks_no_compile(w, dtype)
+        if not _in_graph(w):
+            return _quantize_blocks_no_compile(w, dtype)
+        q, scale = _registered_blocks(w, dtype)
+        return q.transpose(1, 2), scale
     return (_quantize_blocks_eager if type(w) is Tensor else _quantize_blocks_plain)(w, dtype)

@@ -232,3 +232,83 @@ def test_a_tangent_of_the_output_s_gradient_is_refused():
         out = bs.ops.grouped_matmul(x, w, offsets)
         with pytest.raises(ValueError, match="Forward-mode"):
             torch.autograd.grad(out, x, forward_ad.make_dual(grad, torch.ones_like(grad)))
+
+
+def test_registered_operators():
+    """Schemas, fake implementations and autograd of the operators a compiled caller calls."""
+    import blksprs_b200  # noqa: F401
+    ops = torch.ops.blksprs_b200
+    gen = torch.Generator().manual_seed(4)
+    x, w, grad, offsets = whole(20, 32, gen=gen), whole(2, 32, 40, gen=gen), whole(20, 40, gen=gen), bounds_of([11, 9]).to(DEV)
+    f8 = torch.float8_e4m3fn
+    wq, sw = ops.quantize_blocks(w, f8)
+    xq, sx = ops.quantize_rows(x, f8)
+    checks = ("test_schema", "test_autograd_registration", "test_faketensor")
+    for stored in (w, w.transpose(1, 2).contiguous().transpose(1, 2)):
+        torch.library.opcheck(ops.grouped_matmul.default, (x.clone().requires_grad_(), stored.clone().requires_grad_(), offsets),
+                              test_utils=(*checks, "test_aot_dispatch_static"))
+    torch.library.opcheck(ops.grouped_weight_gradient.default, (x, grad, offsets), test_utils=checks)
+    checks = checks[1:]          # the schema's check multiplies what it is given and gets, which torch cannot in 8 bits
+    torch.library.opcheck(ops.quantize_rows.default, (x, f8), test_utils=checks)
+    torch.library.opcheck(ops.quantize_blocks.default, (w, f8), test_utils=checks)
+    torch.library.opcheck(ops.grouped_matmul_scaled.default, (xq, sx, wq.transpose(1, 2), sw, offsets, BF16), test_utils=checks)
+
+
+@pytest.mark.parametrize("stored", ["kn", "nk"])
+def test_compiled_layer_of_experts_without_a_graph_break(stored):
+    """Two products with an activation between, compiled whole: outputs and gradients of whole numbers equal the eager
+    ones, for several numbers of rows, under autocast, and with a broadcast gradient."""
+    import blksprs_b200 as bs
+    gen = torch.Generator().manual_seed(5)
+    up, down = whole(3, 32, 40, gen=gen), whole(3, 40, 24, gen=gen)
+    if stored == "nk":
+        up, down = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (up, down))
+
+    def layer(x, up, down, offsets):
+        hidden = torch.relu(bs.ops.grouped_matmul(x, up, offsets))
+        return bs.ops.grouped_matmul(hidden * 2, down, offsets)
+
+    compiled = torch.compile(layer, fullgraph=True)
+    for rows in (16, 23, 300):
+        x = whole(rows, 32, gen=gen)
+        offsets = bounds_of([5, 0, rows - 7], 1).to(DEV)
+        results = []
+        for f in (compiled, layer):
+            leaves = [t.clone().requires_grad_(True) for t in (x, up, down)]
+            assert leaves[1].stride() == up.stride()
+            out = f(*leaves, offsets)
+            out.sum().backward()
+            results.append([out.detach(), *(t.grad for t in leaves)])
+        for got, want in zip(*results):
+            assert got.dtype == want.dtype and torch.equal(got, want)
+    with torch.autocast("cuda", dtype=BF16):
+        args = (x.float(), up.float(), down.float(), offsets)
+        got, want = compiled(*args), layer(*args)
+    assert got.dtype == BF16 and torch.equal(got, want)
+
+
+def test_compiled_serving_without_a_graph_break():
+    import blksprs_b200 as bs
+    from test_gpu_p_grouped_matmul import make
+    x, w, _, offsets = make([10, 0, 61], 144, 136, BF16, seed=1, behind=3)
+
+    def serve(x, wq, sw, offsets):
+        xq, sx = bs.ops.quantize_rows(x)
+        return bs.ops.grouped_matmul_scaled(xq, sx, wq, sw, offsets, out_dtype=FP32)
+
+    def prepare(w):
+        return bs.ops.quantize_blocks(w, torch.float8_e5m2)
+
+    want_q, want_s = prepare(w)
+    got_q, got_s = torch.compile(prepare, fullgraph=True)(w)
+    assert got_q.stride() == want_q.stride() and torch.equal(got_s, want_s)
+    assert torch.equal(got_q.transpose(1, 2).view(torch.uint8), want_q.transpose(1, 2).view(torch.uint8))
+    compiled = torch.compile(serve, fullgraph=True)
+    for part in (x, x[:40]):
+        bounds = offsets.clamp(max=part.shape[0])
+        assert torch.equal(compiled(part, want_q, want_s, bounds), serve(part, want_q, want_s, bounds))
+    # what is refused without a compiler is refused with one
+    for f, bad in ((lambda t: bs.ops.quantize_rows(t), x.float().requires_grad_(True)),
+                   (lambda t: bs.ops.grouped_matmul(t, w, offsets), x[:, :136])):
+        with pytest.raises(Exception, match="no gradient|Inner dimensions"):
+            torch.compile(f)(bad)
