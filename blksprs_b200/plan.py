@@ -359,7 +359,15 @@ def status_word(device: torch.device) -> Tensor:
             device = torch.device("cuda", torch.cuda.current_device())
         word = _status_words.get(device)
         if word is None:
-            word = torch.zeros(1, dtype=torch.int32, device=device)
+            if torch.cuda.is_current_stream_capturing():
+                # it would lie in the graph's memory, and every replay would clear what other kernels recorded
+                raise RuntimeError("Nothing has run on this device yet: call the operator once before recording it into "
+                                   "a CUDA graph")
+            # an ordinary tensor also when the first call is made in inference mode: it is cleared outside of it
+            with torch.inference_mode(False):
+                word = torch.zeros(1, dtype=torch.int32, device=device)
+            # kernels of other streams may be the next to write it
+            torch.cuda.current_stream(device).synchronize()
             _status_words[device] = word
     return word
 

@@ -312,3 +312,45 @@ def test_compiled_serving_without_a_graph_break():
                    (lambda t: bs.ops.grouped_matmul(t, w, offsets), x[:, :136])):
         with pytest.raises(Exception, match="no gradient|Inner dimensions"):
             torch.compile(f)(bad)
+
+
+def test_first_call_of_a_device_in_inference_mode(monkeypatch):
+    """What it records is reported, and cleared, outside that mode."""
+    import blksprs_b200 as bs
+    from blksprs_b200 import _cabi, plan
+    gen = torch.Generator().manual_seed(6)
+    x, w = whole(20, 32, gen=gen), whole(2, 32, 40, gen=gen)
+    monkeypatch.setattr(plan, "_status_words", {})
+    with torch.inference_mode():
+        bs.ops.grouped_matmul(x, w, bounds_of([11, 30]).to(DEV))
+    with pytest.raises(_cabi.NativeError, match="range"):
+        plan.check_device_status()
+    plan.check_device_status()
+
+
+def test_first_call_of_a_device_in_a_recording(monkeypatch):
+    """Refused: the status word would lie in the graph's memory.  After a call outside it, replays neither clear nor lose
+    what is recorded."""
+    import blksprs_b200 as bs
+    from blksprs_b200 import _cabi, plan
+    gen = torch.Generator().manual_seed(6)
+    x, w, offsets = whole(20, 32, gen=gen), whole(2, 32, 40, gen=gen), bounds_of([11, 9]).to(DEV)
+    want = bs.ops.grouped_matmul(x, w, offsets)
+    monkeypatch.setattr(plan, "_status_words", {})
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="once before recording"):
+            bs.ops.grouped_matmul(x, w, offsets)
+    bs.ops.grouped_matmul(x, w, offsets)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = bs.ops.grouped_matmul(x, w, offsets)
+    bs.ops.grouped_matmul(x, w, bounds_of([11, 30]).to(DEV))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    with pytest.raises(_cabi.NativeError, match="range"):
+        plan.check_device_status()
+    graph.replay()
+    plan.check_device_status()
