@@ -277,7 +277,10 @@ int launch_rows(const void* x, int64_t ld, int64_t rows, int64_t width, void* q,
     int64_t ctas = ceil_div(total, 32);
     const int sms = umma::num_sms();
     if (sms <= 0) return BSP_ERR_CUDA;
-    if (ctas > sms * 3) ctas = sms * 3;       // what is resident at once (37 us; 24 per SM in waves: 44 us)
+    // what is resident at once, as the kernel's launch bounds have it (16384 x 4096 bf16: 37 us, 24 per SM in waves 44; fp32:
+    // 54 us, with three per SM, of which one waits for the others' end, 64)
+    const int resident = sizeof(T) == 2 ? 3 : 2;
+    if (ctas > sms * resident) ctas = sms * resident;
     // 16-byte loads and stores need every row to start on such a boundary
     const bool vec = (ld * (int64_t)sizeof(T)) % 16 == 0 && width % 16 == 0 &&
                      (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
