@@ -354,3 +354,136 @@ def test_first_call_of_a_device_in_a_recording(monkeypatch):
         plan.check_device_status()
     graph.replay()
     plan.check_device_status()
+
+
+def bad_bounds(good):
+    """Bounds that decrease, start below 0, pass the rows' end, or hold anything; and what they are taken for."""
+    rows, n = int(good[-1]), good.numel()
+    low, high = torch.iinfo(good.dtype).min, torch.iinfo(good.dtype).max
+    wild = good.clone()
+    wild[::2] = torch.tensor([high, low, 7, -1, rows + 1])[torch.arange(wild[::2].numel()) % 5].to(good.dtype)
+    swapped, below, beyond = good.flip(0), good.clone(), good.clone()
+    if n > 3:
+        swapped = good.clone()
+        swapped[1], swapped[2] = good[2], good[1]
+    below[0], beyond[-1] = -3, rows + 1
+    for bad in (wild, swapped, below, beyond):
+        yield bad, bad.long().clamp(0, rows).cummax(0).values.to(good.dtype)
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=["int32", "int64"])
+@pytest.mark.parametrize("what,sizes,depth,cols", [
+    ("few", [10, 20, 30], 64, 72), ("rows", [300, 257, 611, 1, 400], 136, 264), ("tall", [800] * 6, 72, 13320),
+    ("gradient", [300, 257, 611, 1, 400], 136, 264), ("gradient", [500] * 8, 2048, 2568), ("gradient", [2500, 3000], 264, 136),
+    ("gradient", [9000], 72, 72), ("scaled", [300, 257, 611, 1, 400], 144, 264), ("scaled", [10, 20, 30], 1040, 72)],
+    ids=str)
+def test_bad_bounds_in_every_kernel(what, sizes, depth, cols, index):
+    """Clamped on the device before use, reported, and computed as the bounds they are taken for."""
+    import blksprs_b200 as bs
+    from blksprs_b200 import _cabi
+    from blksprs_b200.plan import check_device_status
+    gen = torch.Generator().manual_seed(depth)
+    good, rows = bounds_of(sizes, dtype=index), sum(sizes)
+    x = whole(rows, depth, gen=gen)
+    if what == "gradient":
+        grad = whole(rows, cols, gen=gen)
+
+        def call(offsets):
+            return weight_gradient(x, grad, offsets)
+    elif what == "scaled":
+        w = whole(len(sizes), cols, depth, gen=gen).to(torch.float8_e4m3fn).transpose(1, 2)
+        sx = torch.ones((rows, -(-depth // 128)), device=DEV)
+        sw = torch.ones((len(sizes), sx.shape[1], -(-cols // 128)), device=DEV)
+
+        def call(offsets):
+            return bs.ops.grouped_matmul_scaled(x.to(torch.float8_e4m3fn), sx, w, sw, offsets)
+    else:
+        w = whole(len(sizes), depth, cols, gen=gen)
+
+        def call(offsets):
+            return bs.ops.grouped_matmul(x, w, offsets)
+    call(good.to(DEV))
+    check_device_status()
+    for bad, taken in bad_bounds(good):
+        got = call(bad.to(DEV))
+        with pytest.raises(_cabi.NativeError, match="range"):
+            check_device_status()
+        assert torch.equal(got, call(taken.to(DEV)))
+        check_device_status()
+
+
+@pytest.mark.parametrize("stored", ["kn", "nk"])
+@pytest.mark.parametrize("sizes,depth,cols", [([300, 257, 611, 1, 400], 136, 264), ([800, 513, 385, 1, 900, 640], 200, 13320)],
+                         ids=["256", "tall"])
+def test_values_that_are_not_finite_stay_in_their_row_of_many(sizes, depth, cols, stored):
+    """The kernels of many rows: a NaN or infinity reaches its own row of the product and of the row gradient only; one in
+    the weights its own group's."""
+    import blksprs_b200 as bs
+    gen = torch.Generator().manual_seed(cols)
+    rows, at = sum(sizes) + 70, [0, 299, 300, 556, 900, sum(sizes) - 1, sum(sizes) + 3]
+    x, grad = whole(rows, depth, gen=gen), whole(rows, cols, gen=gen)
+    w = whole(len(sizes), depth, cols, gen=gen)
+    w = w if stored == "kn" else w.transpose(1, 2).contiguous().transpose(1, 2)
+    offsets = bounds_of(sizes).to(DEV)
+    keep = torch.ones(rows, dtype=torch.bool, device=DEV)
+    keep[at] = False
+
+    def both(x, w, grad):
+        x = x.detach().requires_grad_(True)
+        out = bs.ops.grouped_matmul(x, w, offsets)
+        return out.detach(), torch.autograd.grad(out, x, grad)[0]
+
+    clean = both(x, w, grad)
+    want = torch.cat([x[a:b].double() @ w[e].double() for e, (a, b) in enumerate(zip(offsets.tolist(), offsets[1:].tolist()))])
+    assert torch.equal(clean[0][:sum(sizes)].double(), want) and not clean[0][sum(sizes):].any()
+    x[at, 5], grad[at, 7] = float("nan"), float("inf")
+    for got, wanted in zip(both(x, w, grad), clean):
+        assert torch.equal(got[keep], wanted[keep])
+        assert not got[at[:-1]].isfinite().all(1).any() and not got[at[-1]].any()
+    x, grad = x.nan_to_num(0.0), grad.nan_to_num(0.0, 0.0)
+    wanted = both(x, w, grad)
+    w[1, 3, 4] = float("nan")
+    group = slice(int(offsets[1]), int(offsets[2]))
+    for got, want, column in zip(both(x, w, grad), wanted, (4, 3)):
+        assert got[group, column].isnan().all()
+        got[group, column] = want[group, column]
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("sizes,depth,cols", [([40000], 128, 264), ([5, 20011, 0, 19990], 72, 136), ([3001] * 8, 520, 2056),
+                                              ([9001, 7030], 2048, 4104)], ids=str)
+def test_every_row_of_a_long_group_counts(sizes, depth, cols, dtype):
+    """Weight gradients of long groups whose rows are zero but for a few at the ends of groups, of parts, of steps and of
+    the last sixteen: sums small enough for the output type to hold, so that a row lost or counted twice shows."""
+    gen = torch.Generator().manual_seed(depth + cols)
+    rows = sum(sizes) + 24
+    offsets = bounds_of(sizes, 8)
+    x, grad = torch.zeros((rows, depth), dtype=dtype, device=DEV), torch.zeros((rows, cols), dtype=dtype, device=DEV)
+    for a, b in zip(offsets.tolist(), offsets[1:].tolist()):
+        steps = torch.randint(0, max(1, (b - a) // 64), (8,), generator=gen) * 64 + a
+        ends = [range(a, a + 17), range(b - 66, b), *(range(s - 1, s + 2) for s in steps.tolist())]
+        at = sorted({r for part in ends for r in part if a <= r < b})
+        assert len(at) < 128
+        x[at], grad[at] = whole(len(at), depth, gen=gen, dtype=dtype), whole(len(at), cols, gen=gen, dtype=dtype)
+    x[:8], grad[:8], x[-16:], grad[-16:] = 1.0, 1.0, 1.0, 1.0          # rows of no group
+    want = plain_weight_gradient(x, grad, offsets)
+    assert want.abs().max() <= 256
+    assert torch.equal(weight_gradient(x, grad, offsets.to(DEV)).double(), want)
+
+
+@pytest.mark.parametrize("sizes,depth,cols", [([5, 0, 3], 4096, 136), ([1200, 1], 2056, 264), ([3000, 2500], 4104, 2568)], ids=str)
+def test_every_value_of_a_long_contraction_counts(sizes, depth, cols):
+    """The same of the rows product: values at the ends of its contraction, of steps and of a cluster's shares."""
+    import blksprs_b200 as bs
+    gen = torch.Generator().manual_seed(depth)
+    x, w = whole(sum(sizes), depth, gen=gen, dtype=BF16), whole(len(sizes), depth, cols, gen=gen, dtype=BF16)
+    keep = torch.zeros(depth, dtype=torch.bool)
+    for s in [0, depth, depth // 2, *(torch.randint(1, depth // 64, (12,), generator=gen) * 64).tolist()]:
+        keep[max(0, s - 4):s + 4] = True
+    x[:, ~keep.to(DEV)] = 0
+    offsets = bounds_of(sizes)
+    want = torch.cat([x[a:b].double() @ w[e].double() for e, (a, b) in enumerate(zip(offsets.tolist(), offsets[1:].tolist()))])
+    assert want.abs().max() <= 256
+    for stored in (w, w.transpose(1, 2).contiguous().transpose(1, 2)):
+        assert torch.equal(bs.ops.grouped_matmul(x, stored, offsets.to(DEV)).double(), want)
