@@ -19,7 +19,8 @@ OUT_DIR = PKG_DIR / "lib"
 LIB_PATH = OUT_DIR / "libblksprs_b200.so"
 SOURCES = ["capi.cu", "lut.cu", "plan_panel.cu", "matmul_mma.cu", "matmul_umma.cu", "conversion.cu", "softmax.cu",
            "linear.cu", "grouped.cu", "grouped_few.cu", "quantize.cu"]
-HEADERS = [CSRC / "common.cuh", CSRC / "umma_common.cuh", CSRC / "grouped_common.cuh", PKG_DIR.parent / "include" / "blksprs_b200.h"]
+HEADERS = [CSRC / "common.cuh", CSRC / "umma_common.cuh", CSRC / "grouped_common.cuh",
+           PKG_DIR.parent / "include" / "blksprs_b200.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -214,7 +214,8 @@ __device__ __forceinline__ void stage_row(uint32_t staging, const uint32_t* word
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                     ::"r"(staging + staged_at(lane, i)), "r"(words[4 * i]), "r"(words[4 * i + 1]), "r"(words[4 * i + 2]), "r"(words[4 * i + 3]) : "memory");
+                     ::"r"(staging + staged_at(lane, i)), "r"(words[4 * i]), "r"(words[4 * i + 1]), "r"(words[4 * i + 2]),
+                       "r"(words[4 * i + 3]) : "memory");
 }
 
 // ---- host side ---------------------------------------------------------------------

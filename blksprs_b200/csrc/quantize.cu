@@ -28,7 +28,9 @@ __device__ __forceinline__ float scale_of(float largest, float reciprocal_of_max
 }
 
 // value / scale, correctly rounded, for one scale and many values: with y the correctly rounded reciprocal and
-// q = x * y, the residual r = x - q * scale is exact and q + r * y rounds to the quotient (Markstein 1990).
+// q = x * y, the residual r = x - q * scale corrects q to q + r * y (Markstein 1990).  Where q is within one last place the
+// residual is exact; q can be off by one and a half, and then it may not be (about 1 % of random pairs).  The result was
+// the quotient all the same in 4e8 of them, and what it is rounded to afterwards has 2 or 3 bits.
 // That needs residuals that do not underflow: for a scale above 2^-60 a quotient of at least 2^-18 (smaller ones
 // round to zero in either type) has a residual above 2^-103.  Other scales divide.
 struct Divider {
@@ -113,8 +115,9 @@ __device__ __forceinline__ void store_tail(uint8_t* dst, uint2 v, int64_t left) 
 }
 
 // ---- rows: a scale for each 1 x 128 ----------------------------------------------------
-// 8 lanes per block, 16 neighbouring values each (37 us on 16384 x 4096 bf16, 5.4 TB/s; with 16 lanes of 8 values
-// 49 us: more shuffles and index arithmetic per value); every quarter warp takes kAhead blocks at a time, whose loads are under way together.
+// 8 lanes per block, 16 neighbouring values each (37 us on 16384 x 4096 bf16, 5.4 TB/s; fp32: 54 us, 6.2 TB/s; with 16
+// lanes of 8 values 49 us in bf16: more shuffles and index arithmetic per value); every quarter warp takes kAhead blocks at
+// a time, whose loads are under way together.
 // HBM-bound: each value once in (2 or 4 bytes) and once out (1 byte).
 constexpr int kAhead = 4;       // the lanes that divide (below) are as many
 
@@ -198,7 +201,8 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int rows, int width, i
 // ---- weights: a scale for each 128 x 128 -------------------------------------------------
 // One CTA of 256 threads per block.  Every thread holds its 64 values in registers between the two passes
 // (largest magnitude, rounding), so that the weights are read once (32 x 4096 x 2048 bf16: 137 us, 5.9 TB/s; the issue
-// slots are 79 % busy); q is stored with the depth innermost.
+// slots are 79 % busy; 16-bit weights stored depth-innermost spill 24 bytes per thread at the four CTAs per SM that fit);
+// q is stored with the depth innermost.
 // DEPTH_INNER: w is stored that way too, a thread has 8 neighbouring depths of 8 columns and writes them as they
 // are.  Otherwise it has 8 neighbouring columns of 8 neighbouring depths, and the rounded block goes through
 // shared memory: column n, 8-byte piece k at piece k ^ (n / 8 mod 16), free of bank conflicts both ways.
@@ -284,8 +288,8 @@ int launch_rows(const void* x, int64_t ld, int64_t rows, int64_t width, void* q,
     // 16-byte loads and stores need every row to start on such a boundary
     const bool vec = (ld * (int64_t)sizeof(T)) % 16 == 0 && width % 16 == 0 &&
                      (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-    if (vec) quantize_rows_kernel<T, E5M2, true><<<(unsigned)ctas, 256, 0, stream>>>((const T*)x, ld, (int)rows, (int)width, (int)blocks, (uint8_t*)q, scale);
-    else quantize_rows_kernel<T, E5M2, false><<<(unsigned)ctas, 256, 0, stream>>>((const T*)x, ld, (int)rows, (int)width, (int)blocks, (uint8_t*)q, scale);
+    auto kern = vec ? quantize_rows_kernel<T, E5M2, true> : quantize_rows_kernel<T, E5M2, false>;
+    kern<<<(unsigned)ctas, 256, 0, stream>>>((const T*)x, ld, (int)rows, (int)width, (int)blocks, (uint8_t*)q, scale);
     BSP_LAUNCH_CHECK();
     return BSP_OK;
 }
@@ -300,10 +304,8 @@ int launch_blocks(const void* w, int64_t sg, int64_t sk, int64_t sn, int64_t gro
     const int64_t size = sizeof(T), outer = depth_inner ? sn : sk;
     const bool vec = (depth_inner || sn == 1) && (reinterpret_cast<uintptr_t>(w) & 15) == 0 && outer * size % 16 == 0 &&
                      sg * size % 16 == 0;
-    if (depth_inner)
-        quantize_blocks_kernel<T, E5M2, true><<<(unsigned)total, 256, 0, stream>>>((const T*)w, sg, sk, sn, depth, cols, kb, nb, vec, (uint8_t*)q, scale);
-    else
-        quantize_blocks_kernel<T, E5M2, false><<<(unsigned)total, 256, 0, stream>>>((const T*)w, sg, sk, sn, depth, cols, kb, nb, vec, (uint8_t*)q, scale);
+    auto kern = depth_inner ? quantize_blocks_kernel<T, E5M2, true> : quantize_blocks_kernel<T, E5M2, false>;
+    kern<<<(unsigned)total, 256, 0, stream>>>((const T*)w, sg, sk, sn, depth, cols, kb, nb, vec, (uint8_t*)q, scale);
     BSP_LAUNCH_CHECK();
     return BSP_OK;
 }

@@ -1,8 +1,9 @@
 """8-bit values with a scale for each block of 128: the operands of ``grouped_matmul_scaled``.
 
 ``scale = max(largest magnitude of the block / largest value of the type, 2**-126)`` (the quotient as a product with the
-rounded reciprocal, as torch divides by a number), ``q = value / scale`` rounded to nearest even.  A block that holds an infinity or a NaN has a scale that is not finite and multiplies out to NaN;
-other blocks are not touched by it.  No counterpart in the blksprs library.
+rounded reciprocal, as torch divides by a number), ``q = value / scale`` rounded to nearest even; -0 stays -0.  A block
+that holds an infinity or a NaN has a scale that is not finite and multiplies out to NaN; other blocks are not touched by
+it.  No counterpart in the blksprs library.
 """
 from __future__ import annotations
 
