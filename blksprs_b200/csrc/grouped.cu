@@ -20,10 +20,10 @@
 //   (one for each row and each 128 features) is one register per thread.
 //
 // What it measured on a B200 (time, rate; bf16): forward, dX and dW of 8 groups of 2048 rows, 4096 x 4096:
-// 370, 375 and 376-415 us, 1486, 1466 and 1325-1462 TFLOP/s, the tensor pipe 79-83 % busy at the 1.52-1.56 GHz
+// 370, 363-375 and 376-454 us, 1486, 1466-1514 and 1210-1462 TFLOP/s, the tensor pipe 76-83 % busy at the 1.51-1.56 GHz
 // that the power cap leaves (a plain library product of 8192^3: 1404 TFLOP/s sustained, 1687 in a burst).  16
-// groups of 1024 rows, 2048 x 4096: 206 us, 1335 TFLOP/s; the same in 8 bits, 4096 x 4096: 293 us, 1876
-// TFLOP/s, tensor pipe 56 %: there the epilogue bounds, 128 multiply-adds per thread and 512 cycles of MMAs, with
+// groups of 1024 rows, 2048 x 4096: 206 us, 1335 TFLOP/s; the same in 8 bits, 4096 x 4096: 298 us, 1845
+// TFLOP/s, tensor pipe 54 %: there the epilogue bounds, 128 multiply-adds per thread and 512 cycles of MMAs, with
 // the waits around them (timed inside the kernel: 700 cycles per step).  64 groups of 64 rows, 2048 x 1024: 52
 // us, HBM 65 % busy; 64 groups of 128 rows: 55 us, 318 MB at 5.8 TB/s.
 //
@@ -843,6 +843,8 @@ int64_t most_row_tiles(int64_t rows, int64_t groups, int64_t height) {
 // pairs fewer than four tiles each, or where the mean group would not fill them (192 rows: 71 / 81 us; 64 groups of
 // 64 rows: 53 / 60 us; 33 groups of 60 rows, 1032 x 1496: 34 / 42 us).  Measured, one / two: 16 groups of 1024 rows,
 // 2048 x 4096: 215 / 213 us; weight gradient of 8 groups of 2048 rows, 4096 x 4096: 559 / 380 us.
+// With all rows in one group, which the host does not see (us, beside the same rows as a group of their own): 64 groups,
+// 2048 x 4096, 12288 rows 140 / 144; 8 groups, 4096 x 4096, 3072 rows 73 / 72.
 int tile_halves(int64_t tiles_of_two, int64_t rows, int64_t groups) {
     return tiles_of_two >= 4 * (num_sms() / 2) && rows >= 384 * (groups < rows ? groups : rows) ? 2 : 1;
 }
@@ -854,6 +856,9 @@ int tile_halves(int64_t tiles_of_two, int64_t rows, int64_t groups) {
 // 1024 rows 12.1 / 9.2, 16384 rows 106 / 15.8; 8 groups, 256 x 256, 1024 rows each 12.5 / 11.4, 4096 rows 31.8 / 15.2;
 // 4 groups, 512 x 520, 16384 rows 108 / 47.7.  Below 1024 rows the second launch costs what it saves (8 groups of 512
 // rows: 9.3 / 10.4), as it does for parts of fewer than 256.
+// The number goes by the mean of the groups.  With all rows in one of them (us, beside the even batch and the same rows as
+// a group of their own): 8 groups, 256 x 256, 8192 rows 28 / 12 / 14; 32 groups, 512 x 512, 8192 rows 59 / 12 / 15; 8 groups,
+// 2048 x 2048, 4096 rows 44 / 37 / 34.
 constexpr int64_t kRowsToSplit = 1024, kPartRows = 256, kPartCost = 13;
 int64_t gradient_parts(int64_t rows, int64_t groups, int64_t depth, int64_t cols) {
     const int64_t tiles = groups * ceil_div(depth, kTile) * ceil_div(cols, kTile), fit = num_sms() / 2 / tiles;

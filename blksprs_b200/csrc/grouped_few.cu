@@ -14,7 +14,7 @@
 //
 // What it measured on a B200: 128 rows over 32 groups, 4096 x 2048 bf16: 77 us, 521 MB
 // of weights at 6.8 TB/s (a plain copy moves 6.5); in 8 bits 45 us, 5.8 TB/s.  Two rows of two groups, 2048 x 4096 bf16
-// (33 MB): 9.1 us; one row, 4096 x 4096 in 8 bits (17 MB): 8.3 us: launch, offsets, one copy's way and the
+// (33 MB): 9.1 us; one row, 4096 x 4096 in 8 bits (17 MB): 7.8 us: launch, offsets, one copy's way and the
 // cluster's exchange are most of both.
 //
 // Warp 0 copies, warp 1 issues the MMAs and owns tensor memory, warps 2-5 are the epilogue, warp 6 stages scales.
@@ -394,7 +394,8 @@ grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
                     if (h * 32 + j < rows)
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(data + ((h * 32 + j) * kFewM + quarter * 32 + lane) * 4), "f"(sum[h][j]) : "memory");
+                        asm volatile("st.shared.f32 [%0], %1;"
+                                     ::"r"(data + ((h * 32 + j) * kFewM + quarter * 32 + lane) * 4), "f"(sum[h][j]) : "memory");
         }
         cluster_sync();
         const int pair = threadIdx.x & 63;                       // two columns of one row per thread
@@ -456,6 +457,10 @@ int launch_kernel(const CUtensorMap& weights, const CUtensorMap& rows_64, const 
 //             4, 1024 x 1024: 4: 5.7 / 8.8, 64: 8.4 / 9.4, 128: 13 / 10   1, 4096 x 4096: 64: 15 / 22, 96: 21 / 22
 //   8 bits    64, 2048 x 1024: 48: 35 / 42, 64: 44 / 43                   16, 4096 x 4096: 4: 45 / 64, 64: 68 / 75
 //             8, 2048 x 2048: 32: 14 / 15, 48: 18 / 15                    1, 4096 x 4096: 64: 14 / 18, 96: 19 / 19
+// The bounds are on the device, so the mean decides also where all rows went to one of the groups.  Such a batch, beside the
+// even one and beside the same rows as a group of their own (us): 16 bits, 64 groups, 2048 x 1024, 2048 rows: 17.8, 47.5,
+// 16.2; 16 groups, 4096 x 4096, 192 rows: 21.6, 81.2, 23.3; 8 bits, 64 groups, 2048 x 1024, 2048 rows: 19.8, 30.8, 13.6; 16
+// groups, 4096 x 4096, 768 rows: 53.4, 55.3, 22.8 (twelve row tiles read the weights, from L2).
 bool few_applies(int64_t rows, int64_t groups, int64_t cols, bool f8) {
     const int64_t hit = groups < rows ? groups : rows;
     if (rows / kFewN + hit > 65535) return false;

@@ -452,7 +452,8 @@ int bsp_grouped_weight_grad(const void* x, int64_t ld_x, const void* grad, int64
  * (group_stride_w, 1, ld_w); scales fp32 with the given element strides; out:
  * contiguous (rows, cols) of BSP_F16 / BSP_BF16 / BSP_F32.  depth is a multiple
  * of 16 (the last block of a row may be short), cols of 8.  The products of a
- * block are added up in fp32, then scaled, then added up in fp32. */
+ * block are added up in fp32, then scaled, then added up in fp32; the scales
+ * are any fp32 numbers, also where their product would not be one. */
 int bsp_grouped_matmul_scaled(const void* x, int64_t ld_x, int type_x, const float* scale_x, int64_t sx_row,
                               int64_t sx_block, const void* w, int64_t group_stride_w, int64_t ld_w, int type_w,
                               const float* scale_w, int64_t sw_group, int64_t sw_k, int64_t sw_n,
