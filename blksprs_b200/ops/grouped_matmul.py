@@ -91,13 +91,17 @@ def _group_and_outer_stride(w: Tensor, mask: int) -> tuple[int, int, bool]:
     return sg, 0, True
 
 
-def _validate_groups(x: Tensor, w: Tensor, group_offsets: Tensor, vector: int) -> None:
+def _validate_offsets(group_offsets: Tensor, groups: int) -> None:
     if group_offsets.dtype not in (torch.int32, torch.int64):
         raise ValueError("Group offsets must have either int32 or int64 dtype")
-    if group_offsets.dim() != 1 or group_offsets.size(0) != w.size(0) + 1:
+    if group_offsets.dim() != 1 or group_offsets.size(0) != groups + 1:
         raise ValueError("Group offsets must have one entry more than there are groups")
     if not group_offsets.is_contiguous():
         raise ValueError("Tensor must be contiguous")
+
+
+def _validate_groups(x: Tensor, w: Tensor, group_offsets: Tensor, vector: int) -> None:
+    _validate_offsets(group_offsets, w.size(0))
     if x.size(1) != w.size(1):
         raise ValueError("Inner dimensions of tensors must match")
     if w.size(0) > MAX_GROUPS:
@@ -124,6 +128,23 @@ def _validate(x: Tensor, w: Tensor, group_offsets: Tensor) -> None:
         raise ValueError("Tensors must have same dtype")
     _validate_groups(x, w, group_offsets, 8)
     check_device(x, w, group_offsets)
+
+
+def _validate_gradient(x: Tensor, grad: Tensor, group_offsets: Tensor) -> None:
+    check_dimensions(2, x, grad)
+    if x.dtype not in _16_BIT:
+        raise ValueError("Tensor must have either float16 or bfloat16 dtype")
+    if grad.dtype != x.dtype:
+        raise ValueError("Tensors must have same dtype")
+    if grad.size(0) != x.size(0):
+        raise ValueError("Numbers of rows must match")
+    groups = max(group_offsets.numel() - 1, 0)
+    _validate_offsets(group_offsets, groups)
+    if groups > MAX_GROUPS:
+        raise ValueError(f"Number of groups must be at most {MAX_GROUPS}")
+    if x.size(1) % 8 or grad.size(1) % 8:
+        raise ValueError("Inner dimension must be divisible by 8 and columns by 8")
+    check_device(x, grad, group_offsets)
 
 
 def _rows_product(x: Tensor, w: Tensor, group_offsets: Tensor, in_backward: bool = False) -> Tensor:
@@ -225,6 +246,8 @@ def _grouped_matmul_eager(x, w, group_offsets):
 
 @torch.library.custom_op("blksprs_b200::grouped_matmul", mutates_args=(), device_types="cuda")
 def _registered_product(x: Tensor, w: Tensor, group_offsets: Tensor, in_backward: bool = False) -> Tensor:
+    if forward_mode():
+        check_no_tangents(x, w)
     _validate(x, w, group_offsets)
     return _rows_product(x, w, group_offsets, in_backward)
 
@@ -236,6 +259,9 @@ def _(x, w, group_offsets, in_backward=False):
 
 @torch.library.custom_op("blksprs_b200::grouped_weight_gradient", mutates_args=(), device_types="cuda")
 def _registered_weight_gradient(x: Tensor, grad: Tensor, group_offsets: Tensor) -> Tensor:
+    if forward_mode():
+        check_no_tangents(x, grad)
+    _validate_gradient(x, grad, group_offsets)
     return _weight_gradient(x, grad, group_offsets, group_offsets.size(0) - 1)
 
 
@@ -287,7 +313,7 @@ def grouped_matmul(x: Tensor, w: Tensor, group_offsets: Tensor) -> Tensor:
         Tensor: The products ``(T, N)``.
     """
     if torch.compiler.is_compiling():
-        if type(x) not in _PLAIN or type(w) not in _PLAIN:
+        if type(x) not in _PLAIN or type(w) not in _PLAIN or forward_mode():
             return _grouped_matmul_no_compile(x, w, group_offsets)
         if torch.is_autocast_enabled():
             x, w = cast_for_autocast(x, w)
@@ -375,8 +401,7 @@ def _scaled_product(x, scale_x, w, scale_w, group_offsets, out_dtype):
 @torch.library.custom_op("blksprs_b200::grouped_matmul_scaled", mutates_args=(), device_types="cuda")
 def _registered_scaled(x: Tensor, scale_x: Tensor, w: Tensor, scale_w: Tensor, group_offsets: Tensor,
                        out_dtype: torch.dtype) -> Tensor:
-    _validate_scaled(x, scale_x, w, scale_w, group_offsets, out_dtype)
-    return _scaled_product(x, scale_x, w, scale_w, group_offsets, out_dtype)
+    return _grouped_matmul_scaled_eager(x, scale_x, w, scale_w, group_offsets, out_dtype)
 
 
 @_registered_scaled.register_fake
@@ -409,7 +434,7 @@ def grouped_matmul_scaled(x: Tensor, scale_x: Tensor, w: Tensor, scale_w: Tensor
         Tensor: The products ``(T, N)``; rows of no group are zero.
     """
     if torch.compiler.is_compiling():
-        if type(x) is not Tensor or type(w) not in _PLAIN or (
+        if type(x) is not Tensor or type(w) not in _PLAIN or forward_mode() or (
                 torch.is_grad_enabled() and (scale_x.requires_grad or scale_w.requires_grad or x.requires_grad
                                              or w.requires_grad)):
             return _grouped_matmul_scaled_no_compile(x, scale_x, w, scale_w, group_offsets, out_dtype)

@@ -99,7 +99,8 @@ _quantize_blocks_no_compile = torch.compiler.disable(_quantize_blocks_plain)
 
 def _in_graph(t: Tensor) -> bool:
     """Whether a compiled call becomes part of the caller's graph; others break it (and are refused where they have to be)."""
-    return type(t) in (Tensor, torch.nn.Parameter) and not (t.requires_grad and torch.is_grad_enabled())
+    return (type(t) in (Tensor, torch.nn.Parameter) and not (t.requires_grad and torch.is_grad_enabled())
+            and not forward_mode())
 
 
 def quantize_rows(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[Tensor, Tensor]:

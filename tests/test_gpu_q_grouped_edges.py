@@ -487,3 +487,39 @@ def test_every_value_of_a_long_contraction_counts(sizes, depth, cols):
     assert want.abs().max() <= 256
     for stored in (w, w.transpose(1, 2).contiguous().transpose(1, 2)):
         assert torch.equal(bs.ops.grouped_matmul(x, stored, offsets.to(DEV)).double(), want)
+
+
+def test_registered_weight_gradient_refuses_what_would_be_read_out_of_bounds():
+    import blksprs_b200  # noqa: F401
+    op = torch.ops.blksprs_b200.grouped_weight_gradient
+    x, grad, offsets = (torch.zeros(s, dtype=BF16, device=DEV) for s in ((20, 32), (20, 40), (3,)))
+    offsets = offsets.int()
+    assert op(x, grad, offsets).shape == (2, 32, 40)
+    for bad, message in (((x, grad[:10], offsets), "rows"), ((x[0], grad, offsets), "2 dimensions"),
+                         ((x, grad.half(), offsets), "same dtype"), ((x.float(), grad.float(), offsets), "float16 or"),
+                         ((x, grad[:, :36], offsets), "divisible"), ((x[:, :28], grad, offsets), "divisible"),
+                         ((x, grad, offsets.float()), "int32 or int64"), ((x, grad, offsets[:0]), "one entry more"),
+                         ((x, grad, offsets[None]), "one entry more"), ((x, grad, offsets.repeat(2)[::2]), "contiguous"),
+                         ((x, grad, offsets.cpu()), "same device"), ((x, grad, offsets.repeat(342)), "at most 1024")):
+        with pytest.raises(ValueError, match=message):
+            op(*bad)
+
+
+def test_tangents_of_registered_and_compiled_calls_are_refused():
+    import blksprs_b200 as bs
+    from torch.autograd import forward_ad
+    gen = torch.Generator().manual_seed(3)
+    x, w, offsets = whole(20, 32, gen=gen), whole(2, 32, 40, gen=gen), bounds_of([11, 9]).to(DEV)
+    wq, sw = bs.ops.quantize_blocks(w)
+    xq, sx = bs.ops.quantize_rows(x)
+    ops = torch.ops.blksprs_b200
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        ds = forward_ad.make_dual(sx, torch.ones_like(sx))
+        for f in (lambda: ops.grouped_matmul(d, w, offsets), lambda: ops.grouped_weight_gradient(x, d, offsets),
+                  lambda: ops.quantize_rows(d, torch.float8_e4m3fn),
+                  lambda: ops.grouped_matmul_scaled(xq, ds, wq, sw, offsets, BF16),
+                  lambda: torch.compile(lambda t: bs.ops.grouped_matmul(t, w, offsets), backend="eager")(d),
+                  lambda: torch.compile(lambda t: bs.ops.quantize_rows(t), backend="eager")(d)):
+            with pytest.raises(ValueError, match="Forward-mode"):
+                f()
